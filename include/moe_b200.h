@@ -319,6 +319,33 @@ int moe_ep_barrier(int64_t* const* flags, int32_t rank, int32_t world, int64_t* 
 int moe_ep_put_counts(const int32_t* counts, int32_t num_experts, int32_t* const* bases,
                       int32_t rank, int32_t world, void* stream);
 
+/* A whole SwiGLU mixture-of-experts layer for a few tokens (the serving form of the layer the
+ * reference assembles from its ops, tests/test_moe.py:68-87; no single reference call):
+ *   l[t] = x[t] . w_router^T + router_bias     (fp32, not rounded to dtype)
+ *   idx  = the K largest l[t] (ties to the lower expert), p = softmax over them
+ *   out[t] = sum_k p[t,k] * ((silu(x[t] . w_gate[idx]^T) * (x[t] . w_up[idx]^T)) . w_down[idx]^T)
+ * x [T, d], w_router [E, d], w_gate / w_up [E, H, d], w_down [E, d, H], out [T, d] of dtype;
+ * router_bias [E] fp32 or NULL.  An expert whose logit is -inf is masked: its slot weighs 0
+ * and its weights are not read; a token with no unmasked expert gets zeros.  T <= 128,
+ * K <= min(E, 16), E <= 1024.  The result does not depend on the order blocks run in.
+ * Workspace: moe_few_tokens_workspace_bytes(...) bytes, 16-byte aligned, not shared with a
+ * call that may run at the same time. */
+size_t moe_few_tokens_workspace_bytes(int64_t num_tokens, int64_t d, int64_t hidden,
+                                      int32_t num_experts, int32_t topk, int dtype);
+int moe_few_tokens_fwd(const void* x, const void* w_router, const float* router_bias,
+                       const void* w_gate, const void* w_up, const void* w_down, int dtype,
+                       int64_t num_tokens, int64_t d, int64_t hidden, int32_t num_experts,
+                       int32_t topk, void* out, void* workspace, size_t workspace_bytes,
+                       void* stream);
+/* The same with the routing given: weights [T, K] fp32, indices [T, K] int32 (an expert may
+ * appear more than once for a token; an index outside [0, E) is dropped and sets device
+ * error 2). */
+int moe_few_experts_fwd(const void* x, const float* weights, const int32_t* indices,
+                        const void* w_gate, const void* w_up, const void* w_down, int dtype,
+                        int64_t num_tokens, int64_t d, int64_t hidden, int32_t num_experts,
+                        int32_t topk, void* out, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,6 +15,8 @@ libmoe_b200.so through its C ABI (include/moe_b200.h):
 Beyond the reference: grouped_gemm_swiglu / grouped_swiglu_mlp (the SwiGLU expert MLP in
 fused launches), permute_with_capacity (token dropping at a per-expert capacity), and
 permute_index + grouped_swiglu_mlp_gathered (the permute fused into the expert GEMMs).
+For serving: moe_few_tokens (the whole layer for up to 128 tokens) and moe_few_experts (the
+same with the routing given).
 
 Layout conventions (same as the reference):
     A:        [total_tokens, K]   (all experts stacked along rows)
@@ -29,6 +31,7 @@ from .unpermute_ops import unpermute, unpermute_forward, unpermute_backward
 from .fused_topk_softmax_ops import fused_topk_softmax
 from .gate_up_ops import grouped_gemm_swiglu, grouped_swiglu_mlp
 from .fused_permute_ops import grouped_swiglu_mlp_gathered, permute_index
+from .few_token_ops import moe_few_experts, moe_few_tokens
 
 __all__ = [
     "grouped_gemm",
@@ -46,4 +49,7 @@ __all__ = [
     "permute_index",
     "grouped_swiglu_mlp_gathered",
     "grouped_swiglu_mlp",
+    # serving: the whole layer for a few tokens
+    "moe_few_tokens",
+    "moe_few_experts",
 ]

@@ -1,0 +1,178 @@
+// Host side of the few-token mixture-of-experts layer (few_tokens.cuh): argument checks,
+// workspace layout and launches.  Included by moe_b200.cu, whose helpers it uses.
+#pragma once
+
+#include "few_tokens.cuh"
+
+namespace moe {
+
+struct FewArgs {
+  const void* x;
+  const void* w_router;        // NULL: weights / indices are given
+  const float* router_bias;
+  const float* weights;
+  const int32_t* indices;
+  const void* w_gate;
+  const void* w_up;
+  const void* w_down;
+  int64_t num_tokens, d, hidden;
+  int32_t E, topk;
+  int dtype;
+  void* out;
+  void* workspace;
+  size_t workspace_bytes;
+  cudaStream_t stream;
+};
+
+static size_t align256(size_t v) { return (v + 255) / 256 * 256; }
+
+// Workspace: logits [T, E] fp32, then h [T*K, H] (fp32).
+struct FewWorkspace {
+  size_t logits, h, total;
+};
+static FewWorkspace few_workspace(int64_t T, int64_t H, int64_t E, int64_t K) {
+  FewWorkspace w;
+  w.logits = 0;
+  w.h = align256((size_t)T * E * 4);
+  w.total = w.h + align256((size_t)T * K * H * 4);
+  return w;
+}
+
+static int check_few(const FewArgs& a) {
+  MOE_REQUIRE(dtype_ok(a.dtype), "few_tokens: bad dtype %d", a.dtype);
+  MOE_REQUIRE(a.num_tokens >= 0 && a.num_tokens <= few::kMaxTokens,
+              "few_tokens: num_tokens must be in [0, %d] (got %lld)", few::kMaxTokens,
+              (long long)a.num_tokens);
+  MOE_REQUIRE(a.E > 0 && a.E <= few::kMaxExperts, "few_tokens: need 0 < E <= %d (E=%d)",
+              few::kMaxExperts, a.E);
+  MOE_REQUIRE(a.topk > 0 && a.topk <= few::kMaxTopk && (a.topk <= a.E || !a.w_router),
+              "few_tokens: need 0 < K <= min(E, %d) (E=%d, K=%d)", few::kMaxTopk, a.E, a.topk);
+  MOE_REQUIRE(a.d >= 0 && a.hidden >= 0 && a.d < (1ll << 30) && a.hidden < (1ll << 30),
+              "few_tokens: bad sizes d=%lld H=%lld", (long long)a.d, (long long)a.hidden);
+  if (a.num_tokens == 0 || a.d == 0) return MOE_OK;
+  MOE_REQUIRE(a.x && a.out && (a.hidden == 0 || (a.w_gate && a.w_up && a.w_down)),
+              "few_tokens: NULL operand");
+  MOE_REQUIRE(a.w_router || (a.weights && a.indices), "few_tokens: NULL routing");
+  const FewWorkspace w = few_workspace(a.num_tokens, a.hidden, a.E, a.topk);
+  if (!a.workspace || a.workspace_bytes < w.total)
+    return set_error(MOE_ERR_WORKSPACE, "few_tokens: workspace has %zu bytes, needs %zu",
+                     a.workspace ? a.workspace_bytes : (size_t)0, w.total);
+  MOE_REQUIRE(aligned16(a.workspace), "few_tokens: workspace must be 16-byte aligned");
+  return MOE_OK;
+}
+
+template <typename T>
+static int few_router_launch(const FewArgs& a, float* logits, int* zero, int num_zero) {
+  const bool vec = (a.d * sizeof(T)) % 16 == 0 && aligned16(a.x) && aligned16(a.w_router);
+  const int64_t warps = (a.num_tokens + few::kRouterTokens - 1) / few::kRouterTokens * a.E;
+  const unsigned grid = (unsigned)std::min<int64_t>((warps + 7) / 8, 4 * num_sms(current_device()));
+  if (vec)
+    few::router_kernel<T, true><<<grid, 256, 0, a.stream>>>(
+        (const T*)a.x, (const T*)a.w_router, a.router_bias, logits, (int)a.num_tokens, (int)a.d,
+        a.E, zero, num_zero);
+  else
+    few::router_kernel<T, false><<<grid, 256, 0, a.stream>>>(
+        (const T*)a.x, (const T*)a.w_router, a.router_bias, logits, (int)a.num_tokens, (int)a.d,
+        a.E, zero, num_zero);
+  MOE_LAUNCH_CHECK();
+  return MOE_OK;
+}
+
+template <typename T>
+static int few_simt_launch(const FewArgs& a, const few::Routing& r, float* h) {
+  const int S = r.num_tokens * r.K;
+  const int plan = few::plan_bytes(S, r.E, few::kSimtRows);
+  const bool vec = (a.d * sizeof(T)) % 16 == 0 && (a.hidden * sizeof(T)) % 16 == 0 &&
+                   aligned16(a.x) && aligned16(a.w_gate) && aligned16(a.w_up) && aligned16(a.w_down);
+  const int sms = num_sms(current_device());
+  const int64_t gu = (int64_t)few::plan_max_units(S, r.E, few::kSimtRows) * a.hidden;
+  const dim3 grid_gu((unsigned)std::max<int64_t>(1, std::min<int64_t>((gu + 7) / 8, 4 * sms)));
+  const dim3 grid_dn((unsigned)std::min<int64_t>((a.d + 7) / 8, 4 * sms));
+  const size_t smem_dn = plan + (size_t)8 * r.num_tokens * 4;
+  const T *x = (const T*)a.x, *wg = (const T*)a.w_gate, *wu = (const T*)a.w_up, *wd = (const T*)a.w_down;
+  T* y = (T*)a.out;
+  const int d = (int)a.d, H = (int)a.hidden;
+  if (vec) {
+    MOE_CUDA_CHECK(launch_pdl(few::gate_up_simt_kernel<T, true>, grid_gu, dim3(256), plan, a.stream,
+                              x, wg, wu, h, r, d, H));
+    MOE_CUDA_CHECK(launch_pdl(few::down_simt_kernel<T, true>, grid_dn, dim3(256), smem_dn, a.stream,
+                              (const float*)h, wd, y, r, d, H));
+  } else {
+    MOE_CUDA_CHECK(launch_pdl(few::gate_up_simt_kernel<T, false>, grid_gu, dim3(256), plan, a.stream,
+                              x, wg, wu, h, r, d, H));
+    MOE_CUDA_CHECK(launch_pdl(few::down_simt_kernel<T, false>, grid_dn, dim3(256), smem_dn, a.stream,
+                              (const float*)h, wd, y, r, d, H));
+  }
+  return MOE_OK;
+}
+
+static int few_tokens_run(const FewArgs& a) {
+  int rc = check_few(a);
+  if (rc) return rc;
+  if (a.num_tokens == 0 || a.d == 0) return MOE_OK;
+  if (a.hidden == 0) {
+    MOE_CUDA_CHECK(cudaMemsetAsync(a.out, 0, (size_t)a.num_tokens * a.d * dtype_size(a.dtype), a.stream));
+    return MOE_OK;
+  }
+  const FewWorkspace w = few_workspace(a.num_tokens, a.hidden, a.E, a.topk);
+  uint8_t* ws = (uint8_t*)a.workspace;
+  float* logits = (float*)(ws + w.logits);
+  few::Routing r = {};
+  r.num_tokens = (int)a.num_tokens;
+  r.E = a.E;
+  r.K = a.topk;
+  if (a.w_router) {
+    rc = MOE_DISPATCH_DTYPE(a.dtype, T, [&] { return few_router_launch<T>(a, logits, nullptr, 0); });
+    if (rc) return rc;
+    r.logits = logits;
+  } else {
+    r.weights = a.weights;
+    r.indices = a.indices;
+  }
+  return MOE_DISPATCH_DTYPE(a.dtype, T, [&] { return few_simt_launch<T>(a, r, (float*)(ws + w.h)); });
+}
+
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" {
+
+size_t moe_few_tokens_workspace_bytes(int64_t num_tokens, int64_t d, int64_t hidden,
+                                      int32_t num_experts, int32_t topk, int dtype) {
+  (void)d;
+  (void)dtype;
+  if (num_tokens <= 0 || hidden < 0 || num_experts <= 0 || topk <= 0) return 0;
+  return few_workspace(num_tokens, hidden, num_experts, topk).total;
+}
+
+int moe_few_tokens_fwd(const void* x, const void* w_router, const float* router_bias,
+                       const void* w_gate, const void* w_up, const void* w_down, int dtype,
+                       int64_t num_tokens, int64_t d, int64_t hidden, int32_t num_experts,
+                       int32_t topk, void* out, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  MOE_REQUIRE(w_router || num_tokens == 0, "few_tokens: w_router is NULL");
+  FewArgs a = {};
+  a.x = x; a.w_router = w_router; a.router_bias = router_bias;
+  a.w_gate = w_gate; a.w_up = w_up; a.w_down = w_down; a.dtype = dtype;
+  a.num_tokens = num_tokens; a.d = d; a.hidden = hidden; a.E = num_experts; a.topk = topk;
+  a.out = out; a.workspace = workspace; a.workspace_bytes = workspace_bytes;
+  a.stream = (cudaStream_t)stream;
+  return few_tokens_run(a);
+}
+
+int moe_few_experts_fwd(const void* x, const float* weights, const int32_t* indices,
+                        const void* w_gate, const void* w_up, const void* w_down, int dtype,
+                        int64_t num_tokens, int64_t d, int64_t hidden, int32_t num_experts,
+                        int32_t topk, void* out, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  FewArgs a = {};
+  a.x = x; a.weights = weights; a.indices = indices;
+  a.w_gate = w_gate; a.w_up = w_up; a.w_down = w_down; a.dtype = dtype;
+  a.num_tokens = num_tokens; a.d = d; a.hidden = hidden; a.E = num_experts; a.topk = topk;
+  a.out = out; a.workspace = workspace; a.workspace_bytes = workspace_bytes;
+  a.stream = (cudaStream_t)stream;
+  return few_tokens_run(a);
+}
+
+}  // extern "C"

@@ -1318,3 +1318,5 @@ int moe_selftest_bounded_wait(uint64_t timeout_ns, int32_t* result, void* stream
 }
 
 }  // extern "C"
+
+#include "few_api.cuh"

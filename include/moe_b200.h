@@ -37,6 +37,14 @@ enum moe_status {
   MOE_ERR_DEVICE = 5         /* a kernel reported a device-side error flag        */
 };
 
+enum moe_activation {
+  MOE_ACT_NONE = 0,
+  MOE_ACT_RELU = 1,
+  MOE_ACT_GELU = 2,       /* z * (1 + erf(z / sqrt(2))) / 2                       */
+  MOE_ACT_GELU_TANH = 3,  /* its tanh form                                        */
+  MOE_ACT_SILU = 4
+};
+
 /* Library version string, e.g. "moe_b200 0.1.0 sm_100a". */
 const char* moe_version(void);
 
@@ -345,6 +353,33 @@ int moe_few_experts_fwd(const void* x, const float* weights, const int32_t* indi
                         int64_t num_tokens, int64_t d, int64_t hidden, int32_t num_experts,
                         int32_t topk, void* out, void* workspace, size_t workspace_bytes,
                         void* stream);
+
+/* Matrix product with bias, activation and residual in its epilogue, dense or per expert:
+ *   z[r] = A[r] . op(B[g]) + bias[g]     (g: the expert of row r)
+ *   out[r] = act(z[r]) + residual[r]
+ * A [m_total, k], B [E, N, K] if trans_b else [E, K, N], bias [E, n] or NULL, residual
+ * [m_total, n] or NULL, out [m_total, n]; preact [m_total, n] receives z rounded to dtype (for
+ * the backward), or NULL.  Offsets as in moe_gmm_fwd (replaces an moe_gmm_fwd followed by
+ * elementwise passes); a dense product is offsets NULL, num_offsets 0, num_experts 1.  Rows
+ * behind the last offset get residual (or zero).  residual may not overlap out.  The sum, the
+ * bias, the activation and the residual are in fp32; out is rounded once. */
+int moe_linear_fwd(const void* A, const void* B, const void* bias, const void* residual, void* out,
+                   void* preact, const int32_t* offsets, int32_t num_offsets, int64_t m_total,
+                   int64_t n, int64_t k, int32_t num_experts, int trans_b, int activation, int dtype,
+                   void* stream);
+/* The elementwise part of its backward: grad_preact = grad_out * act'(preact) and grad_bias
+ * [E, n] = its sum over each expert's rows (from the unrounded products, in a fixed order; NULL:
+ * not wanted).  For MOE_ACT_NONE grad_preact is grad_out itself: it is not written, and preact
+ * and grad_preact may be NULL.  The products' gradients are moe_gmm_dgrad and moe_gmm_wgrad on
+ * grad_preact (which take offsets NULL, num_offsets 0, num_experts 1 for a dense product). */
+size_t moe_linear_act_bwd_workspace_bytes(int64_t m_total, int64_t n, int32_t num_experts);
+int moe_linear_act_bwd(const void* grad_out, const void* preact, void* grad_preact, void* grad_bias,
+                       const int32_t* offsets, int32_t num_offsets, int64_t m_total, int64_t n,
+                       int32_t num_experts, int activation, int dtype, void* workspace,
+                       size_t workspace_bytes, void* stream);
+/* Zeroes the rows of out [m_total, n] behind the last offset. */
+int moe_zero_tail_rows(void* out, const int32_t* offsets, int32_t num_offsets, int64_t m_total,
+                       int64_t n, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -16,7 +16,8 @@ Beyond the reference: grouped_gemm_swiglu / grouped_swiglu_mlp (the SwiGLU exper
 fused launches), permute_with_capacity (token dropping at a per-expert capacity), and
 permute_index + grouped_swiglu_mlp_gathered (the permute fused into the expert GEMMs).
 For serving: moe_few_tokens (the whole layer for up to 128 tokens) and moe_few_experts (the
-same with the routing given).
+same with the routing given).  linear / grouped_linear: a dense or per-expert product with
+bias, activation and residual in its epilogue, differentiable.
 
 Layout conventions (same as the reference):
     A:        [total_tokens, K]   (all experts stacked along rows)
@@ -32,6 +33,7 @@ from .fused_topk_softmax_ops import fused_topk_softmax
 from .gate_up_ops import grouped_gemm_swiglu, grouped_swiglu_mlp
 from .fused_permute_ops import grouped_swiglu_mlp_gathered, permute_index
 from .few_token_ops import moe_few_experts, moe_few_tokens
+from .linear_ops import grouped_linear, linear
 
 __all__ = [
     "grouped_gemm",
@@ -52,4 +54,7 @@ __all__ = [
     # serving: the whole layer for a few tokens
     "moe_few_tokens",
     "moe_few_experts",
+    # matrix products with bias, activation and residual in their epilogue
+    "linear",
+    "grouped_linear",
 ]

@@ -1,0 +1,64 @@
+// Activations of the linear operators' epilogues and their derivatives, in fp32.
+//
+//   relu       max(z, 0)
+//   gelu       z * Phi(z),  Phi(z) = (1 + erf(z / sqrt(2))) / 2
+//   gelu_tanh  z * (1 + tanh(a * (z + 0.044715 z^3))) / 2,  a = sqrt(2 / pi)
+//   silu       z / (1 + exp(-z))
+#pragma once
+
+#include "common.cuh"
+#include "swiglu.cuh"
+
+namespace moe {
+
+// tanh through one exponential of a non-positive argument (it cannot overflow); near 0 its
+// absolute error is of the order of 2^-24, which is all that 1 + tanh needs.
+__device__ __forceinline__ float tanh_exp(float u) {
+  const float t = expf(-2.f * fabsf(u));
+  return copysignf((1.f - t) / (1.f + t), u);
+}
+
+template <int ACT>
+__device__ __forceinline__ float act_fwd(float z) {
+  if constexpr (ACT == MOE_ACT_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
+  if constexpr (ACT == MOE_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678f));
+  if constexpr (ACT == MOE_ACT_GELU_TANH)
+    return 0.5f * z * (1.f + tanh_exp(0.79788456f * (z + 0.044715f * z * z * z)));
+  if constexpr (ACT == MOE_ACT_SILU) return z * sigmoid_f32(z);
+  return z;
+}
+
+template <int ACT>
+__device__ __forceinline__ float act_bwd(float z) {
+  if constexpr (ACT == MOE_ACT_RELU) return z > 0.f ? 1.f : (z != z ? z : 0.f);
+  if constexpr (ACT == MOE_ACT_GELU)
+    return 0.5f * (1.f + erff(z * 0.70710678f)) + z * (expf(-0.5f * z * z) * 0.39894228f);
+  if constexpr (ACT == MOE_ACT_GELU_TANH) {
+    const float th = tanh_exp(0.79788456f * (z + 0.044715f * z * z * z));
+    // beyond |z| = 8 the second term is below 2^-24 of the first and z^2 may overflow
+    const float zc = fminf(fmaxf(z, -8.f), 8.f);
+    return 0.5f * (1.f + th) + 0.5f * zc * (1.f - th * th) * 0.79788456f * (1.f + 0.134145f * zc * zc);
+  }
+  if constexpr (ACT == MOE_ACT_SILU) {
+    const float s = sigmoid_f32(z);
+    return s == 0.f ? 0.f : s * (1.f + z * (1.f - s));
+  }
+  return 1.f;
+}
+
+// Runs the statements with the activation code as a compile-time constant ACT.
+#define MOE_SWITCH_ACT(code, ACT, ...)                                        \
+  switch (code) {                                                             \
+    case MOE_ACT_RELU: { constexpr int ACT = MOE_ACT_RELU; __VA_ARGS__; break; }           \
+    case MOE_ACT_GELU: { constexpr int ACT = MOE_ACT_GELU; __VA_ARGS__; break; }           \
+    case MOE_ACT_GELU_TANH: { constexpr int ACT = MOE_ACT_GELU_TANH; __VA_ARGS__; break; } \
+    case MOE_ACT_SILU: { constexpr int ACT = MOE_ACT_SILU; __VA_ARGS__; break; }           \
+    default: { constexpr int ACT = MOE_ACT_NONE; __VA_ARGS__; break; }                     \
+  }
+
+__device__ __forceinline__ float act_fwd_rt(int act, float z) {
+  MOE_SWITCH_ACT(act, A, return act_fwd<A>(z));
+  return z;
+}
+
+}  // namespace moe

@@ -20,23 +20,35 @@ struct GroupRange {
   int64_t start, rows;
 };
 
-__device__ __forceinline__ GroupRange group_range(const int32_t* offsets, int plus_one, int g) {
+// offsets == nullptr: one group of all m_total rows.
+__device__ __forceinline__ GroupRange group_range(const int32_t* offsets, int plus_one, int g,
+                                                  int64_t m_total) {
   GroupRange r;
+  if (offsets == nullptr) { r.start = 0; r.rows = m_total; return r; }
   if (plus_one) { r.start = offsets[g]; r.rows = (int64_t)offsets[g + 1] - offsets[g]; }
   else { r.start = g > 0 ? offsets[g - 1] : 0; r.rows = (int64_t)offsets[g] - r.start; }
   if (r.rows < 0) r.rows = 0;
   return r;
 }
 
+// What happens to a finished element (row, column n of group g); this one stores it.
+template <typename T>
+struct StoreEpilogue {
+  T* C;
+  __device__ __forceinline__ void operator()(float acc, int, int64_t row, int64_t n, int64_t Nout) const {
+    C[row * Nout + n] = from_f32<T>(acc);
+  }
+};
+
 // Row mode: C[start+m, n] = sum_k A[start+m, k] * B(g, n, k),
 // B(g, n, k) = b_mn ? B[(g*Kc + k)*Nout + n] : B[(g*Nout + n)*Kc + k].
-template <typename T>
+template <typename T, typename Epi>
 __global__ void __launch_bounds__(256)
-gmm_rows_simt_kernel(const T* __restrict__ A, const T* __restrict__ B, T* __restrict__ C,
-                     const int32_t* __restrict__ offsets, int plus_one, int64_t Nout, int64_t Kc,
-                     int b_mn) {
+gmm_rows_simt_kernel(const T* __restrict__ A, const T* __restrict__ B, const Epi epi,
+                     const int32_t* __restrict__ offsets, int plus_one, int64_t m_total,
+                     int64_t Nout, int64_t Kc, int b_mn) {
   const int g = blockIdx.z;
-  const GroupRange gr = group_range(offsets, plus_one, g);
+  const GroupRange gr = group_range(offsets, plus_one, g, m_total);
   const int64_t m0 = (int64_t)blockIdx.x * TM;
   if (m0 >= gr.rows) return;
   const int64_t n0 = (int64_t)blockIdx.y * TN;
@@ -79,7 +91,7 @@ gmm_rows_simt_kernel(const T* __restrict__ A, const T* __restrict__ B, T* __rest
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t n = n0 + tx * 4 + j;
-      if (n < Nout) C[(gr.start + m) * Nout + n] = from_f32<T>(acc[i][j]);
+      if (n < Nout) epi(acc[i][j], g, gr.start + m, n, Nout);
     }
   }
 }
@@ -88,9 +100,10 @@ gmm_rows_simt_kernel(const T* __restrict__ A, const T* __restrict__ B, T* __rest
 template <typename T>
 __global__ void __launch_bounds__(256)
 gmm_wgrad_simt_kernel(const T* __restrict__ X, const T* __restrict__ Y, T* __restrict__ Out,
-                      const int32_t* __restrict__ offsets, int plus_one, int64_t P, int64_t Q) {
+                      const int32_t* __restrict__ offsets, int plus_one, int64_t m_total,
+                      int64_t P, int64_t Q) {
   const int g = blockIdx.z;
-  const GroupRange gr = group_range(offsets, plus_one, g);
+  const GroupRange gr = group_range(offsets, plus_one, g, m_total);
   const int64_t p0 = (int64_t)blockIdx.y * TM, q0 = (int64_t)blockIdx.x * TN;
   __shared__ float Xs[TK][TM + 1];
   __shared__ float Ys[TK][TN + 1];

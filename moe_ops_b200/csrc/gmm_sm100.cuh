@@ -5,10 +5,11 @@
 //                    gmm_forward_kernel         triton_gmm_ops/grouped_gemm_ops.py:20-69
 //   wgrad            gmm_gradB_kernel           triton_gmm_ops/grouped_gemm_ops.py:126-165
 //
-// One kernel template, two modes:
+// One kernel template, the main modes:
 //   kModeRows   (forward and dgrad): C[rows of g] = A[rows of g] . op(B[g]); the tiles of
 //               expert g cover its ragged row range, the contraction length is fixed.
 //               A is K-major; B[g] is K-major ([Nout, Kc]) or MN-major ([Kc, Nout]).
+//   kModeLinear  kModeRows with bias, activation and residual in the epilogue.
 //   kModeWgrad  (wgrad): Out[g] = X[rows of g]^T . Y[rows of g]  ([P, Q] per expert); the
 //               contraction runs over the ragged rows of expert g.  X and Y are MN-major.
 //
@@ -60,6 +61,7 @@
 
 #include "common.cuh"
 #include "sm100_ptx.cuh"
+#include "activation.cuh"
 #include "swiglu.cuh"
 
 #include <type_traits>
@@ -98,7 +100,11 @@ struct Shape {
   static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;  // per CTA per stage
 };
 
-enum Mode { kModeRows = 0, kModeWgrad = 1, kModeGateUp = 2, kModeSwiGLUBwd = 3 };
+enum Mode { kModeRows = 0, kModeWgrad = 1, kModeGateUp = 2, kModeSwiGLUBwd = 3, kModeLinear = 4 };
+
+// Modes whose tiles are row tiles of one output with every column of the accumulator.
+template <int MODE>
+__host__ __device__ constexpr bool plain_rows() { return MODE == kModeRows || MODE == kModeLinear; }
 
 // Output columns one tile covers: a gate/up tile holds 128 gate and 128 up columns in its
 // 256-column accumulator and writes 128 columns of each output.
@@ -145,6 +151,12 @@ struct Params {
   // box is one row high).  Row mode (1-SM tiles): the operand is A; wgrad mode: Y.
   const int32_t* gather_rows;
   int gather_src_rows;
+  // kModeLinear: out = act(A . op(B[g]) + bias[g]) + residual; the sum before the activation
+  // goes to preact (any of the three may be NULL).
+  const void* bias;      // [num_groups, n_out]
+  const void* residual;  // [m_total, n_out]
+  void* preact;          // [m_total, n_out], through map_c2
+  int act;
   int k_red2;            // kModeRows: > 0 adds a second contraction segment into the same
                          // accumulator: C = A . op(B[g]) + A2 . op(B2[g]), A2 [m_total,
                          // k_red2] through map_c2 and B2 through map_b2 (two-segment dgrad)
@@ -162,6 +174,7 @@ struct TileInfo {
 // First row and row count of expert g (negative counts clamp to zero).
 __device__ __forceinline__ void group_range(const Params& p, int g, int& start, int& rows) {
   int st, en;
+  if (p.offsets == nullptr) { start = 0; rows = (int)p.m_total; return; }  // one group
   if (p.offsets_plus_one) { st = __ldg(p.offsets + g); en = __ldg(p.offsets + g + 1); }
   else { st = g > 0 ? __ldg(p.offsets + g - 1) : 0; en = __ldg(p.offsets + g); }
   start = st;
@@ -225,7 +238,7 @@ __device__ __forceinline__ TileInfo decode_tile(const int* tile_prefix, const Pa
 // 128-255 of rows 0-63.
 template <int MODE, int CG>
 __device__ __forceinline__ bool is_half_tile(const TileInfo& ti) {
-  return MODE == kModeRows && CG == 2 && ti.rows <= BMC;
+  return plain_rows<MODE>() && CG == 2 && ti.rows <= BMC;
 }
 
 // Packs 8 fp32 values into 8 16-bit values (round to nearest even) as one 16-byte vector.
@@ -675,6 +688,22 @@ gmm_sm100_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       const TileInfo ti = decode_tile<MODE, CG>(s.tile_prefix, p, t);
       const int buf = acc & 1;
       const uint32_t acc_phase = (acc >> 1) & 1;
+      if constexpr (MODE == kModeLinear) {
+        // While this tile's main loop runs, pull the residual its epilogue will add into L2
+        // (this lane's row, 128 columns: 256 bytes, up to 3 lines).
+        if (p.residual != nullptr) {
+          const bool half = is_half_tile<MODE, CG>(ti);
+          const int r = (half ? (q & 1) : q) * 32 + lane;
+          const int cta_rows = half ? BMC / 2 : BMC;
+          const int c0 = ti.n_blk * BN + (half ? (q >> 1) * (BN / 2) + h * 64 : h * (BN / 2));
+          if (r < min(cta_rows, ti.rows - (int)rank * cta_rows) && c0 < p.n_out) {
+            const int64_t e0 = (int64_t)(ti.row0 + (int)rank * cta_rows + r) * p.n_out + c0;
+            const int64_t e1 = e0 + min(half ? 64 : BN / 2, p.n_out - c0) - 1;
+            for (int64_t e = e0; e <= e1 + 63; e += 64)
+              ptx::prefetch_l2(static_cast<const OutT*>(p.residual) + (e < e1 ? e : e1));
+          }
+        }
+      }
       if constexpr (MODE == kModeSwiGLUBwd) {
         // While this tile's main loop runs, pull the gate / up values its epilogue will
         // read into L2: this lane's row, the warp's 128 columns (256 bytes, up to 3 lines).
@@ -793,6 +822,66 @@ gmm_sm100_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                                     row_base + q * 32, du_out + off, p.n_out, vr, valid_cols - col);
           }
         }
+      } else if constexpr (MODE == kModeLinear) {
+        // As the plain row tiles below (same geometry, half tiles included), with the bias,
+        // the activation and the residual applied to the fp32 accumulator: out is rounded
+        // once.  preact is the one value the backward needs; it is rounded to 16 bits (half a
+        // step of z moves act'(z) by at most |act''| times that, less than the rounding of
+        // the gradient it scales).
+        const int n0 = ti.n_blk * BN;
+        const bool half = is_half_tile<MODE, CG>(ti);
+        const int rq = half ? (q & 1) : q;
+        const int tcol = half ? h * 64 : h * (BN / 2);
+        const int col_lo = half ? (q >> 1) * (BN / 2) + h * 64 : h * (BN / 2);
+        const int ncols = half ? 64 : BN / 2;
+        const int valid_cols = min(BN, p.n_out - n0);
+        const int cta_rows = half ? BMC / 2 : BMC;
+        const int valid_rows = min(cta_rows, ti.rows - (int)rank * cta_rows);
+        const int row_base = ti.row0 + (int)rank * cta_rows;
+        const int vr = min(32, valid_rows - rq * 32);
+        const bool use_tma = vr == 32;
+        const int nchunks = vr <= 0 ? 0 : max(0, min(ncols, valid_cols - col_lo) + 31) / 32;
+        const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + buf * BN + tcol;
+        const OutT* bias = static_cast<const OutT*>(p.bias);
+        const OutT* res = static_cast<const OutT*>(p.residual);
+        if (bias) bias += (int64_t)ti.g * p.n_out;
+        uint32_t v[32];
+        if (nchunks > 0) ptx::tmem_ld_32x32b_x32(tbase, v);
+        for (int c = 0; c < nchunks; ++c) {
+          const int col = n0 + col_lo + c * 32;  // first column of the chunk
+          const int64_t off = (int64_t)(row_base + rq * 32) * p.n_out + col;
+          uint4 braw[4], rraw[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool in = col + i * 8 < p.n_out;
+            braw[i] = bias && in ? __ldg(reinterpret_cast<const uint4*>(bias + col + i * 8))
+                                 : make_uint4(0, 0, 0, 0);
+            rraw[i] = res && in && lane < vr
+                          ? __ldg(reinterpret_cast<const uint4*>(res + off + (int64_t)lane * p.n_out + i * 8))
+                          : make_uint4(0, 0, 0, 0);
+          }
+          ptx::tmem_wait_ld();
+          const OutT* bv = reinterpret_cast<const OutT*>(braw);
+          const OutT* rv = reinterpret_cast<const OutT*>(rraw);
+          uint32_t wz[16], wy[16];
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            v[i] = __float_as_uint(__uint_as_float(v[i]) + to_f32(bv[i]));
+          if (p.preact) pack32_16b<OutT>(v, wz);
+          MOE_SWITCH_ACT(p.act, ACT, {
+            _Pragma("unroll") for (int i = 0; i < 32; ++i)
+              v[i] = __float_as_uint(act_fwd<ACT>(__uint_as_float(v[i])) + to_f32(rv[i]));
+          })
+          pack32_16b<OutT>(v, wy);
+          if (c + 1 < nchunks) ptx::tmem_ld_32x32b_x32(tbase + (c + 1) * 32, v);
+          if (p.preact)
+            stage_store_block<OutT>(wz, cbuf, cbuf_u32, lane, use_tma, &map_c2, col,
+                                    row_base + rq * 32, static_cast<OutT*>(p.preact) + off, p.n_out,
+                                    vr, p.n_out - col);
+          stage_store_block<OutT>(wy, cbuf, cbuf_u32, lane, use_tma, &map_c, col,
+                                  row_base + rq * 32, out + off, p.n_out, vr, p.n_out - col);
+        }
+        ptx::tmem_wait_ld();
       } else {
         const int n0 = ti.n_blk * BN;
         // Full tile: this warp reads TMEM lanes of rows 32q..32q+31 and tile columns

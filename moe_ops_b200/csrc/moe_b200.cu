@@ -274,16 +274,18 @@ static int gmm_rows(const void* A, const void* B, void* C, const int32_t* offset
     switch (dtype) {
       case MOE_F32:
         simt::gmm_rows_simt_kernel<float><<<grid, 256, 0, stream>>>(
-            (const float*)A, (const float*)B, (float*)C, offsets, plus_one, n_out, k_red, b_mn);
+            (const float*)A, (const float*)B, simt::StoreEpilogue<float>{(float*)C}, offsets, plus_one,
+            m_total, n_out, k_red, b_mn);
         break;
       case MOE_F16:
         simt::gmm_rows_simt_kernel<__half><<<grid, 256, 0, stream>>>(
-            (const __half*)A, (const __half*)B, (__half*)C, offsets, plus_one, n_out, k_red, b_mn);
+            (const __half*)A, (const __half*)B, simt::StoreEpilogue<__half>{(__half*)C}, offsets, plus_one,
+            m_total, n_out, k_red, b_mn);
         break;
       default:
         simt::gmm_rows_simt_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(
-            (const __nv_bfloat16*)A, (const __nv_bfloat16*)B, (__nv_bfloat16*)C, offsets,
-            plus_one, n_out, k_red, b_mn);
+            (const __nv_bfloat16*)A, (const __nv_bfloat16*)B, simt::StoreEpilogue<__nv_bfloat16>{(__nv_bfloat16*)C}, offsets, plus_one,
+            m_total, n_out, k_red, b_mn);
     }
     MOE_LAUNCH_CHECK();
     return MOE_OK;
@@ -396,16 +398,18 @@ static int gmm_wgrad(const void* X, const void* Y, void* Out, const int32_t* off
     switch (dtype) {
       case MOE_F32:
         simt::gmm_wgrad_simt_kernel<float><<<grid, 256, 0, stream>>>(
-            (const float*)X, (const float*)Y, (float*)Out, offsets, plus_one, P, Q);
+            (const float*)X, (const float*)Y, (float*)Out, offsets,
+            plus_one, m_total, P, Q);
         break;
       case MOE_F16:
         simt::gmm_wgrad_simt_kernel<__half><<<grid, 256, 0, stream>>>(
-            (const __half*)X, (const __half*)Y, (__half*)Out, offsets, plus_one, P, Q);
+            (const __half*)X, (const __half*)Y, (__half*)Out, offsets,
+            plus_one, m_total, P, Q);
         break;
       default:
         simt::gmm_wgrad_simt_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(
             (const __nv_bfloat16*)X, (const __nv_bfloat16*)Y, (__nv_bfloat16*)Out, offsets,
-            plus_one, P, Q);
+            plus_one, m_total, P, Q);
     }
     MOE_LAUNCH_CHECK();
     return MOE_OK;
@@ -456,9 +460,11 @@ static int check_gmm_args(const void* a, const void* b, const void* c, const int
                           int num_offsets, int64_t m_total, int64_t n, int64_t k, int E, int dtype) {
   MOE_REQUIRE(dtype_ok(dtype), "gmm: bad dtype %d", dtype);
   MOE_REQUIRE(E >= 0 && m_total >= 0 && n >= 0 && k >= 0, "gmm: negative size");
-  MOE_REQUIRE(num_offsets == E || num_offsets == E + 1,
+  // No offsets: one group of all m_total rows (a dense product).
+  const bool dense = offsets == nullptr && num_offsets == 0 && E == 1;
+  MOE_REQUIRE(dense || num_offsets == E || num_offsets == E + 1,
               "gmm: num_offsets must be E or E+1 (got %d, E=%d)", num_offsets, E);
-  MOE_REQUIRE(E == 0 || offsets != nullptr, "gmm: offsets is NULL");
+  MOE_REQUIRE(dense || E == 0 || offsets != nullptr, "gmm: offsets is NULL");
   MOE_REQUIRE((a && b && c) || m_total == 0 || E == 0, "gmm: NULL operand");
   return MOE_OK;
 }
@@ -1320,3 +1326,4 @@ int moe_selftest_bounded_wait(uint64_t timeout_ns, int32_t* result, void* stream
 }  // extern "C"
 
 #include "few_api.cuh"
+#include "linear_api.cuh"

@@ -1,0 +1,198 @@
+"""Matrix product with bias, activation and residual in its epilogue, dense and per expert.
+
+    linear(x, weight, bias=None, activation="none", residual=None) -> y
+    grouped_linear(A, B, offsets, bias=None, activation="none", residual=None, trans_b=True) -> C
+
+        z = x . W^T + bias            (per expert row range for grouped_linear)
+        y = act(z) + residual
+
+``grouped_linear`` stands beside ``grouped_gemm`` (same A, B, offsets and trans_b) for experts
+with biases or an activation of their own; ``linear`` is the dense product next to the routed
+experts (a shared expert, a projection).  One launch: the sum, the bias, the activation and the
+residual are in fp32 and y is rounded once.
+
+Both are differentiable in every tensor argument.  With an activation the forward also writes z
+(rounded to the dtype) when a gradient will be needed; the backward is one elementwise pass
+(dz = dy * act'(z), and the bias gradient from the unrounded dz), then the library's dgrad and
+wgrad GEMMs.  The residual's gradient is dy itself.
+
+Activations: "none", "relu", "gelu" (erf), "gelu_tanh", "silu".
+
+Plain functions and autograd Functions over the C ABI (no ``torch.library`` ops): for one row
+the host's part of a call is of the order of the kernel's time.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+def _check(x, w, bias, residual, out_shape, bias_shape, activation) -> int:
+    _lib.require_cuda(x, w, bias, residual)
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)} (got {activation!r})")
+    _lib.dtype_code(x.dtype)
+    for name, t, shape in (("weight", w, None), ("bias", bias, bias_shape),
+                           ("residual", residual, out_shape)):
+        if t is None:
+            continue
+        if t.dtype != x.dtype or t.device != x.device:
+            raise ValueError(f"{name} must have the input's dtype and device")
+        if shape is not None and tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{name} must be {list(shape)} (got {list(t.shape)})")
+    return act
+
+
+def _forward(x, w, bias, residual, offsets, act: int, trans_b: bool, E: int, n: int, want_z: bool):
+    """x [m, k], w [E, n, k] or [E, k, n] (2-D when dense), contiguous; returns (y, z or None)."""
+    m, k = x.shape
+    y = torch.empty((m, n), device=x.device, dtype=x.dtype)
+    z = torch.empty_like(y) if want_z else None
+    lib = _lib.load()
+    with torch.cuda.device(x.device):
+        st = lib.moe_linear_fwd(
+            x.data_ptr(), w.data_ptr(), _lib.ptr(bias), _lib.ptr(residual), y.data_ptr(), _lib.ptr(z),
+            _lib.ptr(offsets), 0 if offsets is None else offsets.numel(), m, n, k, E, int(trans_b),
+            act, _lib.dtype_code(x.dtype), _lib.stream_of(x))
+    _lib.check(st, "moe_linear_fwd")
+    _lib.count_launches(1)
+    return y, z
+
+
+def _act_bwd(dy, z, offsets, E: int, act: int, want_bias: bool, bias_shape):
+    """(dz, dbias): one pass over dy and z."""
+    m, n = dy.shape
+    code = _lib.dtype_code(dy.dtype)
+    dz = torch.empty_like(dy) if act else dy
+    db = torch.empty(bias_shape, device=dy.device, dtype=dy.dtype) if want_bias else None
+    if not act and db is None:
+        return dz, None
+    lib = _lib.load()
+    ws_bytes = lib.moe_linear_act_bwd_workspace_bytes(m, n, E) if want_bias else 0
+    ws = torch.empty(ws_bytes, device=dy.device, dtype=torch.uint8)
+    with torch.cuda.device(dy.device):
+        st = lib.moe_linear_act_bwd(
+            dy.data_ptr(), _lib.ptr(z), dz.data_ptr() if act else None, _lib.ptr(db),
+            _lib.ptr(offsets), 0 if offsets is None else offsets.numel(), m, n, E, act, code,
+            ws.data_ptr() if ws_bytes else None, ws_bytes, _lib.stream_of(dy))
+    _lib.check(st, "moe_linear_act_bwd")
+    _lib.count_launches(1 + int(want_bias))
+    return dz, db
+
+
+def _gemm(fn: str, a, b, shape, offsets, m, n, k, E, trans_b):
+    out = torch.empty(shape, device=a.device, dtype=a.dtype)
+    if out.numel() == 0 or (n if fn == "moe_gmm_dgrad" else m) == 0:
+        return out.zero_()
+    lib = _lib.load()
+    with torch.cuda.device(a.device):
+        st = getattr(lib, fn)(
+            a.data_ptr(), b.data_ptr(), out.data_ptr(), _lib.ptr(offsets),
+            0 if offsets is None else offsets.numel(), m, n, k, E, int(trans_b),
+            _lib.dtype_code(a.dtype), _lib.stream_of(a))
+        _lib.check(st, fn)
+        if fn == "moe_gmm_dgrad" and offsets is not None:
+            _lib.check(lib.moe_zero_tail_rows(out.data_ptr(), offsets.data_ptr(), offsets.numel(), m,
+                                              k, _lib.dtype_code(a.dtype), _lib.stream_of(a)),
+                       "moe_zero_tail_rows")
+    _lib.count_launches(1)
+    return out
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, residual, offsets, act, trans_b, E, n):
+        y, z = _forward(x, w, bias, residual, offsets, act, trans_b, E, n,
+                        want_z=act != 0 and any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x, w, z, offsets)
+        ctx.cfg = (act, trans_b, E, n, None if bias is None else bias.shape)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, z, offsets = ctx.saved_tensors
+        act, trans_b, E, n, bias_shape = ctx.cfg
+        m, k = x.shape
+        want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
+        dx = dw = db = None
+        if want_x or want_w or want_b:
+            dyc = dy.contiguous()
+            dz, db = _act_bwd(dyc, z, offsets, E, act if (want_x or want_w or want_b) else 0, want_b,
+                              bias_shape)
+            if want_x:
+                dx = _gemm("moe_gmm_dgrad", dz, w, (m, k), offsets, m, n, k, E, trans_b)
+            if want_w:
+                dw = _gemm("moe_gmm_wgrad", x, dz, w.shape, offsets, m, n, k, E, trans_b)
+        return dx, dw, db, dy if want_r else None, None, None, None, None, None
+
+
+def _apply(x, w, bias, residual, offsets, act, trans_b, E, n):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias, residual)):
+        return _Linear.apply(x, w, bias, residual, offsets, act, trans_b, E, n)
+    return _forward(x, w, bias, residual, offsets, act, trans_b, E, n, False)[0]
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+           activation: str = "none", residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """act(x . weight^T + bias) + residual, in one launch.
+
+    Args:
+        x: [..., K].
+        weight: [N, K].
+        bias: [N], or None.
+        activation: "none", "relu", "gelu", "gelu_tanh" or "silu".
+        residual: [..., N] (the output's shape), or None.
+
+    Returns:
+        [..., N] in x's dtype.
+    """
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x [..., K] and weight [N, K] do not match: {list(x.shape)}, {list(weight.shape)}")
+    n, k = weight.shape
+    out_shape = x.shape[:-1] + (n,)
+    act = _check(x, weight, bias, residual, out_shape, (n,), activation)
+    x2 = x.reshape(-1, k) if k else x.reshape(out_shape[:-1].numel(), 0)
+    r2 = None if residual is None else residual.reshape(x2.shape[0], n).contiguous()
+    y = _apply(x2.contiguous(), weight.contiguous(), None if bias is None else bias.contiguous(), r2,
+               None, act, True, 1, n)
+    return y.view(out_shape)
+
+
+def grouped_linear(A: torch.Tensor, B: torch.Tensor, offsets: torch.Tensor,
+                   bias: Optional[torch.Tensor] = None, activation: str = "none",
+                   residual: Optional[torch.Tensor] = None, trans_b: bool = True) -> torch.Tensor:
+    """``grouped_gemm`` with a bias per expert, an activation and a residual in its epilogue.
+
+    Args:
+        A: [total_tokens, K], the experts' rows stacked.
+        B: [E, N, K] if trans_b else [E, K, N].
+        offsets: int32 [E+1] (starting at 0) or [E] end rows, as in ``grouped_gemm``.
+        bias: [E, N], or None.
+        activation, residual: as in ``linear``; residual [total_tokens, N].
+
+    Returns:
+        [total_tokens, N].  Rows behind the last offset get the residual (zero without one), and
+        their input gradient is zero.
+    """
+    if A.dim() != 2 or B.dim() != 3 or B.shape[2 if trans_b else 1] != A.shape[1]:
+        raise ValueError(f"A [M, K] and B do not match: {list(A.shape)}, {list(B.shape)}, trans_b={trans_b}")
+    E, n = B.shape[0], B.shape[1 if trans_b else 2]
+    act = _check(A, B, bias, residual, (A.shape[0], n), (E, n), activation)
+    _lib.require_cuda(offsets)
+    if offsets.numel() not in (E, E + 1) or offsets.numel() == 0 or offsets.device != A.device:
+        raise ValueError(f"offsets must have E ({E}) or E+1 entries on A's device, got {offsets.numel()}")
+    if offsets.dtype != torch.int32:
+        offsets = offsets.to(torch.int32)
+    return _apply(A.contiguous(), B.contiguous(), None if bias is None else bias.contiguous(),
+                  None if residual is None else residual.contiguous(), offsets.contiguous(), act,
+                  bool(trans_b), E, n)
+
+
+__all__ = ["linear", "grouped_linear"]

@@ -2,6 +2,7 @@
 // workspace layout and launches.  Included by moe_b200.cu, whose helpers it uses.
 #pragma once
 
+#include "few_sm100.cuh"
 #include "few_tokens.cuh"
 
 namespace moe {
@@ -26,17 +27,40 @@ struct FewArgs {
 
 static size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
-// Workspace: logits [T, E] fp32, then h [T*K, H] (fp32).
+// Rows of a unit of the tensor-core kernel, by the most rows that one expert (one group) can
+// have unless an expert repeats: smaller units leave room for more stages, larger ones read a
+// crowded expert's weights once.
+static int few_nb(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+
+// Workspace: logits [T, E] fp32, h [T*K, H] (fp32 for the CUDA cores, else 16 bits), then for
+// the tensor-core kernel its counters and fp32 partial results.
 struct FewWorkspace {
-  size_t logits, h, total;
+  size_t logits, h, counters, part, o, extra, total;
+  int num_counters, max_chunks, max_units;
 };
-static FewWorkspace few_workspace(int64_t T, int64_t H, int64_t E, int64_t K) {
-  FewWorkspace w;
+static FewWorkspace few_workspace(int64_t T, int64_t d, int64_t H, int64_t E, int64_t K, int dtype,
+                                  int chunks) {
+  FewWorkspace w = {};
+  const size_t S = (size_t)(T * K), strips = (size_t)((d + 255) / 256);
   w.logits = 0;
   w.h = align256((size_t)T * E * 4);
-  w.total = w.h + align256((size_t)T * K * H * 4);
+  w.counters = w.h + align256(S * H * 4);
+  if (dtype == MOE_F32) {
+    w.total = w.counters;
+    return w;
+  }
+  const int nb = few_nb(T);
+  w.max_chunks = chunks;
+  w.max_units = few::plan_max_units((int)S, (int)E, nb);
+  w.num_counters = 1 + w.max_chunks + w.max_units + (int)strips;
+  w.part = w.counters + align256((size_t)w.num_counters * 4);
+  w.o = w.part + align256((size_t)2 * chunks * nb * 256 * 4);
+  w.extra = w.o + align256(S * strips * 256 * 4);
+  w.total = w.extra + align256((size_t)chunks * nb * 256 * 4);
   return w;
 }
+// One chunk of each phase per SM: the phases' streams end together.
+static int few_chunks() { return num_sms(current_device()); }
 
 static int check_few(const FewArgs& a) {
   MOE_REQUIRE(dtype_ok(a.dtype), "few_tokens: bad dtype %d", a.dtype);
@@ -53,7 +77,7 @@ static int check_few(const FewArgs& a) {
   MOE_REQUIRE(a.x && a.out && (a.hidden == 0 || (a.w_gate && a.w_up && a.w_down)),
               "few_tokens: NULL operand");
   MOE_REQUIRE(a.w_router || (a.weights && a.indices), "few_tokens: NULL routing");
-  const FewWorkspace w = few_workspace(a.num_tokens, a.hidden, a.E, a.topk);
+  const FewWorkspace w = few_workspace(a.num_tokens, a.d, a.hidden, a.E, a.topk, a.dtype, few_chunks());
   if (!a.workspace || a.workspace_bytes < w.total)
     return set_error(MOE_ERR_WORKSPACE, "few_tokens: workspace has %zu bytes, needs %zu",
                      a.workspace ? a.workspace_bytes : (size_t)0, w.total);
@@ -106,6 +130,79 @@ static int few_simt_launch(const FewArgs& a, const few::Routing& r, float* h) {
   return MOE_OK;
 }
 
+// 16-bit operands whose rows are 16-byte multiples (TMA and 16-byte copies).
+static bool few_tc_ok(const FewArgs& a) {
+  return a.dtype != MOE_F32 && a.d % 8 == 0 && a.hidden % 8 == 0 && aligned16(a.x) &&
+         aligned16(a.w_gate) && aligned16(a.w_up) && aligned16(a.w_down);
+}
+
+constexpr size_t kMaxSmem = 232448;  // dynamic shared memory a block may have on sm_100
+
+template <int MODE, int FMT, typename T, int NB>
+static int few_kernel_launch(const CUtensorMap* maps, fewtc::Params p, unsigned grid, int table_bytes,
+                             cudaStream_t stream) {
+  auto kern = fewtc::few_kernel<MODE, FMT, T, NB>;
+  const size_t stage = fewtc::kWBytes + NB * 128;
+  const size_t fixed = 1024 + (sizeof(fewtc::Ctl) + 15) / 16 * 16 + (size_t)table_bytes;
+  p.stages = (int)std::min<size_t>(fewtc::kMaxStages, (kMaxSmem - fixed) / stage);
+  MOE_REQUIRE(fixed < kMaxSmem && p.stages > fewtc::kLag, "few rows: routing tables too large");
+  const int dev = current_device();
+  static unsigned long long attr_set = 0;  // per-device bitmask, one per instantiation
+  {
+    std::lock_guard<std::mutex> lock(g_cache_mu);
+    if (dev >= 64 || !(attr_set & (1ull << dev))) {
+      MOE_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem));
+      if (dev < 64) attr_set |= 1ull << dev;
+    }
+  }
+  MOE_CUDA_CHECK(launch_pdl(kern, dim3(grid), dim3(fewtc::kThreads), fixed + p.stages * stage, stream,
+                            maps[0], maps[1], maps[2], p));
+  return MOE_OK;
+}
+
+template <int MODE, int FMT, typename T>
+static int few_kernel_nb(int nb, const CUtensorMap* maps, const fewtc::Params& p, unsigned grid,
+                         int table_bytes, cudaStream_t stream) {
+  if (nb == 16) return few_kernel_launch<MODE, FMT, T, 16>(maps, p, grid, table_bytes, stream);
+  if (nb == 32) return few_kernel_launch<MODE, FMT, T, 32>(maps, p, grid, table_bytes, stream);
+  return few_kernel_launch<MODE, FMT, T, 64>(maps, p, grid, table_bytes, stream);
+}
+
+static int few_weight_map(CUtensorMap* map, const void* w, int dtype, int64_t inner, int64_t rows, int64_t E) {
+  const uint64_t dims[3] = {(uint64_t)inner, (uint64_t)rows, (uint64_t)E};
+  const uint32_t box[3] = {(uint32_t)fewtc::BK, 128, 1};
+  return make_map(map, w, dtype, 3, dims, box);
+}
+
+static int few_tc_launch(const FewArgs& a, const few::Routing& r, const FewWorkspace& w) {
+  CUtensorMap maps[3];
+  int rc;
+  if ((rc = few_weight_map(&maps[0], a.w_gate, a.dtype, a.d, a.hidden, a.E))) return rc;
+  if ((rc = few_weight_map(&maps[1], a.w_up, a.dtype, a.d, a.hidden, a.E))) return rc;
+  if ((rc = few_weight_map(&maps[2], a.w_down, a.dtype, a.hidden, a.d, a.E))) return rc;
+  uint8_t* ws = (uint8_t*)a.workspace;
+  fewtc::Params p = {};
+  p.r = r;
+  p.d = (int)a.d;
+  p.H = (int)a.hidden;
+  p.x = a.x;
+  p.y = a.out;
+  p.h = ws + w.h;
+  p.part = (float*)(ws + w.part);
+  p.o = (float*)(ws + w.o);
+  p.extra = (float*)(ws + w.extra);
+  p.counters = (int*)(ws + w.counters);
+  p.max_chunks = w.max_chunks;
+  p.max_units = w.max_units;
+  p.min_blocks = 2;
+  const int nb = few_nb(a.num_tokens);
+  const int table = few::plan_bytes(r.num_tokens * r.K, r.E, nb);
+  const unsigned grid = (unsigned)w.max_chunks;
+  if (a.dtype == MOE_BF16)
+    return few_kernel_nb<fewtc::kMoe, 1, __nv_bfloat16>(nb, maps, p, grid, table, a.stream);
+  return few_kernel_nb<fewtc::kMoe, 0, __half>(nb, maps, p, grid, table, a.stream);
+}
+
 static int few_tokens_run(const FewArgs& a) {
   int rc = check_few(a);
   if (rc) return rc;
@@ -114,21 +211,29 @@ static int few_tokens_run(const FewArgs& a) {
     MOE_CUDA_CHECK(cudaMemsetAsync(a.out, 0, (size_t)a.num_tokens * a.d * dtype_size(a.dtype), a.stream));
     return MOE_OK;
   }
-  const FewWorkspace w = few_workspace(a.num_tokens, a.hidden, a.E, a.topk);
+  const FewWorkspace w = few_workspace(a.num_tokens, a.d, a.hidden, a.E, a.topk, a.dtype, few_chunks());
   uint8_t* ws = (uint8_t*)a.workspace;
   float* logits = (float*)(ws + w.logits);
+  const bool tc = few_tc_ok(a);
+  int* counters = tc ? (int*)(ws + w.counters) : nullptr;
+  const int num_counters = tc ? w.num_counters : 0;
   few::Routing r = {};
   r.num_tokens = (int)a.num_tokens;
   r.E = a.E;
   r.K = a.topk;
   if (a.w_router) {
-    rc = MOE_DISPATCH_DTYPE(a.dtype, T, [&] { return few_router_launch<T>(a, logits, nullptr, 0); });
+    rc = MOE_DISPATCH_DTYPE(a.dtype, T, [&] { return few_router_launch<T>(a, logits, counters, num_counters); });
     if (rc) return rc;
     r.logits = logits;
   } else {
     r.weights = a.weights;
     r.indices = a.indices;
+    if (tc) {
+      fewtc::zero_counters_kernel<<<1, 256, 0, a.stream>>>(counters, num_counters);
+      MOE_LAUNCH_CHECK();
+    }
   }
+  if (tc) return few_tc_launch(a, r, w);
   return MOE_DISPATCH_DTYPE(a.dtype, T, [&] { return few_simt_launch<T>(a, r, (float*)(ws + w.h)); });
 }
 
@@ -140,10 +245,10 @@ extern "C" {
 
 size_t moe_few_tokens_workspace_bytes(int64_t num_tokens, int64_t d, int64_t hidden,
                                       int32_t num_experts, int32_t topk, int dtype) {
-  (void)d;
-  (void)dtype;
-  if (num_tokens <= 0 || hidden < 0 || num_experts <= 0 || topk <= 0) return 0;
-  return few_workspace(num_tokens, hidden, num_experts, topk).total;
+  if (num_tokens <= 0 || num_tokens > few::kMaxTokens || d < 0 || hidden < 0 || num_experts <= 0 ||
+      topk <= 0 || topk > few::kMaxTopk)
+    return 0;
+  return few_workspace(num_tokens, d, hidden, num_experts, topk, dtype, few_chunks()).total;
 }
 
 int moe_few_tokens_fwd(const void* x, const void* w_router, const float* router_bias,

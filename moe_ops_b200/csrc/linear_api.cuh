@@ -2,6 +2,7 @@
 // moe_b200.cu, whose helpers it uses.
 #pragma once
 
+#include "few_sm100.cuh"
 #include "linear.cuh"
 
 namespace moe {

@@ -60,10 +60,10 @@ def _run(x, route, w_gate, w_up, w_down, dims, K: int, given: bool) -> torch.Ten
                                w_down.contiguous())
     lib = _lib.load()
     y = torch.empty((T, d), device=x.device, dtype=x.dtype)
-    ws_bytes = lib.moe_few_tokens_workspace_bytes(T, d, H, E, K, code)
-    ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8)
     fn = lib.moe_few_experts_fwd if given else lib.moe_few_tokens_fwd
     with torch.cuda.device(x.device):
+        ws_bytes = lib.moe_few_tokens_workspace_bytes(T, d, H, E, K, code)
+        ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8)
         st = fn(x.data_ptr(), _lib.ptr(route[0]), _lib.ptr(route[1]), w_gate.data_ptr(),
                 w_up.data_ptr(), w_down.data_ptr(), code, T, d, H, E, K, y.data_ptr(),
                 ws.data_ptr(), ws_bytes, _lib.stream_of(x))

@@ -362,11 +362,15 @@ int moe_few_experts_fwd(const void* x, const float* weights, const int32_t* indi
  * the backward), or NULL.  Offsets as in moe_gmm_fwd (replaces an moe_gmm_fwd followed by
  * elementwise passes); a dense product is offsets NULL, num_offsets 0, num_experts 1.  Rows
  * behind the last offset get residual (or zero).  residual may not overlap out.  The sum, the
- * bias, the activation and the residual are in fp32; out is rounded once. */
+ * bias, the activation and the residual are in fp32; out is rounded once.  Workspace:
+ * moe_linear_workspace_bytes(...) bytes (0 for many rows: then it may be NULL), 16-byte aligned,
+ * not shared with a call that may run at the same time. */
+size_t moe_linear_workspace_bytes(int64_t m_total, int64_t n, int64_t k, int32_t num_experts,
+                                  int trans_b, int dtype);
 int moe_linear_fwd(const void* A, const void* B, const void* bias, const void* residual, void* out,
                    void* preact, const int32_t* offsets, int32_t num_offsets, int64_t m_total,
                    int64_t n, int64_t k, int32_t num_experts, int trans_b, int activation, int dtype,
-                   void* stream);
+                   void* workspace, size_t workspace_bytes, void* stream);
 /* The elementwise part of its backward: grad_preact = grad_out * act'(preact) and grad_bias
  * [E, n] = its sum over each expert's rows (from the unrounded products, in a fixed order; NULL:
  * not wanted).  For MOE_ACT_NONE grad_preact is grad_out itself: it is not written, and preact

@@ -88,7 +88,8 @@ SIGNATURES = {
     "moe_gmm_wgrad": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i32, _c_i64, _c_i64, _c_i64, _c_i32,
                                _c_int, _c_int, _c_ptr]),
     "moe_linear_fwd": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i32, _c_i64,
-                                _c_i64, _c_i64, _c_i32, _c_int, _c_int, _c_int, _c_ptr]),
+                                _c_i64, _c_i64, _c_i32, _c_int, _c_int, _c_int, _c_ptr, _c_size, _c_ptr]),
+    "moe_linear_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64, _c_i32, _c_int, _c_int]),
     "moe_linear_act_bwd_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i32]),
     "moe_linear_act_bwd": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i32, _c_i64, _c_i64,
                                     _c_i32, _c_int, _c_int, _c_ptr, _c_size, _c_ptr]),

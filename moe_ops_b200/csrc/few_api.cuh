@@ -25,6 +25,9 @@ struct FewArgs {
   cudaStream_t stream;
 };
 
+// Smallest chunk of a phase, in 64-deep blocks of 256 weight rows (32 KB).
+constexpr int kFewMinBlocks = 2;
+
 static size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
 // Rows of a unit of the tensor-core kernel, by the most rows that one expert (one group) can
@@ -194,7 +197,7 @@ static int few_tc_launch(const FewArgs& a, const few::Routing& r, const FewWorks
   p.counters = (int*)(ws + w.counters);
   p.max_chunks = w.max_chunks;
   p.max_units = w.max_units;
-  p.min_blocks = 2;
+  p.min_blocks = kFewMinBlocks;
   const int nb = few_nb(a.num_tokens);
   const int table = few::plan_bytes(r.num_tokens * r.K, r.E, nb);
   const unsigned grid = (unsigned)w.max_chunks;

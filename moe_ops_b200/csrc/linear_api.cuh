@@ -7,6 +7,9 @@
 
 namespace moe {
 
+// Rows up to which the few-row kernel takes a product.
+static int64_t few_linear_max_rows(int E) { return E <= 1 ? 64 : 64; }
+
 struct LinearArgs {
   const void* A;
   const void* B;
@@ -92,6 +95,64 @@ static int linear_tiles(const LinearArgs& a) {
                  : launch_sm100<ML, 1, 0, false, false, __half>(ma, mb, mc, p, a.stream, extra);
 }
 
+// The few-row kernel: its counters and partials for `grid` chunks.
+struct FewLinear {
+  int nb, units, grid;
+  size_t part, total;
+};
+static FewLinear few_linear_plan(int64_t m, int64_t n, int64_t k, int E, bool dense) {
+  FewLinear f = {};
+  f.nb = few_nb(m);
+  f.units = fewtc::row_units_max(m, E, f.nb);
+  f.grid = num_sms(current_device());
+  if (dense) {
+    // all units and blocks are known here: no more blocks than chunks
+    const int64_t blocks = (m + f.nb - 1) / f.nb * ((n + 255) / 256) * ((k + fewtc::BK - 1) / fewtc::BK);
+    f.grid = (int)std::max<int64_t>(1, std::min<int64_t>(f.grid, blocks / kFewMinBlocks));
+  }
+  f.part = align256((size_t)(1 + f.grid + f.units) * 4);
+  f.total = f.part + align256((size_t)2 * f.grid * f.nb * 256 * 4);
+  return f;
+}
+
+static bool few_linear_ok(const LinearArgs& a) {
+  return linear_tc_ok(a) && !a.b_mn && a.m <= few_linear_max_rows(a.E);
+}
+
+static int few_linear(const LinearArgs& a, void* workspace) {
+  const FewLinear f = few_linear_plan(a.m, a.n, a.k, a.E, a.offsets == nullptr);
+  CUtensorMap map;
+  int rc;
+  if ((rc = few_weight_map(&map, a.B, a.dtype, a.k, a.n, a.E))) return rc;
+  uint8_t* ws = (uint8_t*)workspace;
+  fewtc::Params p = {};
+  p.offsets = a.offsets;
+  p.plus_one = a.plus_one;
+  p.E = a.E;
+  p.m = a.m;
+  p.N = (int)a.n;
+  p.K = (int)a.k;
+  p.bias = a.bias;
+  p.residual = a.residual;
+  p.preact = a.preact;
+  p.act = a.act;
+  p.x = a.A;
+  p.y = a.out;
+  p.counters = (int*)ws;
+  p.part = (float*)(ws + f.part);
+  p.max_chunks = f.grid;
+  p.max_units = f.units;
+  p.min_blocks = kFewMinBlocks;
+  const int counters = 1 + f.grid + f.units;
+  fewtc::zero_counters_kernel<<<1, 256, 0, a.stream>>>(p.counters, counters);
+  MOE_LAUNCH_CHECK();
+  const CUtensorMap maps[3] = {map, map, map};
+  const int table = fewtc::row_units_bytes(f.units);
+  if (a.dtype == MOE_BF16)
+    return few_kernel_nb<fewtc::kLinear, 1, __nv_bfloat16>(f.nb, maps, p, (unsigned)f.grid, table, a.stream);
+  return few_kernel_nb<fewtc::kLinear, 0, __half>(f.nb, maps, p, (unsigned)f.grid, table, a.stream);
+}
+
 static int tail_rows(void* out, const void* residual, const int32_t* offsets, int last, int64_t m,
                      int64_t n, int dtype, cudaStream_t s) {
   if (offsets == nullptr || m == 0 || n == 0) return MOE_OK;
@@ -118,17 +179,32 @@ static int check_linear(const void* a, const void* b, const void* out, const int
 
 extern "C" {
 
+size_t moe_linear_workspace_bytes(int64_t m_total, int64_t n, int64_t k, int32_t num_experts,
+                                  int trans_b, int dtype) {
+  if (m_total <= 0 || n <= 0 || k <= 0 || num_experts <= 0 || !trans_b || dtype == MOE_F32 ||
+      m_total > few_linear_max_rows(num_experts))
+    return 0;
+  return few_linear_plan(m_total, n, k, num_experts, false).total;
+}
+
 int moe_linear_fwd(const void* A, const void* B, const void* bias, const void* residual, void* out,
                    void* preact, const int32_t* offsets, int32_t num_offsets, int64_t m_total,
                    int64_t n, int64_t k, int32_t num_experts, int trans_b, int activation, int dtype,
-                   void* stream) {
+                   void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_linear(A, B, out, offsets, num_offsets, m_total, n, k, num_experts, activation, dtype);
   if (rc) return rc;
   if (m_total == 0 || n == 0) return MOE_OK;
   LinearArgs a = {A, B, bias, residual, out, preact, offsets, num_offsets == num_experts + 1,
                   m_total, n, k, num_experts, !trans_b, activation, dtype, (cudaStream_t)stream};
+  const size_t need = moe_linear_workspace_bytes(m_total, n, k, num_experts, trans_b, dtype);
+  if (need && (!workspace || workspace_bytes < need))
+    return set_error(MOE_ERR_WORKSPACE, "linear: workspace has %zu bytes, needs %zu",
+                     workspace ? workspace_bytes : (size_t)0, need);
+  MOE_REQUIRE(!need || aligned16(workspace), "linear: workspace must be 16-byte aligned");
   if (num_experts > 0) {
-    if (linear_tc_ok(a)) {
+    if (few_linear_ok(a)) {
+      rc = few_linear(a, workspace);
+    } else if (linear_tc_ok(a)) {
       rc = linear_tiles(a);
     } else {
       rc = MOE_DISPATCH_DTYPE(dtype, T, [&] { return linear_simt<T>(a); });

@@ -55,11 +55,14 @@ def _forward(x, w, bias, residual, offsets, act: int, trans_b: bool, E: int, n: 
     y = torch.empty((m, n), device=x.device, dtype=x.dtype)
     z = torch.empty_like(y) if want_z else None
     lib = _lib.load()
+    code = _lib.dtype_code(x.dtype)
     with torch.cuda.device(x.device):
+        ws_bytes = lib.moe_linear_workspace_bytes(m, n, k, E, int(trans_b), code)
+        ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8) if ws_bytes else None
         st = lib.moe_linear_fwd(
             x.data_ptr(), w.data_ptr(), _lib.ptr(bias), _lib.ptr(residual), y.data_ptr(), _lib.ptr(z),
             _lib.ptr(offsets), 0 if offsets is None else offsets.numel(), m, n, k, E, int(trans_b),
-            act, _lib.dtype_code(x.dtype), _lib.stream_of(x))
+            act, code, _lib.ptr(ws), ws_bytes, _lib.stream_of(x))
     _lib.check(st, "moe_linear_fwd")
     _lib.count_launches(1)
     return y, z

@@ -15,8 +15,8 @@ def lib():
 def test_c_abi_refusals(lib):
     p = 16
 
-    def fwd(m=4, n=8, k=8, E=1, act=0, dtype=2, num_offsets=0, off=None, a=p):
-        st = lib.moe_linear_fwd(a, p, p, p, p, None, off, num_offsets, m, n, k, E, 1, act, dtype, None)
+    def fwd(m=4, n=8, k=8, E=1, act=0, dtype=2, num_offsets=0, off=None, a=p, ws=1 << 40):
+        st = lib.moe_linear_fwd(a, p, p, p, p, None, off, num_offsets, m, n, k, E, 1, act, dtype, p, ws, None)
         return st, lib.moe_last_error_string()
 
     for kw, word in ((dict(act=5), b"activation"), (dict(act=-1), b"activation"),
@@ -26,6 +26,10 @@ def test_c_abi_refusals(lib):
         st, msg = fwd(**kw)
         assert st == 1 and word in msg, (kw, st, msg)
     assert fwd(m=0)[0] == 0
+    ws = lib.moe_linear_workspace_bytes(4, 8, 8, 1, 1, 2)
+    assert ws > 0 and lib.moe_linear_workspace_bytes(100000, 8, 8, 1, 1, 2) == 0
+    st, msg = fwd(ws=ws - 1)
+    assert st == 4 and b"workspace" in msg
     need = lib.moe_linear_act_bwd_workspace_bytes(300, 64, 3)
     assert need >= 3 * 64 * 4
     st = lib.moe_linear_act_bwd(p, p, p, p, None, 0, 300, 64, 1, 4, 2, p, 8, None)

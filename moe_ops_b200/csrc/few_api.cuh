@@ -25,9 +25,6 @@ struct FewArgs {
   cudaStream_t stream;
 };
 
-// Smallest chunk of a phase, in 64-deep blocks of 256 weight rows (32 KB).
-constexpr int kFewMinBlocks = 2;
-
 static size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
 // Rows of a unit of the tensor-core kernel, by the most rows that one expert (one group) can
@@ -35,35 +32,50 @@ static size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 // crowded expert's weights once.
 static int few_nb(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
+// Chunks a tile's contraction of KB 64-deep blocks is cut into when there are about `tiles`
+// tiles: about 6 chunks per SM, so that SMs of different speed end together, but no chunk under 4
+// blocks (128 KB) nor so small that its partial sums (n rows of 1 KB) weigh against its weights
+// (32 KB a block).
+static int few_parts(double tiles, int64_t KB, int nb) {
+  const double want = 6.0 * num_sms(current_device());
+  int64_t len = (int64_t)(tiles * KB / want);
+  len = std::max<int64_t>(len, std::max(4, nb / 4));
+  len = std::min(len, KB);
+  const int64_t parts = (KB + len - 1) / len;
+  len = (KB + parts - 1) / parts;  // equal chunks, none empty
+  return (int)((KB + len - 1) / len);
+}
+
 // Workspace: logits [T, E] fp32, h [T*K, H] (fp32 for the CUDA cores, else 16 bits), then for
 // the tensor-core kernel its counters and fp32 partial results.
 struct FewWorkspace {
-  size_t logits, h, counters, part, o, extra, total;
-  int num_counters, max_chunks, max_units;
+  size_t logits, h, counters, part0, part1, total;
+  int num_counters, max_units, parts0, parts1;
 };
-static FewWorkspace few_workspace(int64_t T, int64_t d, int64_t H, int64_t E, int64_t K, int dtype,
-                                  int chunks) {
+static FewWorkspace few_workspace(int64_t T, int64_t d, int64_t H, int64_t E, int64_t K, int dtype) {
   FewWorkspace w = {};
-  const size_t S = (size_t)(T * K), strips = (size_t)((d + 255) / 256);
+  const size_t S = (size_t)(T * K), strips = (size_t)((d + 255) / 256), MT = (size_t)((H + 127) / 128);
   w.logits = 0;
   w.h = align256((size_t)T * E * 4);
   w.counters = w.h + align256(S * H * 4);
-  if (dtype == MOE_F32) {
+  if (dtype == MOE_F32 || d == 0 || H == 0) {
     w.total = w.counters;
     return w;
   }
   const int nb = few_nb(T);
-  w.max_chunks = chunks;
+  // experts that T tokens are expected to touch when each picks K of E
+  const double touched = K >= E ? (double)E : E * (1.0 - pow(1.0 - (double)K / E, (double)T));
+  const int64_t KB0 = (d + fewtc::BK - 1) / fewtc::BK, KB1 = (H + fewtc::BK - 1) / fewtc::BK;
+  w.parts0 = few_parts(touched * MT, KB0, nb);
+  if (w.parts0 > 1 && (size_t)w.parts0 * S * MT * 1024 > (64u << 20)) w.parts0 = 1;
+  w.parts1 = few_parts(touched * strips, KB1, nb);
   w.max_units = few::plan_max_units((int)S, (int)E, nb);
-  w.num_counters = 1 + w.max_chunks + w.max_units + (int)strips;
-  w.part = w.counters + align256((size_t)w.num_counters * 4);
-  w.o = w.part + align256((size_t)2 * chunks * nb * 256 * 4);
-  w.extra = w.o + align256(S * strips * 256 * 4);
-  w.total = w.extra + align256((size_t)chunks * nb * 256 * 4);
+  w.num_counters = 1 + (w.parts0 > 1 ? w.max_units * (int)MT : 0) + w.max_units + (int)strips;
+  w.part0 = w.counters + align256((size_t)w.num_counters * 4);
+  w.part1 = w.part0 + (w.parts0 > 1 ? align256((size_t)w.parts0 * S * MT * 1024) : 0);
+  w.total = w.part1 + align256((size_t)w.parts1 * S * strips * 1024);
   return w;
 }
-// One chunk of each phase per SM: the phases' streams end together.
-static int few_chunks() { return num_sms(current_device()); }
 
 static int check_few(const FewArgs& a) {
   MOE_REQUIRE(dtype_ok(a.dtype), "few_tokens: bad dtype %d", a.dtype);
@@ -80,7 +92,7 @@ static int check_few(const FewArgs& a) {
   MOE_REQUIRE(a.x && a.out && (a.hidden == 0 || (a.w_gate && a.w_up && a.w_down)),
               "few_tokens: NULL operand");
   MOE_REQUIRE(a.w_router || (a.weights && a.indices), "few_tokens: NULL routing");
-  const FewWorkspace w = few_workspace(a.num_tokens, a.d, a.hidden, a.E, a.topk, a.dtype, few_chunks());
+  const FewWorkspace w = few_workspace(a.num_tokens, a.d, a.hidden, a.E, a.topk, a.dtype);
   if (!a.workspace || a.workspace_bytes < w.total)
     return set_error(MOE_ERR_WORKSPACE, "few_tokens: workspace has %zu bytes, needs %zu",
                      a.workspace ? a.workspace_bytes : (size_t)0, w.total);
@@ -171,6 +183,12 @@ static int few_kernel_nb(int nb, const CUtensorMap* maps, const fewtc::Params& p
   return few_kernel_launch<MODE, FMT, T, 64>(maps, p, grid, table_bytes, stream);
 }
 
+static int zero_counters(int* counters, int n, cudaStream_t s) {
+  fewtc::zero_counters_kernel<<<std::min(num_sms(current_device()), (n + 511) / 512), 256, 0, s>>>(counters, n);
+  MOE_LAUNCH_CHECK();
+  return MOE_OK;
+}
+
 static int few_weight_map(CUtensorMap* map, const void* w, int dtype, int64_t inner, int64_t rows, int64_t E) {
   const uint64_t dims[3] = {(uint64_t)inner, (uint64_t)rows, (uint64_t)E};
   const uint32_t box[3] = {(uint32_t)fewtc::BK, 128, 1};
@@ -191,16 +209,16 @@ static int few_tc_launch(const FewArgs& a, const few::Routing& r, const FewWorks
   p.x = a.x;
   p.y = a.out;
   p.h = ws + w.h;
-  p.part = (float*)(ws + w.part);
-  p.o = (float*)(ws + w.o);
-  p.extra = (float*)(ws + w.extra);
+  p.rows = r.num_tokens * r.K;
+  p.parts0 = w.parts0;
+  p.parts1 = w.parts1;
+  p.part0 = (float*)(ws + w.part0);
+  p.part1 = (float*)(ws + w.part1);
   p.counters = (int*)(ws + w.counters);
-  p.max_chunks = w.max_chunks;
   p.max_units = w.max_units;
-  p.min_blocks = kFewMinBlocks;
   const int nb = few_nb(a.num_tokens);
   const int table = few::plan_bytes(r.num_tokens * r.K, r.E, nb);
-  const unsigned grid = (unsigned)w.max_chunks;
+  const unsigned grid = (unsigned)num_sms(current_device());
   if (a.dtype == MOE_BF16)
     return few_kernel_nb<fewtc::kMoe, 1, __nv_bfloat16>(nb, maps, p, grid, table, a.stream);
   return few_kernel_nb<fewtc::kMoe, 0, __half>(nb, maps, p, grid, table, a.stream);
@@ -214,7 +232,7 @@ static int few_tokens_run(const FewArgs& a) {
     MOE_CUDA_CHECK(cudaMemsetAsync(a.out, 0, (size_t)a.num_tokens * a.d * dtype_size(a.dtype), a.stream));
     return MOE_OK;
   }
-  const FewWorkspace w = few_workspace(a.num_tokens, a.d, a.hidden, a.E, a.topk, a.dtype, few_chunks());
+  const FewWorkspace w = few_workspace(a.num_tokens, a.d, a.hidden, a.E, a.topk, a.dtype);
   uint8_t* ws = (uint8_t*)a.workspace;
   float* logits = (float*)(ws + w.logits);
   const bool tc = few_tc_ok(a);
@@ -232,8 +250,7 @@ static int few_tokens_run(const FewArgs& a) {
     r.weights = a.weights;
     r.indices = a.indices;
     if (tc) {
-      fewtc::zero_counters_kernel<<<1, 256, 0, a.stream>>>(counters, num_counters);
-      MOE_LAUNCH_CHECK();
+      if ((rc = zero_counters(counters, num_counters, a.stream))) return rc;
     }
   }
   if (tc) return few_tc_launch(a, r, w);
@@ -251,7 +268,7 @@ size_t moe_few_tokens_workspace_bytes(int64_t num_tokens, int64_t d, int64_t hid
   if (num_tokens <= 0 || num_tokens > few::kMaxTokens || d < 0 || hidden < 0 || num_experts <= 0 ||
       topk <= 0 || topk > few::kMaxTopk)
     return 0;
-  return few_workspace(num_tokens, d, hidden, num_experts, topk, dtype, few_chunks()).total;
+  return few_workspace(num_tokens, d, hidden, num_experts, topk, dtype).total;
 }
 
 int moe_few_tokens_fwd(const void* x, const void* w_router, const float* router_bias,

@@ -16,16 +16,20 @@
 //            p * result over the slots in order.
 //   kLinear  one phase: 256 weight rows times up to NB rows; bias, activation, residual.
 //
-// Work split.  A phase is a flat list of 64-deep blocks (tile-major), cut into G chunks of equal
-// size whatever the sizes are, so every SM streams the same number of bytes.  A tile cut by a
-// chunk border leaves fp32 partials; the chunk that finds the tile complete (an atomic counter
-// of finished blocks) adds them in chunk order, so results do not depend on timing.
+// Work split.  Every tile's contraction is cut into `parts` chunks (fixed by the host from the
+// sizes, so results do not depend on routing or timing), small enough for about
+// kChunksPerSm chunks per SM: SMs do not all stream equally fast, and with one equal share each
+// the slowest held the others up (one token, d = 4096, H = 11008: 15 us of 115).  An atomic
+// ticket hands the chunks out in order, phase 0's before phase 1's.  A block waits only for
+// chunks with smaller tickets, each of which a running block has taken and finishes without
+// waiting for a later one: the kernel makes progress whatever share of its blocks is resident.
+// Partial sums are fp32 and added in chunk order: those of h by the block that finishes a tile
+// last, those of the outputs in a final stage that all blocks share once the tickets are used
+// up.
 //
-// kMoe's chunks are handed out by an atomic ticket, phase 0's before phase 1's.  A block waits
-// only for phase-0 chunks, each of which a running block has taken and finishes without waiting
-// for anyone: the kernel makes progress whatever share of its blocks is resident.  The weight
-// producer never waits for h, so the ring (about 200 KB per SM) fills with Wd while the last h
-// tiles are finished: the stream does not stop between the phases.
+// The weight producer never waits for h, so the ring (about 200 KB per SM) fills with Wd while
+// the last h tiles are finished.  Phase 1 goes unit by unit in phase 0's order, so that the h
+// it needs first was finished first: the stream does not stop between the phases.
 //
 // Warp roles (256 threads, one block per SM):
 //   warp 0      weights: TMA boxes of 64 x 128, 128-byte swizzle; also fetches the tickets.
@@ -60,9 +64,6 @@ struct Params {
   few::Routing r;
   int d, H;
   void* h;       // [S, H]
-  float* o;      // [S, strips * 256] results of phase 1 (each tile's first chunk)
-  float* extra;  // [max_chunks, NB, 256] the other chunks of a tile
-  void* y;       // [T, d]; kLinear: [m, N]
   // kLinear
   const int32_t* offsets;
   int plus_one, E;
@@ -74,18 +75,25 @@ struct Params {
   int act;
   // both
   const void* x;     // activations, rows of d (K) elements
-  float* part;       // [2 * max_chunks, NB, 256] partials of phase 0 (kLinear: of the phase)
-  int* counters;     // zeroed before the launch: ticket, tile[max_chunks], done[units], strip[]
-  int max_chunks, max_units;
-  int min_blocks;    // blocks of a chunk, at least
+  void* y;           // [T, d]; kLinear: [m, N]
+  int parts0, parts1;  // chunks per tile of each phase
+  float* part0;      // [parts0, rows, MT * 256] partials of phase 0 (parts0 > 1); rows: S or m
+  float* part1;      // [parts1, S, strips * 256] results of phase 1
+  int rows;          // S (kMoe) or m
+  int* counters;     // zeroed before the launch: ticket; tile[max_units * MT] finished chunks of
+                     // a tile (parts0 > 1); kMoe: done[max_units] finished h tiles, strip[strips]
+                     // finished chunks of a 256-column strip of y
+  int max_units;
   int stages;
 };
+
+constexpr int kTickets = 4;  // ticket ring
 
 struct Ctl {
   uint64_t full[kMaxStages], empty[kMaxStages];
   uint64_t tmem_full[2], tmem_empty[2];
-  uint64_t tk_full[2], tk_empty[2];
-  int tk[2];
+  uint64_t tk_full[kTickets], tk_empty[kTickets];
+  int tk[kTickets];
   uint32_t tmem_base;
   int abort;
   int flag;
@@ -103,21 +111,23 @@ __host__ __device__ inline int row_units_max(int64_t m, int E, int nb) {
 }
 __host__ __device__ inline int row_units_bytes(int units) { return (8 * units + 15) / 16 * 16; }
 
-// A phase's blocks: `tiles` tiles of KB blocks, cut into G chunks.
-struct Phase {
-  int KB;
-  long long total;
-  int G;
-  __device__ __forceinline__ void set(long long tiles, int kb, int max_chunks, int min_blocks) {
-    KB = kb;
-    total = tiles * kb;
-    const long long g = total / min_blocks;
-    G = total == 0 ? 0 : (int)(g < 1 ? 1 : (g < max_chunks ? g : max_chunks));
-  }
-  __device__ __forceinline__ long long begin(int c) const { return c * total / G; }
-  // The chunk that holds block b: the largest c with begin(c) <= b.
-  __device__ __forceinline__ int chunk_of(long long b) const { return (int)(((b + 1) * G - 1) / total); }
-};
+// Contraction blocks [first, first + len) of chunk `part` of a tile of KB blocks.
+__device__ __forceinline__ void part_range(int KB, int parts, int part, int& first, int& len) {
+  const int L = (KB + parts - 1) / parts;
+  first = part * L;
+  len = min(L, KB - first);
+}
+
+// kLinear's epilogue on one element: z = the sum and the bias.
+template <typename T>
+__device__ __forceinline__ void linear_out(const Params& p, int64_t row, int col, float z) {
+  if (col >= p.N) return;
+  const int64_t at = row * p.N + col;
+  if (p.preact) static_cast<T*>(p.preact)[at] = from_f32<T>(z);
+  float y = act_fwd_rt(p.act, z);
+  if (p.residual) y += to_f32(static_cast<const T*>(p.residual)[at]);
+  static_cast<T*>(p.y)[at] = from_f32<T>(y);
+}
 
 template <int MODE, int FMT, typename T, int NB>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -141,6 +151,8 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(ptx::smem_u32(&s.tmem_full[i]), 1);
       ptx::mbar_init(ptx::smem_u32(&s.tmem_empty[i]), 4);
+    }
+    for (int i = 0; i < kTickets; ++i) {
       ptx::mbar_init(ptx::smem_u32(&s.tk_full[i]), 1);
       ptx::mbar_init(ptx::smem_u32(&s.tk_empty[i]), 7);
     }
@@ -210,155 +222,129 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
   ptx::tc_fence_after();
   const int U = MODE == kMoe ? *plan.num_units : s.num_units;
   const uint32_t tmem_base = s.tmem_base;
-  // Tiles per unit and 64-deep blocks per tile of each phase.
+  // Tiles per unit, 64-deep blocks per tile and chunks of each phase.
   const int MT = MODE == kMoe ? (p.H + 127) / 128 : (p.N + 255) / 256;
-  const int strips = (p.d + 255) / 256;
-  Phase ph0, ph1;
-  ph0.set((long long)U * MT, ((MODE == kMoe ? p.d : p.K) + BK - 1) / BK, p.max_chunks, p.min_blocks);
-  if (MODE == kMoe) ph1.set((long long)U * strips, (p.H + BK - 1) / BK, p.max_chunks, p.min_blocks);
-  else { ph1.KB = 1; ph1.total = 0; ph1.G = 0; }
+  const int strips = MODE == kMoe ? (p.d + 255) / 256 : 0;
+  const int KB0 = ((MODE == kMoe ? p.d : p.K) + BK - 1) / BK, KB1 = (p.H + BK - 1) / BK;
+  const int G0 = U * MT * p.parts0, G1 = MODE == kMoe ? U * strips * p.parts1 : 0;
   int* const c_tile = p.counters + 1;
-  int* const c_done = c_tile + p.max_chunks;
+  int* const c_done = c_tile + (p.parts0 > 1 ? p.max_units * MT : 0);
   int* const c_strip = c_done + p.max_units;
 
-  auto unit = [&](int u, int& e, int& row0, int& n) {
-    if constexpr (MODE == kMoe) { e = plan.unit_e[u]; row0 = plan.unit_pos[u]; n = plan.unit_n[u]; }
-    else { e = ru.e[u]; row0 = ru.row[u]; n = ru.n[u]; }
+  // Chunk t: unit u (expert e, first row row0, n rows), tile mt, blocks [kb0, kb0 + len).
+  struct Chunk {
+    int phase, u, mt, part, kb0, len, e, row0, n;
   };
-  // Tile q of phase 1 is (strip, unit), strip-major; of phase 0 (unit, tile).
-  auto decode = [&](int phase, long long q, int& u, int& mt) {
-    if (phase) { mt = (int)(q / U); u = (int)(q % U); }
-    else { u = (int)(q / MT); mt = (int)(q % MT); }
+  auto decode = [&](int t) {
+    Chunk c;
+    c.phase = MODE == kMoe && t >= G0;
+    const int i = c.phase ? t - G0 : t;
+    const int parts = c.phase ? p.parts1 : p.parts0, tiles = c.phase ? strips : MT;
+    const int q = i / parts;
+    c.part = i - q * parts;
+    c.u = q / tiles;
+    c.mt = q - c.u * tiles;
+    part_range(c.phase ? KB1 : KB0, parts, c.part, c.kb0, c.len);
+    if constexpr (MODE == kMoe) {
+      c.e = plan.unit_e[c.u]; c.row0 = plan.unit_pos[c.u]; c.n = plan.unit_n[c.u];
+    } else {
+      c.e = ru.e[c.u]; c.row0 = ru.row[c.u]; c.n = ru.n[c.u];
+    }
+    return c;
   };
   // A whole warp's wait: every lane leaves with the same answer, so that no lane meets a warp
   // barrier that another has skipped.
   auto warp_wait = [&](uint64_t& bar, uint32_t parity) {
     return __all_sync(0xffffffffu, ptx::wait_bounded(ptx::smem_u32(&bar), parity, abort_flag, kWaitNs)) != 0;
   };
-  // The it-th ticket of this block (kLinear: its one chunk); false at the end.
-  auto ticket = [&](int it, int& phase, int& c) -> bool {
-    int t;
-    if constexpr (MODE == kMoe) {
-      const int slot = it & 1;
-      if (!warp_wait(s.tk_full[slot], (it >> 1) & 1)) return false;
-      t = *(volatile int*)&s.tk[slot];
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&s.tk_empty[slot]));
-    } else {
-      t = it == 0 ? (int)blockIdx.x : ph0.G;
-    }
-    phase = t >= ph0.G;
-    c = phase ? t - ph0.G : t;
-    return t < ph0.G + ph1.G;
+  // This block's it-th ticket, for the warps that follow the producer; false at the end.
+  auto ticket = [&](int it, Chunk& c) -> bool {
+    const int slot = it % kTickets;
+    if (!warp_wait(s.tk_full[slot], (it / kTickets) & 1)) return false;
+    const int t = *(volatile int*)&s.tk[slot];
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&s.tk_empty[slot]));
+    if (t >= G0 + G1) return false;
+    c = decode(t);
+    return true;
   };
 
-  if (MODE == kMoe && U == 0) {
-    // Every slot is dropped: y is zero.
-    T* y = static_cast<T*>(p.y);
-    const int64_t n = (int64_t)p.r.num_tokens * p.d;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads)
-      y[i] = from_f32<T>(0.f);
-  } else if (warp == 0) {
+  if (warp == 0) {
     // ---------------------------------------------------------- weights
     if (lane == 0) {
+      if (MODE == kLinear) pdl_wait();  // the counters are zeroed
       int stage = 0;
       uint32_t parity = 1;
       bool ok = true;
       for (int it = 0; ok; ++it) {
-        int t;
-        if constexpr (MODE == kMoe) {
-          const int slot = it & 1;
-          if (!ptx::wait_bounded(ptx::smem_u32(&s.tk_empty[slot]), ((it >> 1) & 1) ^ 1, abort_flag, kWaitNs)) break;
-          t = atomicAdd(p.counters, 1);
-          *(volatile int*)&s.tk[slot] = t;
-          ptx::mbar_arrive(ptx::smem_u32(&s.tk_full[slot]));
-        } else {
-          t = it == 0 ? (int)blockIdx.x : ph0.G;
-        }
-        if (t >= ph0.G + ph1.G) break;
-        const int phase = t >= ph0.G;
-        const Phase& ph = phase ? ph1 : ph0;
-        const int c = phase ? t - ph0.G : t;
-        long long b = ph.begin(c);
-        const long long end = ph.begin(c + 1);
-        while (b < end && ok) {
-          const long long q = b / ph.KB;
-          const int kb0 = (int)(b - q * ph.KB);
-          const int len = (int)min((long long)(ph.KB - kb0), end - b);
-          int u, mt, e, row0, n;
-          decode(phase, q, u, mt);
-          unit(u, e, row0, n);
-          const CUtensorMap* m0 = MODE == kMoe && phase ? &map2 : &map0;
-          const CUtensorMap* m1 = MODE == kMoe && !phase ? &map1 : m0;
-          const int r0 = MODE == kMoe && !phase ? mt * 128 : mt * 256;
-          const int r1 = MODE == kMoe && !phase ? r0 : r0 + 128;
-          for (int kb = kb0; kb < kb0 + len; ++kb) {
-            if (!ptx::wait_bounded(ptx::smem_u32(&s.empty[stage]), parity, abort_flag, kWaitNs)) { ok = false; break; }
-            const uint32_t bar = ptx::smem_u32(&s.full[stage]);
-            const uint32_t dst = ptx::smem_u32(smem) + stage * kStage;
-            ptx::mbar_arrive_expect_tx(bar, kWBytes);
-            ptx::tma_load_3d(dst, m0, bar, kb * BK, r0, e);
-            ptx::tma_load_3d(dst + kBoxBytes, m1, bar, kb * BK, r1, e);
-            if (++stage == ST) { stage = 0; parity ^= 1; }
-          }
-          b += len;
+        const int slot = it % kTickets;
+        // The next ticket is taken when the last chunk's loads have been issued, so a slower
+        // SM takes fewer; its latency hides behind the ring.
+        if (!ptx::wait_bounded(ptx::smem_u32(&s.tk_empty[slot]), ((it / kTickets) & 1) ^ 1, abort_flag, kWaitNs)) break;
+        const int t = atomicAdd(p.counters, 1);
+        *(volatile int*)&s.tk[slot] = t;
+        ptx::mbar_arrive(ptx::smem_u32(&s.tk_full[slot]));
+        if (t >= G0 + G1) break;
+        const Chunk c = decode(t);
+        const bool gate_up = MODE == kMoe && !c.phase;
+        const CUtensorMap* m0 = MODE == kMoe && c.phase ? &map2 : &map0;
+        const CUtensorMap* m1 = gate_up ? &map1 : m0;
+        const int r0 = gate_up ? c.mt * 128 : c.mt * 256;
+        const int r1 = gate_up ? r0 : r0 + 128;
+        for (int kb = c.kb0; kb < c.kb0 + c.len; ++kb) {
+          if (!ptx::wait_bounded(ptx::smem_u32(&s.empty[stage]), parity, abort_flag, kWaitNs)) { ok = false; break; }
+          const uint32_t bar = ptx::smem_u32(&s.full[stage]);
+          const uint32_t dst = ptx::smem_u32(smem) + stage * kStage;
+          ptx::mbar_arrive_expect_tx(bar, kWBytes);
+          ptx::tma_load_3d(dst, m0, bar, kb * BK, r0, c.e);
+          ptx::tma_load_3d(dst + kBoxBytes, m1, bar, kb * BK, r1, c.e);
+          if (++stage == ST) { stage = 0; parity ^= 1; }
         }
       }
     }
     __syncwarp();
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA
-    int stage = 0, seg = 0, phase, c;
+    int stage = 0;
     uint32_t parity = 0;
     bool ok = true;
-    for (int it = 0; ok && ticket(it, phase, c); ++it) {
-      const Phase& ph = phase ? ph1 : ph0;
-      long long b = ph.begin(c);
-      const long long end = ph.begin(c + 1);
-      while (b < end && ok) {
-        const long long q = b / ph.KB;
-        const int kb0 = (int)(b - q * ph.KB);
-        const int len = (int)min((long long)(ph.KB - kb0), end - b);
-        int u, mt, e, row0, n;
-        decode(phase, q, u, mt);
-        unit(u, e, row0, n);
-        const uint32_t idesc = ptx::make_idesc_f16(FMT, 0, 0, 128, (n + 15) / 16 * 16);
-        const int buf = seg & 1;
-        if (!warp_wait(s.tmem_empty[buf], ((seg >> 1) & 1) ^ 1)) { ok = false; break; }
+    Chunk c;
+    for (int it = 0; ok && ticket(it, c); ++it) {
+      const uint32_t idesc = ptx::make_idesc_f16(FMT, 0, 0, 128, (c.n + 15) / 16 * 16);
+      const int buf = it & 1;
+      if (!warp_wait(s.tmem_empty[buf], ((it >> 1) & 1) ^ 1)) break;
+      ptx::tc_fence_after();
+      const uint32_t d0 = tmem_base + buf * 2 * NB;
+      for (int i = 0; i < c.len; ++i) {
+        if (!warp_wait(s.full[stage], parity)) { ok = false; break; }
         ptx::tc_fence_after();
-        const uint32_t d0 = tmem_base + buf * 2 * NB;
-        for (int i = 0; i < len; ++i) {
-          if (!warp_wait(s.full[stage], parity)) { ok = false; break; }
-          ptx::tc_fence_after();
-          if (lane == 0) {
-            const uint32_t sa = ptx::smem_u32(smem) + stage * kStage;
-            const uint32_t sb = sa + kWBytes;
+        if (lane == 0) {
+          const uint32_t sa = ptx::smem_u32(smem) + stage * kStage;
+          const uint32_t sb = sa + kWBytes;
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-              const uint64_t bd = ptx::make_sw128_desc(sb + kk * 32, 16, 1024);
-              ptx::mma_f16_ss<1>(d0, ptx::make_sw128_desc(sa + kk * 32, 16, 1024), bd, idesc, (i | kk) != 0);
-              ptx::mma_f16_ss<1>(d0 + NB, ptx::make_sw128_desc(sa + kBoxBytes + kk * 32, 16, 1024), bd,
-                                 idesc, (i | kk) != 0);
-            }
-            ptx::mma_commit<1>(ptx::smem_u32(&s.empty[stage]));
+          for (int kk = 0; kk < 4; ++kk) {
+            const uint64_t bd = ptx::make_sw128_desc(sb + kk * 32, 16, 1024);
+            ptx::mma_f16_ss<1>(d0, ptx::make_sw128_desc(sa + kk * 32, 16, 1024), bd, idesc, (i | kk) != 0);
+            ptx::mma_f16_ss<1>(d0 + NB, ptx::make_sw128_desc(sa + kBoxBytes + kk * 32, 16, 1024), bd,
+                               idesc, (i | kk) != 0);
           }
-          __syncwarp();
-          if (++stage == ST) { stage = 0; parity ^= 1; }
+          ptx::mma_commit<1>(ptx::smem_u32(&s.empty[stage]));
         }
-        if (!ok) break;
-        if (lane == 0) ptx::mma_commit<1>(ptx::smem_u32(&s.tmem_full[buf]));
         __syncwarp();
-        ++seg;
-        b += len;
+        if (++stage == ST) { stage = 0; parity ^= 1; }
       }
+      if (!ok) break;
+      if (lane == 0) ptx::mma_commit<1>(ptx::smem_u32(&s.tmem_full[buf]));
+      __syncwarp();
     }
   } else if (warp < 4) {
     // ---------------------------------------------------------- activations
     const int l64 = (warp - 2) * 32 + lane;
     const int c16 = l64 & 7;  // 16-byte column of a 128-byte row
-    int stage = 0, held = 0, held_stage = 0, phase, c;
+    int stage = 0, held = 0, held_stage = 0;
     uint32_t parity = 1;
     bool ok = true;
+    Chunk c;
     // Hands over the oldest `count` stages whose copies have landed.
     auto hand_over = [&](int count) {
       ptx::fence_proxy_async_smem();
@@ -370,213 +356,213 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
       held -= count;
     };
     auto drain = [&]() {
+      if (held == 0) return;
       ptx::cp_async_wait<0>();
       hand_over(held);
     };
     for (int it = 0; ok; ++it) {
-      drain();  // nothing is held back while this warp waits for a ticket
-      if (!ticket(it, phase, c)) break;
-      const Phase& ph = phase ? ph1 : ph0;
-      long long b = ph.begin(c);
-      const long long end = ph.begin(c + 1);
-      while (b < end && ok) {
-        const long long q = b / ph.KB;
-        const int kb0 = (int)(b - q * ph.KB);
-        const int len = (int)min((long long)(ph.KB - kb0), end - b);
-        int u, mt, e, row0, n;
-        decode(phase, q, u, mt);
-        unit(u, e, row0, n);
-        const int cols = MODE == kLinear ? p.K : phase ? p.H : p.d;
-        const T* rows[NB / 8];
+      // Nothing is held back while this warp waits for a ticket (or, below, for h).
+      if (!__all_sync(0xffffffffu, ptx::mbar_try_wait(ptx::smem_u32(&s.tk_full[it % kTickets]),
+                                                      (it / kTickets) & 1)))
+        drain();
+      if (!ticket(it, c)) break;
+      const int cols = MODE == kLinear ? p.K : c.phase ? p.H : p.d;
+      const T* rows[NB / 8];
+#pragma unroll
+      for (int i = 0; i < NB / 8; ++i) {
+        const int r = (l64 >> 3) + 8 * i;
+        int64_t src = c.row0 + (r < c.n ? r : 0);
+        if (MODE == kMoe && !c.phase) src = plan.slot[src] / p.r.K;
+        rows[i] = static_cast<const T*>(MODE == kMoe && c.phase ? p.h : p.x) + src * cols + c16 * 8;
+      }
+      if (MODE == kMoe && c.phase) {
+        // the unit's h: every one of its MT tiles finished
+        if (!__all_sync(0xffffffffu, ptx::ld_acquire_gpu(c_done + c.u) >= MT)) {
+          drain();
+          const uint64_t t0 = ptx::globaltimer();
+          while (ptx::ld_acquire_gpu(c_done + c.u) < MT) {
+            if (*abort_flag || ptx::globaltimer() - t0 > kWaitNs) { *abort_flag = 1; ok = false; break; }
+            __nanosleep(32);
+          }
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
+      }
+      for (int kb = c.kb0; kb < c.kb0 + c.len; ++kb) {
+        if (!warp_wait(s.empty[stage], parity)) { ok = false; break; }
+        const uint32_t dst = ptx::smem_u32(smem) + stage * kStage + kWBytes;
+        const bool in = kb * BK + c16 * 8 < cols;  // cols is a multiple of 8
 #pragma unroll
         for (int i = 0; i < NB / 8; ++i) {
           const int r = (l64 >> 3) + 8 * i;
-          int64_t src = row0 + (r < n ? r : 0);
-          if (MODE == kMoe && !phase) src = plan.slot[src] / p.r.K;
-          rows[i] = static_cast<const T*>(phase ? p.h : p.x) + src * cols + c16 * 8;
+          if (r < c.n)
+            ptx::cp_async16(dst + r * 128 + ((c16 ^ (r & 7)) << 4),
+                            rows[i] + (in ? kb * BK : -(c16 * 8)), in ? 16u : 0u);
         }
-        if (MODE == kMoe && phase) {
-          // the unit's h: every one of its MT tiles finished
-          if (!__all_sync(0xffffffffu, ptx::ld_acquire_gpu(c_done + u) >= MT)) {
-            drain();
-            const uint64_t t0 = ptx::globaltimer();
-            while (ptx::ld_acquire_gpu(c_done + u) < MT) {
-              if (*abort_flag || ptx::globaltimer() - t0 > kWaitNs) { *abort_flag = 1; ok = false; break; }
-              __nanosleep(64);
-            }
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-          }
+        ptx::cp_async_commit();
+        if (++stage == ST) { stage = 0; parity ^= 1; }
+        if (++held > kLag) {
+          ptx::cp_async_wait<kLag>();
+          hand_over(1);
         }
-        for (int kb = kb0; kb < kb0 + len; ++kb) {
-          if (!warp_wait(s.empty[stage], parity)) { ok = false; break; }
-          const uint32_t dst = ptx::smem_u32(smem) + stage * kStage + kWBytes;
-          const bool in = kb * BK + c16 * 8 < cols;  // cols is a multiple of 8
-#pragma unroll
-          for (int i = 0; i < NB / 8; ++i) {
-            const int r = (l64 >> 3) + 8 * i;
-            if (r < n)
-              ptx::cp_async16(dst + r * 128 + ((c16 ^ (r & 7)) << 4),
-                              rows[i] + (in ? kb * BK : -(c16 * 8)), in ? 16u : 0u);
-          }
-          ptx::cp_async_commit();
-          if (++stage == ST) { stage = 0; parity ^= 1; }
-          if (++held > kLag) {
-            ptx::cp_async_wait<kLag>();
-            hand_over(1);
-          }
-        }
-        b += len;
       }
     }
-    ptx::cp_async_wait<0>();
+    drain();
   } else {
     // ---------------------------------------------------------- epilogue
     const int row = (warp - 4) * 32 + lane;  // accumulator lane
     const bool lead = row == 0;
-    int seg = 0, phase, c;
-    bool ok = true;
-    if (MODE == kLinear) pdl_wait();  // the counters are zeroed
+    const int64_t ld0 = (int64_t)MT * 256, ld1 = (int64_t)strips * 256;
+    Chunk c;
     // The four warps meet at barriers, so each wait's outcome is agreed on by all of them.
-    for (int it = 0; ok; ++it) {
-      const bool more = ticket(it, phase, c);
+    for (int it = 0;; ++it) {
+      const bool more = ticket(it, c);
       if (!ptx::named_barrier_all(1, 128, more)) break;
-      const Phase& ph = phase ? ph1 : ph0;
-      long long b = ph.begin(c);
-      const long long end = ph.begin(c + 1);
-      for (; b < end && ok; ++seg) {
-        const long long q = b / ph.KB;
-        const int kb0 = (int)(b - q * ph.KB);
-        const int len = (int)min((long long)(ph.KB - kb0), end - b);
-        b += len;
-        int u, mt, e, row0, n;
-        decode(phase, q, u, mt);
-        unit(u, e, row0, n);
-        const int buf = seg & 1;
-        ok = ptx::named_barrier_all(1, 128, warp_wait(s.tmem_full[buf], (seg >> 1) & 1));
-        if (!ok) break;
-        ptx::tc_fence_after();
-        const uint32_t tb = tmem_base + ((uint32_t)((warp - 4) * 32) << 16) + buf * 2 * NB;
-        const bool whole = len == ph.KB && !phase;
-        // Applies the tile's epilogue to row j of the unit (v0, v1: this thread's D0 and D1).
-        float bias0 = 0.f, bias1 = 0.f;
-        const int col0 = MODE == kMoe ? mt * 128 + row : mt * 256 + row, col1 = col0 + 128;
-        if (MODE == kLinear && p.bias) {
-          const T* bp = static_cast<const T*>(p.bias) + (int64_t)e * p.N;
-          if (col0 < p.N) bias0 = to_f32(bp[col0]);
-          if (col1 < p.N) bias1 = to_f32(bp[col1]);
-        }
-        auto finish = [&](int j, float v0, float v1) {
-          if constexpr (MODE == kMoe) {
-            if (col0 < p.H)
-              static_cast<T*>(p.h)[(int64_t)(row0 + j) * p.H + col0] = from_f32<T>(v0 * sigmoid_f32(v0) * v1);
-          } else {
-            const int64_t at = (int64_t)(row0 + j) * p.N;
-            auto put = [&](int col, float z) {
-              if (col >= p.N) return;
-              if (p.preact) static_cast<T*>(p.preact)[at + col] = from_f32<T>(z);
-              float y = act_fwd_rt(p.act, z);
-              if (p.residual) y += to_f32(static_cast<const T*>(p.residual)[at + col]);
-              static_cast<T*>(p.y)[at + col] = from_f32<T>(y);
-            };
-            put(col0, v0 + bias0);
-            put(col1, v1 + bias1);
-          }
-        };
-        // Where the partial sums of a cut tile (or of any phase-1 tile) go: [row][256].
-        float* dst;
-        int64_t pitch = 256;
-        if (phase) {
-          if (kb0 == 0) { pitch = (int64_t)strips * 256; dst = p.o + row0 * pitch + mt * 256; }
-          else dst = p.extra + (int64_t)c * NB * 256;
+      const int buf = it & 1;
+      if (!ptx::named_barrier_all(1, 128, warp_wait(s.tmem_full[buf], (it >> 1) & 1))) break;
+      ptx::tc_fence_after();
+      const uint32_t tb = tmem_base + ((uint32_t)((warp - 4) * 32) << 16) + buf * 2 * NB;
+      const bool whole = !c.phase && p.parts0 == 1;
+      const int col0 = MODE == kMoe ? c.mt * 128 + row : c.mt * 256 + row, col1 = col0 + 128;
+      float bias0 = 0.f, bias1 = 0.f;
+      if (MODE == kLinear && p.bias && whole) {
+        const T* bp = static_cast<const T*>(p.bias) + (int64_t)c.e * p.N;
+        if (col0 < p.N) bias0 = to_f32(bp[col0]);
+        if (col1 < p.N) bias1 = to_f32(bp[col1]);
+      }
+      // The tile's epilogue on row j of the unit (v0, v1: this thread's D0 and D1).
+      auto finish = [&](int j, float v0, float v1) {
+        if constexpr (MODE == kMoe) {
+          if (col0 < p.H)
+            static_cast<T*>(p.h)[(int64_t)(c.row0 + j) * p.H + col0] = from_f32<T>(v0 * sigmoid_f32(v0) * v1);
         } else {
-          dst = p.part + ((int64_t)2 * c + (kb0 == 0)) * NB * 256;
+          linear_out<T>(p, c.row0 + j, col0, v0 + bias0);
+          linear_out<T>(p, c.row0 + j, col1, v1 + bias1);
         }
-        for (int j0 = 0; j0 < n; j0 += 16) {
-          uint32_t v0[16], v1[16];
-          ptx::tmem_ld_32x32b_x16(tb + j0, v0);
-          ptx::tmem_ld_32x32b_x16(tb + NB + j0, v1);
-          ptx::tmem_wait_ld();
+      };
+      // Partial sums: this thread's two columns of the tile, row by row.
+      const int64_t ld = c.phase ? ld1 : ld0;
+      float* dst = (c.phase ? p.part1 : p.part0) + ((int64_t)c.part * p.rows + c.row0) * ld + c.mt * 256 + row;
+      for (int j0 = 0; j0 < c.n; j0 += 16) {
+        uint32_t v0[16], v1[16];
+        ptx::tmem_ld_32x32b_x16(tb + j0, v0);
+        ptx::tmem_ld_32x32b_x16(tb + NB + j0, v1);
+        ptx::tmem_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if (j0 + j < n) {
-              const float a = __uint_as_float(v0[j]), g = __uint_as_float(v1[j]);
-              if (whole) finish(j0 + j, a, g);
-              else {
-                dst[(j0 + j) * pitch + row] = a;
-                dst[(j0 + j) * pitch + 128 + row] = g;
-              }
+        for (int j = 0; j < 16; ++j) {
+          if (j0 + j < c.n) {
+            const float a = __uint_as_float(v0[j]), g = __uint_as_float(v1[j]);
+            if (whole) finish(j0 + j, a, g);
+            else {
+              dst[(j0 + j) * ld] = a;
+              dst[(j0 + j) * ld + 128] = g;
             }
-          }
-        }
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&s.tmem_empty[buf]));
-
-        if (!phase) {
-          if (!whole) {
-            // Cut tile: the chunk that completes its block count adds the partials in order.
-            const int f = ph.chunk_of(q * ph.KB), l = ph.chunk_of(q * ph.KB + ph.KB - 1);
-            __threadfence();
-            ptx::named_barrier(1, 128);
-            if (lead) s.flag = ptx::atom_add_acq_rel_gpu(c_tile + f, len) + len == ph.KB;
-            ptx::named_barrier(1, 128);
-            if (!*(volatile int*)&s.flag) continue;
-            __threadfence();
-            for (int j = 0; j < n; ++j) {
-              const float* src = p.part + ((int64_t)(2 * f + 1) * NB + j) * 256 + row;
-              float a = __ldcg(src), g = __ldcg(src + 128);
-              for (int cc = f + 1; cc <= l; ++cc) {
-                src = p.part + ((int64_t)2 * cc * NB + j) * 256 + row;
-                a += __ldcg(src);
-                g += __ldcg(src + 128);
-              }
-              finish(j, a, g);
-            }
-          }
-          if (MODE == kMoe) {
-            __threadfence();
-            ptx::named_barrier(1, 128);
-            if (lead) ptx::atom_add_acq_rel_gpu(c_done + u, 1);
-          }
-        } else {
-          // The strip's last finished chunk forms its 256 columns of y.
-          __threadfence();
-          ptx::named_barrier(1, 128);
-          if (lead)
-            s.flag = (long long)ptx::atom_add_acq_rel_gpu(c_strip + mt, len) + len == (long long)U * ph.KB;
-          ptx::named_barrier(1, 128);
-          if (!*(volatile int*)&s.flag) continue;
-          __threadfence();
-          const int64_t ld = (int64_t)strips * 256;
-          for (int item = warp - 4; item < p.r.num_tokens * 4; item += 4) {
-            const int t = item >> 2, at = (item & 3) * 64 + lane * 2;  // columns at, at + 1
-            float2 acc = make_float2(0.f, 0.f);
-#pragma unroll 4
-            for (int k = 0; k < p.r.K; ++k) {
-              const int sl = t * p.r.K + k;
-              const int pos = plan.pos[sl];
-              if (pos < 0) continue;
-              const int uu = plan.unit_of[pos], j = pos - plan.unit_pos[uu];
-              float2 v = __ldcg(reinterpret_cast<const float2*>(p.o + pos * ld + mt * 256 + at));
-              const long long q0 = ((long long)mt * U + uu) * ph.KB;
-              const int f = ph.chunk_of(q0), l = ph.chunk_of(q0 + ph.KB - 1);
-              for (int cc = f + 1; cc <= l; ++cc) {
-                const float2 w = __ldcg(reinterpret_cast<const float2*>(
-                    p.extra + ((int64_t)cc * NB + j) * 256 + at));
-                v.x += w.x;
-                v.y += w.y;
-              }
-              acc.x = fmaf(plan.w[sl], v.x, acc.x);
-              acc.y = fmaf(plan.w[sl], v.y, acc.y);
-            }
-            const int col = mt * 256 + at;
-            T* yr = static_cast<T*>(p.y) + (int64_t)t * p.d;
-            if (col < p.d) yr[col] = from_f32<T>(acc.x);
-            if (col + 1 < p.d) yr[col + 1] = from_f32<T>(acc.y);
           }
         }
       }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&s.tmem_empty[buf]));
+      if (MODE == kLinear && whole) continue;
+
+      __threadfence();
+      ptx::named_barrier(1, 128);
+      if (c.phase) {
+        if (lead) ptx::atom_add_acq_rel_gpu(c_strip + c.mt, 1);
+        continue;
+      }
+      if (!whole) {
+        if (lead) s.flag = ptx::atom_add_acq_rel_gpu(c_tile + c.u * MT + c.mt, 1) + 1 == p.parts0;
+        if (MODE == kLinear) continue;  // the final stage adds the parts
+        ptx::named_barrier(1, 128);
+        if (!*(volatile int*)&s.flag) continue;
+        // h of a cut tile: the block that finishes it last adds the parts in order.
+        __threadfence();
+        const float* src = p.part0 + (int64_t)c.row0 * ld0 + c.mt * 256 + row;
+        const int64_t step = (int64_t)p.rows * ld0;
+        for (int j0 = 0; j0 < c.n; j0 += 4) {
+          float a[4] = {}, g[4] = {};
+          for (int q = 0; q < p.parts0; ++q) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float* v = src + q * step + min(j0 + j, c.n - 1) * ld0;
+              a[j] += __ldcg(v);
+              g[j] += __ldcg(v + 128);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j0 + j < c.n) finish(j0 + j, a[j], g[j]);
+        }
+        __threadfence();
+        ptx::named_barrier(1, 128);
+      }
+      if (lead) ptx::atom_add_acq_rel_gpu(c_done + c.u, 1);
+    }
+  }
+
+  // ------------------------------------------------------------ final stage
+  // Every ticket is taken.  64 columns of one output row at a time: 4 threads per column each
+  // add a quarter of the terms, then the quarters are added in order.
+  __syncthreads();
+  if (!*abort_flag && (MODE == kMoe || p.parts0 > 1)) {
+    float* red = reinterpret_cast<float*>(smem);  // the ring is idle
+    int* go = &s.flag;
+    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    const int width = MODE == kMoe ? p.d : p.N;
+    const int groups = (width + 63) / 64;
+    const int out_rows = MODE == kMoe ? p.r.num_tokens : p.rows;
+    const int64_t ld = (int64_t)(MODE == kMoe ? strips : MT) * 256;
+    const int parts = MODE == kMoe ? p.parts1 : p.parts0;
+    const int64_t step = (int64_t)p.rows * ld;
+    for (int i = blockIdx.x; i < groups * out_rows; i += gridDim.x) {
+      const int r = i / groups, g = i - r * groups, col = g * 64 + tx;
+      int unit = 0;
+      if constexpr (MODE == kLinear) {  // the row's unit: the last that starts at or before it
+        int hi = U - 1;
+        while (unit < hi) {
+          const int mid = (unit + hi + 1) >> 1;
+          if (ru.row[mid] <= r) unit = mid; else hi = mid - 1;
+        }
+        if (U == 0 || r < ru.row[unit] || r >= ru.row[unit] + ru.n[unit]) continue;  // in no group
+      }
+      if (threadIdx.x == 0) {
+        const int* count = MODE == kMoe ? c_strip + (g >> 2) : c_tile + unit * MT + (g >> 2);
+        const int want = MODE == kMoe ? U * p.parts1 : p.parts0;
+        const uint64_t t0 = ptx::globaltimer();
+        *go = 1;
+        while (ptx::ld_acquire_gpu(count) < want) {
+          if (ptx::globaltimer() - t0 > kWaitNs) { *go = 0; *abort_flag = 1; break; }
+          __nanosleep(32);
+        }
+      }
+      __syncthreads();
+      if (!*(volatile int*)go) break;
+      float acc = 0.f;
+      if constexpr (MODE == kMoe) {
+        const int terms = p.r.K * parts;
+#pragma unroll 4
+        for (int j = ty; j < terms; j += 4) {
+          const int k = j / parts, sl = r * p.r.K + k, pos = plan.pos[sl];
+          if (pos >= 0)
+            acc = fmaf(plan.w[sl], __ldcg(p.part1 + (int64_t)(j - k * parts) * step + pos * ld + col), acc);
+        }
+      } else {
+#pragma unroll 4
+        for (int j = ty; j < parts; j += 4) acc += __ldcg(p.part0 + j * step + r * ld + col);
+      }
+      red[threadIdx.x] = acc;
+      __syncthreads();
+      if (ty == 0 && col < width) {
+        const float v = ((red[tx] + red[64 + tx]) + red[128 + tx]) + red[192 + tx];
+        if constexpr (MODE == kMoe) {
+          static_cast<T*>(p.y)[(int64_t)r * p.d + col] = from_f32<T>(v);
+        } else {
+          const float b = p.bias ? to_f32(static_cast<const T*>(p.bias)[(int64_t)ru.e[unit] * p.N + col]) : 0.f;
+          linear_out<T>(p, r, col, v + b);
+        }
+      }
+      __syncthreads();
     }
   }
 

@@ -105,9 +105,10 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 // One warp: the K largest of row[0..E) (ties to the lower index) and the softmax over them.
 // An expert whose logit is -inf is masked: its slot gets index -1 and weight 0, so a token
 // with no unmasked expert has an all-zero output row.
+// VPT = logits held per lane (E <= 32 * VPT).
+template <int VPT>
 __device__ __forceinline__ void topk_token(const float* __restrict__ row, int E, int K, int lane,
                                            int16_t* __restrict__ idx, float* __restrict__ w) {
-  constexpr int VPT = kMaxExperts / 32;
   uint32_t key[VPT];
   uint32_t best = 0;
   int best_e = 0x7fffffff;
@@ -208,8 +209,12 @@ __device__ __forceinline__ void build_plan(const Plan& p, const Routing& r, int 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   for (int e = threadIdx.x; e < r.E; e += blockDim.x) p.cnt[e] = 0;
   if (r.logits) {
-    for (int t = warp; t < r.num_tokens; t += warps)
-      topk_token(r.logits + (int64_t)t * r.E, r.E, r.K, lane, p.pos + t * r.K, p.w + t * r.K);
+    for (int t = warp; t < r.num_tokens; t += warps) {
+      const float* row = r.logits + (int64_t)t * r.E;
+      if (r.E <= 64) topk_token<2>(row, r.E, r.K, lane, p.pos + t * r.K, p.w + t * r.K);
+      else if (r.E <= 256) topk_token<8>(row, r.E, r.K, lane, p.pos + t * r.K, p.w + t * r.K);
+      else topk_token<kMaxExperts / 32>(row, r.E, r.K, lane, p.pos + t * r.K, p.w + t * r.K);
+    }
   } else {
     for (int s = threadIdx.x; s < S; s += blockDim.x) {
       const int e = r.indices[s];

@@ -95,23 +95,25 @@ static int linear_tiles(const LinearArgs& a) {
                  : launch_sm100<ML, 1, 0, false, false, __half>(ma, mb, mc, p, a.stream, extra);
 }
 
-// The few-row kernel: its counters and partials for `grid` chunks.
+// The few-row kernel's split, counters and partials.
 struct FewLinear {
-  int nb, units, grid;
+  int nb, max_units, parts, num_counters, grid;
   size_t part, total;
 };
 static FewLinear few_linear_plan(int64_t m, int64_t n, int64_t k, int E, bool dense) {
   FewLinear f = {};
   f.nb = few_nb(m);
-  f.units = fewtc::row_units_max(m, E, f.nb);
+  f.max_units = fewtc::row_units_max(m, E, f.nb);
+  const int64_t MT = (n + 255) / 256;
+  // groups that are likely to have a row, when the rows pick groups at random
+  const double live = E <= 1 ? 1.0 : E * (1.0 - pow(1.0 - 1.0 / E, (double)m));
+  const double units = dense ? (double)((m + f.nb - 1) / f.nb) : std::max(live, (double)m / f.nb);
+  f.parts = few_parts(units * MT, (k + fewtc::BK - 1) / fewtc::BK, f.nb);
+  f.num_counters = 1 + (f.parts > 1 ? f.max_units * (int)MT : 0);
+  f.part = align256((size_t)f.num_counters * 4);
+  f.total = f.part + (f.parts > 1 ? (size_t)f.parts * m * MT * 1024 : 0);
   f.grid = num_sms(current_device());
-  if (dense) {
-    // all units and blocks are known here: no more blocks than chunks
-    const int64_t blocks = (m + f.nb - 1) / f.nb * ((n + 255) / 256) * ((k + fewtc::BK - 1) / fewtc::BK);
-    f.grid = (int)std::max<int64_t>(1, std::min<int64_t>(f.grid, blocks / kFewMinBlocks));
-  }
-  f.part = align256((size_t)(1 + f.grid + f.units) * 4);
-  f.total = f.part + align256((size_t)2 * f.grid * f.nb * 256 * 4);
+  if (dense) f.grid = (int)std::min<int64_t>(f.grid, (int64_t)units * MT * f.parts);
   return f;
 }
 
@@ -139,15 +141,13 @@ static int few_linear(const LinearArgs& a, void* workspace) {
   p.x = a.A;
   p.y = a.out;
   p.counters = (int*)ws;
-  p.part = (float*)(ws + f.part);
-  p.max_chunks = f.grid;
-  p.max_units = f.units;
-  p.min_blocks = kFewMinBlocks;
-  const int counters = 1 + f.grid + f.units;
-  fewtc::zero_counters_kernel<<<1, 256, 0, a.stream>>>(p.counters, counters);
-  MOE_LAUNCH_CHECK();
+  p.part0 = (float*)(ws + f.part);
+  p.rows = (int)a.m;
+  p.parts0 = f.parts;
+  p.max_units = f.max_units;
+  if ((rc = zero_counters(p.counters, f.num_counters, a.stream))) return rc;
   const CUtensorMap maps[3] = {map, map, map};
-  const int table = fewtc::row_units_bytes(f.units);
+  const int table = fewtc::row_units_bytes(f.max_units);
   if (a.dtype == MOE_BF16)
     return few_kernel_nb<fewtc::kLinear, 1, __nv_bfloat16>(f.nb, maps, p, (unsigned)f.grid, table, a.stream);
   return few_kernel_nb<fewtc::kLinear, 0, __half>(f.nb, maps, p, (unsigned)f.grid, table, a.stream);
@@ -184,7 +184,9 @@ size_t moe_linear_workspace_bytes(int64_t m_total, int64_t n, int64_t k, int32_t
   if (m_total <= 0 || n <= 0 || k <= 0 || num_experts <= 0 || !trans_b || dtype == MOE_F32 ||
       m_total > few_linear_max_rows(num_experts))
     return 0;
-  return few_linear_plan(m_total, n, k, num_experts, false).total;
+  // whether the product is dense only changes the split: the larger of the two
+  return std::max(few_linear_plan(m_total, n, k, num_experts, false).total,
+                  few_linear_plan(m_total, n, k, num_experts, true).total);
 }
 
 int moe_linear_fwd(const void* A, const void* B, const void* bias, const void* residual, void* out,

@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <math.h>
 #include <mutex>
 #include <stdarg.h>
 #include <stdio.h>

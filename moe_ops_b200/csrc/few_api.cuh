@@ -70,7 +70,7 @@ static FewWorkspace few_workspace(int64_t T, int64_t d, int64_t H, int64_t E, in
   if (w.parts0 > 1 && (size_t)w.parts0 * S * MT * 1024 > (64u << 20)) w.parts0 = 1;
   w.parts1 = few_parts(touched * strips, KB1, nb);
   w.max_units = few::plan_max_units((int)S, (int)E, nb);
-  w.num_counters = 1 + (w.parts0 > 1 ? w.max_units * (int)MT : 0) + w.max_units + (int)strips;
+  w.num_counters = 2 + w.max_units + (w.parts0 > 1 ? w.max_units * (int)MT : 0);
   w.part0 = w.counters + align256((size_t)w.num_counters * 4);
   w.part1 = w.part0 + (w.parts0 > 1 ? align256((size_t)w.parts0 * S * MT * 1024) : 0);
   w.total = w.part1 + align256((size_t)w.parts1 * S * strips * 1024);
@@ -158,7 +158,7 @@ static int few_kernel_launch(const CUtensorMap* maps, fewtc::Params p, unsigned 
                              cudaStream_t stream) {
   auto kern = fewtc::few_kernel<MODE, FMT, T, NB>;
   const size_t stage = fewtc::kWBytes + NB * 128;
-  const size_t fixed = 1024 + (sizeof(fewtc::Ctl) + 15) / 16 * 16 + (size_t)table_bytes;
+  const size_t fixed = 1024 + fewtc::kCtlBytes + fewtc::kStagedBytes + (size_t)table_bytes;
   p.stages = (int)std::min<size_t>(fewtc::kMaxStages, (kMaxSmem - fixed) / stage);
   MOE_REQUIRE(fixed < kMaxSmem && p.stages > fewtc::kLag, "few rows: routing tables too large");
   const int dev = current_device();

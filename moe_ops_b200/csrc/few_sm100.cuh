@@ -38,6 +38,12 @@
 //               token, any h row), handed over kLag stages later.
 //   warps 4-7   epilogue, one accumulator lane (weight row) per thread.
 //
+// While the weights saturate HBM a fence or an atomic takes microseconds (measured: 6 us and 5 us
+// for the first ones of a block), as long as a chunk's loads.  So they stay off the chunk's path:
+// there are several accumulator pairs, a finished h tile is published only when the next
+// chunk's accumulator is ready (its stores have long landed, the fence is short) or when there is
+// nothing else to do, and finished output chunks are counted once per block.
+//
 // Every wait is bounded; one that gives up sets the abort flag and device error 1.
 #pragma once
 
@@ -80,18 +86,21 @@ struct Params {
   float* part0;      // [parts0, rows, MT * 256] partials of phase 0 (parts0 > 1); rows: S or m
   float* part1;      // [parts1, S, strips * 256] results of phase 1
   int rows;          // S (kMoe) or m
-  int* counters;     // zeroed before the launch: ticket; tile[max_units * MT] finished chunks of
-                     // a tile (parts0 > 1); kMoe: done[max_units] finished h tiles, strip[strips]
-                     // finished chunks of a 256-column strip of y
+  int* counters;     // zeroed before the launch: ticket; finished chunks of the outputs; kMoe:
+                     // done[max_units] finished h tiles of a unit, tile[max_units * MT] finished
+                     // chunks of an h tile (parts0 > 1)
   int max_units;
   int stages;
 };
 
 constexpr int kTickets = 4;  // ticket ring
 
+// Accumulator pairs of a unit size: 256 TMEM columns, 512 for NB = 64.
+__host__ __device__ constexpr int acc_bufs(int nb) { return nb == 16 ? 8 : 4; }
+
 struct Ctl {
   uint64_t full[kMaxStages], empty[kMaxStages];
-  uint64_t tmem_full[2], tmem_empty[2];
+  uint64_t tmem_full[8], tmem_empty[8];
   uint64_t tk_full[kTickets], tk_empty[kTickets];
   int tk[kTickets];
   uint32_t tmem_base;
@@ -99,6 +108,9 @@ struct Ctl {
   int flag;
   int num_units;
 };
+
+constexpr int kCtlBytes = (int)((sizeof(Ctl) + 15) / 16 * 16);
+constexpr int kStagedBytes = 8 * 256 * 4;  // accumulators of 8 rows on their way out
 
 // Units of kLinear: at most NB consecutive rows of one group.
 struct RowUnits {
@@ -118,10 +130,11 @@ __device__ __forceinline__ void part_range(int KB, int parts, int part, int& fir
   len = min(L, KB - first);
 }
 
-// kLinear's epilogue on one element: z = the sum and the bias.
+// kLinear's epilogue on one element: z = the products' sum, of group e.
 template <typename T>
-__device__ __forceinline__ void linear_out(const Params& p, int64_t row, int col, float z) {
+__device__ __forceinline__ void linear_out(const Params& p, int e, int64_t row, int col, float z) {
   if (col >= p.N) return;
+  if (p.bias) z += to_f32(static_cast<const T*>(p.bias)[(int64_t)e * p.N + col]);
   const int64_t at = row * p.N + col;
   if (p.preact) static_cast<T*>(p.preact)[at] = from_f32<T>(z);
   float y = act_fwd_rt(p.act, z);
@@ -136,10 +149,12 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   constexpr uint32_t kStage = kWBytes + NB * 128;
-  constexpr uint32_t kTmemCols = 4 * NB;  // two accumulator pairs
+  constexpr int kBufs = acc_bufs(NB);
+  constexpr uint32_t kTmemCols = kBufs * 2 * NB;
   const int ST = p.stages;
   Ctl& s = *reinterpret_cast<Ctl*>(smem + ST * kStage);
-  uint8_t* plan_mem = smem + ST * kStage + (sizeof(Ctl) + 15) / 16 * 16;
+  float* const staged = reinterpret_cast<float*>(smem + ST * kStage + kCtlBytes);  // [8][256]
+  uint8_t* plan_mem = smem + ST * kStage + kCtlBytes + kStagedBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &s.abort;
 
@@ -148,7 +163,7 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
       ptx::mbar_init(ptx::smem_u32(&s.full[i]), 3);
       ptx::mbar_init(ptx::smem_u32(&s.empty[i]), 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kBufs; ++i) {
       ptx::mbar_init(ptx::smem_u32(&s.tmem_full[i]), 1);
       ptx::mbar_init(ptx::smem_u32(&s.tmem_empty[i]), 4);
     }
@@ -227,9 +242,9 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
   const int strips = MODE == kMoe ? (p.d + 255) / 256 : 0;
   const int KB0 = ((MODE == kMoe ? p.d : p.K) + BK - 1) / BK, KB1 = (p.H + BK - 1) / BK;
   const int G0 = U * MT * p.parts0, G1 = MODE == kMoe ? U * strips * p.parts1 : 0;
-  int* const c_tile = p.counters + 1;
-  int* const c_done = c_tile + (p.parts0 > 1 ? p.max_units * MT : 0);
-  int* const c_strip = c_done + p.max_units;
+  int* const c_out = p.counters + 1;
+  int* const c_done = p.counters + 2;
+  int* const c_tile = c_done + p.max_units;
 
   // Chunk t: unit u (expert e, first row row0, n rows), tile mt, blocks [kb0, kb0 + len).
   struct Chunk {
@@ -311,8 +326,8 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
     Chunk c;
     for (int it = 0; ok && ticket(it, c); ++it) {
       const uint32_t idesc = ptx::make_idesc_f16(FMT, 0, 0, 128, (c.n + 15) / 16 * 16);
-      const int buf = it & 1;
-      if (!warp_wait(s.tmem_empty[buf], ((it >> 1) & 1) ^ 1)) break;
+      const int buf = it % kBufs;
+      if (!warp_wait(s.tmem_empty[buf], ((it / kBufs) & 1) ^ 1)) break;
       ptx::tc_fence_after();
       const uint32_t d0 = tmem_base + buf * 2 * NB;
       for (int i = 0; i < c.len; ++i) {
@@ -413,91 +428,105 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
     const int row = (warp - 4) * 32 + lane;  // accumulator lane
     const bool lead = row == 0;
     const int64_t ld0 = (int64_t)MT * 256, ld1 = (int64_t)strips * 256;
-    Chunk c;
+    Chunk c, held = {};
+    bool pending = false;  // `held` is a phase-0 chunk of kMoe that is stored but not published
+    int outputs = 0;       // chunks of the outputs that this block has stored
+    // h of column `row` of a tile: D0 is its gate, D1 its up.
+    auto store_h = [&](const Chunk& k, int j, float gate, float up) {
+      const int col = k.mt * 128 + row;
+      if (col < p.H)
+        static_cast<T*>(p.h)[(int64_t)(k.row0 + j) * p.H + col] = from_f32<T>(gate * sigmoid_f32(gate) * up);
+    };
+    // Counts `held`; of a cut tile, the block that finishes it last adds the parts in order.
+    auto publish = [&]() {
+      pending = false;
+      ptx::fence_acq_rel_gpu();
+      ptx::named_barrier(1, 128);
+      if (p.parts0 > 1) {
+        if (lead) s.flag = ptx::atom_add_gpu(c_tile + held.u * MT + held.mt, 1) + 1 == p.parts0;
+        ptx::named_barrier(1, 128);
+        if (!*(volatile int*)&s.flag) return;
+        ptx::fence_acq_rel_gpu();
+        const float* src = p.part0 + (int64_t)held.row0 * ld0 + held.mt * 256 + row;
+        const int64_t step = (int64_t)p.rows * ld0;
+#pragma unroll 1
+        for (int j = 0; j < held.n; ++j) {
+          float a = 0.f, g = 0.f;
+#pragma unroll 8
+          for (int q = 0; q < p.parts0; ++q) {
+            a += __ldcg(src + q * step + j * ld0);
+            g += __ldcg(src + q * step + j * ld0 + 128);
+          }
+          store_h(held, j, a, g);
+        }
+        ptx::fence_acq_rel_gpu();
+        ptx::named_barrier(1, 128);
+      }
+      if (lead) ptx::atom_add_gpu(c_done + held.u, 1);
+    };
     // The four warps meet at barriers, so each wait's outcome is agreed on by all of them.
     for (int it = 0;; ++it) {
+      const int buf = it % kBufs;
+      const uint32_t parity = (it / kBufs) & 1;
+      if (pending) {
+        const bool ready = ptx::mbar_try_wait(ptx::smem_u32(&s.tk_full[it % kTickets]), (it / kTickets) & 1) &&
+                           ptx::mbar_try_wait(ptx::smem_u32(&s.tmem_full[buf]), parity);
+        if (!ptx::named_barrier_all(1, 128, ready)) publish();
+      }
       const bool more = ticket(it, c);
       if (!ptx::named_barrier_all(1, 128, more)) break;
-      const int buf = it & 1;
-      if (!ptx::named_barrier_all(1, 128, warp_wait(s.tmem_full[buf], (it >> 1) & 1))) break;
+      if (!ptx::named_barrier_all(1, 128, warp_wait(s.tmem_full[buf], parity))) break;
+      if (pending) publish();
       ptx::tc_fence_after();
       const uint32_t tb = tmem_base + ((uint32_t)((warp - 4) * 32) << 16) + buf * 2 * NB;
       const bool whole = !c.phase && p.parts0 == 1;
-      const int col0 = MODE == kMoe ? c.mt * 128 + row : c.mt * 256 + row, col1 = col0 + 128;
-      float bias0 = 0.f, bias1 = 0.f;
-      if (MODE == kLinear && p.bias && whole) {
-        const T* bp = static_cast<const T*>(p.bias) + (int64_t)c.e * p.N;
-        if (col0 < p.N) bias0 = to_f32(bp[col0]);
-        if (col1 < p.N) bias1 = to_f32(bp[col1]);
-      }
-      // The tile's epilogue on row j of the unit (v0, v1: this thread's D0 and D1).
-      auto finish = [&](int j, float v0, float v1) {
-        if constexpr (MODE == kMoe) {
-          if (col0 < p.H)
-            static_cast<T*>(p.h)[(int64_t)(c.row0 + j) * p.H + col0] = from_f32<T>(v0 * sigmoid_f32(v0) * v1);
-        } else {
-          linear_out<T>(p, c.row0 + j, col0, v0 + bias0);
-          linear_out<T>(p, c.row0 + j, col1, v1 + bias1);
-        }
-      };
       // Partial sums: this thread's two columns of the tile, row by row.
       const int64_t ld = c.phase ? ld1 : ld0;
       float* dst = (c.phase ? p.part1 : p.part0) + ((int64_t)c.part * p.rows + c.row0) * ld + c.mt * 256 + row;
-      for (int j0 = 0; j0 < c.n; j0 += 16) {
-        uint32_t v0[16], v1[16];
-        ptx::tmem_ld_32x32b_x16(tb + j0, v0);
-        ptx::tmem_ld_32x32b_x16(tb + NB + j0, v1);
+#pragma unroll 1
+      for (int j0 = 0; j0 < c.n; j0 += 8) {
+        uint32_t v0[8], v1[8];
+        ptx::tmem_ld_32x32b_x8(tb + j0, v0);
+        ptx::tmem_ld_32x32b_x8(tb + NB + j0, v1);
         ptx::tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          if (j0 + j < c.n) {
-            const float a = __uint_as_float(v0[j]), g = __uint_as_float(v1[j]);
-            if (whole) finish(j0 + j, a, g);
-            else {
-              dst[(j0 + j) * ld] = a;
-              dst[(j0 + j) * ld + 128] = g;
-            }
+        for (int j = 0; j < 8; ++j) {
+          staged[j * 256 + row] = __uint_as_float(v0[j]);
+          staged[j * 256 + 128 + row] = __uint_as_float(v1[j]);
+        }
+        // each thread reads back what it wrote
+        const int m = min(8, c.n - j0);
+#pragma unroll 1
+        for (int j = 0; j < m; ++j) {
+          const float a = staged[j * 256 + row], g = staged[j * 256 + 128 + row];
+          if (!whole) {
+            dst[(j0 + j) * ld] = a;
+            dst[(j0 + j) * ld + 128] = g;
+          } else if constexpr (MODE == kMoe) {
+            store_h(c, j0 + j, a, g);
+          } else {
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i)
+              linear_out<T>(p, c.e, c.row0 + j0 + j, c.mt * 256 + i * 128 + row, i ? g : a);
           }
         }
       }
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&s.tmem_empty[buf]));
-      if (MODE == kLinear && whole) continue;
-
-      __threadfence();
+      if (MODE == kMoe && !c.phase) {
+        held = c;
+        pending = true;
+      } else {
+        ++outputs;
+      }
+    }
+    // Abandoned work is not published (the wait that gave up has set the abort flag).
+    if (pending && !ptx::named_barrier_all(1, 128, *abort_flag != 0)) publish();
+    if (MODE == kMoe || p.parts0 > 1) {
+      ptx::fence_acq_rel_gpu();
       ptx::named_barrier(1, 128);
-      if (c.phase) {
-        if (lead) ptx::atom_add_acq_rel_gpu(c_strip + c.mt, 1);
-        continue;
-      }
-      if (!whole) {
-        if (lead) s.flag = ptx::atom_add_acq_rel_gpu(c_tile + c.u * MT + c.mt, 1) + 1 == p.parts0;
-        if (MODE == kLinear) continue;  // the final stage adds the parts
-        ptx::named_barrier(1, 128);
-        if (!*(volatile int*)&s.flag) continue;
-        // h of a cut tile: the block that finishes it last adds the parts in order.
-        __threadfence();
-        const float* src = p.part0 + (int64_t)c.row0 * ld0 + c.mt * 256 + row;
-        const int64_t step = (int64_t)p.rows * ld0;
-        for (int j0 = 0; j0 < c.n; j0 += 4) {
-          float a[4] = {}, g[4] = {};
-          for (int q = 0; q < p.parts0; ++q) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float* v = src + q * step + min(j0 + j, c.n - 1) * ld0;
-              a[j] += __ldcg(v);
-              g[j] += __ldcg(v + 128);
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (j0 + j < c.n) finish(j0 + j, a[j], g[j]);
-        }
-        __threadfence();
-        ptx::named_barrier(1, 128);
-      }
-      if (lead) ptx::atom_add_acq_rel_gpu(c_done + c.u, 1);
+      if (lead && outputs > 0) ptx::atom_add_gpu(c_out, outputs);
     }
   }
 
@@ -507,7 +536,16 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
   __syncthreads();
   if (!*abort_flag && (MODE == kMoe || p.parts0 > 1)) {
     float* red = reinterpret_cast<float*>(smem);  // the ring is idle
-    int* go = &s.flag;
+    if (threadIdx.x == 0) {
+      const int want = MODE == kMoe ? G1 : G0;
+      const uint64_t t0 = ptx::globaltimer();
+      s.flag = 1;
+      while (ptx::ld_acquire_gpu(c_out) < want) {
+        if (ptx::globaltimer() - t0 > kWaitNs) { s.flag = 0; *abort_flag = 1; break; }
+        __nanosleep(32);
+      }
+    }
+    __syncthreads();
     const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
     const int width = MODE == kMoe ? p.d : p.N;
     const int groups = (width + 63) / 64;
@@ -515,7 +553,8 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
     const int64_t ld = (int64_t)(MODE == kMoe ? strips : MT) * 256;
     const int parts = MODE == kMoe ? p.parts1 : p.parts0;
     const int64_t step = (int64_t)p.rows * ld;
-    for (int i = blockIdx.x; i < groups * out_rows; i += gridDim.x) {
+    const int items = *(volatile int*)&s.flag ? groups * out_rows : 0;
+    for (int i = blockIdx.x; i < items; i += gridDim.x) {
       const int r = i / groups, g = i - r * groups, col = g * 64 + tx;
       int unit = 0;
       if constexpr (MODE == kLinear) {  // the row's unit: the last that starts at or before it
@@ -526,18 +565,6 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
         }
         if (U == 0 || r < ru.row[unit] || r >= ru.row[unit] + ru.n[unit]) continue;  // in no group
       }
-      if (threadIdx.x == 0) {
-        const int* count = MODE == kMoe ? c_strip + (g >> 2) : c_tile + unit * MT + (g >> 2);
-        const int want = MODE == kMoe ? U * p.parts1 : p.parts0;
-        const uint64_t t0 = ptx::globaltimer();
-        *go = 1;
-        while (ptx::ld_acquire_gpu(count) < want) {
-          if (ptx::globaltimer() - t0 > kWaitNs) { *go = 0; *abort_flag = 1; break; }
-          __nanosleep(32);
-        }
-      }
-      __syncthreads();
-      if (!*(volatile int*)go) break;
       float acc = 0.f;
       if constexpr (MODE == kMoe) {
         const int terms = p.r.K * parts;
@@ -558,8 +585,7 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
         if constexpr (MODE == kMoe) {
           static_cast<T*>(p.y)[(int64_t)r * p.d + col] = from_f32<T>(v);
         } else {
-          const float b = p.bias ? to_f32(static_cast<const T*>(p.bias)[(int64_t)ru.e[unit] * p.N + col]) : 0.f;
-          linear_out<T>(p, r, col, v + b);
+          linear_out<T>(p, ru.e[unit], r, col, v);
         }
       }
       __syncthreads();

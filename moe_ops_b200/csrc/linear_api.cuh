@@ -109,7 +109,7 @@ static FewLinear few_linear_plan(int64_t m, int64_t n, int64_t k, int E, bool de
   const double live = E <= 1 ? 1.0 : E * (1.0 - pow(1.0 - 1.0 / E, (double)m));
   const double units = dense ? (double)((m + f.nb - 1) / f.nb) : std::max(live, (double)m / f.nb);
   f.parts = few_parts(units * MT, (k + fewtc::BK - 1) / fewtc::BK, f.nb);
-  f.num_counters = 1 + (f.parts > 1 ? f.max_units * (int)MT : 0);
+  f.num_counters = 2;
   f.part = align256((size_t)f.num_counters * 4);
   f.total = f.part + (f.parts > 1 ? (size_t)f.parts * m * MT * 1024 : 0);
   f.grid = num_sms(current_device());

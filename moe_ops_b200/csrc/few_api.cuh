@@ -25,6 +25,8 @@ struct FewArgs {
   cudaStream_t stream;
 };
 
+constexpr size_t kMaxSmem = 232448;  // dynamic shared memory a block may have on sm_100
+
 static size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
 // Rows of a unit of the tensor-core kernel, by the most rows that one expert (one group) can
@@ -32,48 +34,59 @@ static size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 // crowded expert's weights once.
 static int few_nb(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
-// Chunks a tile's contraction of KB 64-deep blocks is cut into when there are about `tiles`
-// tiles: about 6 chunks per SM, so that SMs of different speed end together, but no chunk under 4
-// blocks (128 KB) nor so small that its partial sums (n rows of 1 KB) weigh against its weights
-// (32 KB a block).
-static int few_parts(double tiles, int64_t KB, int nb) {
-  const double want = 6.0 * num_sms(current_device());
-  int64_t len = (int64_t)(tiles * KB / want);
-  len = std::max<int64_t>(len, std::max(4, nb / 4));
-  len = std::min(len, KB);
-  const int64_t parts = (KB + len - 1) / len;
-  len = (KB + parts - 1) / parts;  // equal chunks, none empty
-  return (int)((KB + len - 1) / len);
+// Tiles of a phase: `rows` weight rows per unit (per box: gate_up tiles hold two boxes of the same
+// rows), about `units` units.  As few waves of tiles over the SMs as a tile's height allows, and
+// tiles as high as then fill the waves; never lower than the activations' rows would make
+// worthwhile (a tile re-reads them all).
+static fewtc::Params::Shape few_shape(double units, int64_t rows, bool gate_up, int nb) {
+  fewtc::Params::Shape s = {};
+  const int64_t most = gate_up ? 128 : 256;
+  const double sms = num_sms(current_device());
+  const double waves = ceil(units * (double)rows / ((double)most * sms));
+  int64_t tiles = std::max<int64_t>(1, (int64_t)(sms * waves / units));
+  int64_t height = std::max((rows + tiles - 1) / tiles, std::min<int64_t>(rows, std::max(16, nb / 2)));
+  height = std::min(height, most);
+  s.boxes = !gate_up && height > 128 ? 2 : 1;
+  s.box_rows = (int)((height + s.boxes - 1) / s.boxes);
+  s.tiles = (int)((rows + s.boxes * s.box_rows - 1) / (s.boxes * s.box_rows));
+  return s;
+}
+
+// Ring geometry: as many 64-deep blocks per stage as about 40 KB hold, then as many stages as
+// shared memory holds.
+static int few_ring(fewtc::Params& p, int phases, int nb, int table_bytes) {
+  int bytes = 0;
+  for (int i = 0; i < phases; ++i) {
+    auto& s = p.shape[i];
+    const int boxes = phases == 2 && i == 0 ? 2 : s.boxes;
+    const int block = boxes * ((s.box_rows + 7) / 8 * 1024) + nb * 128;
+    s.blocks = std::max(1, std::min(fewtc::kMaxBlocksPerStage, 40960 / block));
+    bytes = std::max(bytes, s.blocks * block);
+  }
+  p.stage_bytes = bytes;
+  const size_t fixed = 1024 + fewtc::kCtlBytes + fewtc::kStagedBytes + (size_t)table_bytes;
+  MOE_REQUIRE(fixed < kMaxSmem, "few rows: routing tables too large");
+  p.stages = (int)std::min<size_t>(fewtc::kMaxStages, (kMaxSmem - fixed) / bytes);
+  MOE_REQUIRE(p.stages >= 2, "few rows: routing tables too large");
+  return MOE_OK;
 }
 
 // Workspace: logits [T, E] fp32, h [T*K, H] (fp32 for the CUDA cores, else 16 bits), then for
-// the tensor-core kernel its counters and fp32 partial results.
+// the tensor-core kernel its counters and fp32 results.
 struct FewWorkspace {
-  size_t logits, h, counters, part0, part1, total;
-  int num_counters, max_units, parts0, parts1;
+  size_t logits, h, counters, part, total;
+  int num_counters, max_units;
 };
 static FewWorkspace few_workspace(int64_t T, int64_t d, int64_t H, int64_t E, int64_t K, int dtype) {
   FewWorkspace w = {};
-  const size_t S = (size_t)(T * K), strips = (size_t)((d + 255) / 256), MT = (size_t)((H + 127) / 128);
+  const size_t S = (size_t)(T * K);
   w.logits = 0;
   w.h = align256((size_t)T * E * 4);
   w.counters = w.h + align256(S * H * 4);
-  if (dtype == MOE_F32 || d == 0 || H == 0) {
-    w.total = w.counters;
-    return w;
-  }
-  const int nb = few_nb(T);
-  // experts that T tokens are expected to touch when each picks K of E
-  const double touched = K >= E ? (double)E : E * (1.0 - pow(1.0 - (double)K / E, (double)T));
-  const int64_t KB0 = (d + fewtc::BK - 1) / fewtc::BK, KB1 = (H + fewtc::BK - 1) / fewtc::BK;
-  w.parts0 = few_parts(touched * MT, KB0, nb);
-  if (w.parts0 > 1 && (size_t)w.parts0 * S * MT * 1024 > (64u << 20)) w.parts0 = 1;
-  w.parts1 = few_parts(touched * strips, KB1, nb);
-  w.max_units = few::plan_max_units((int)S, (int)E, nb);
-  w.num_counters = 2 + w.max_units + (w.parts0 > 1 ? w.max_units * (int)MT : 0);
-  w.part0 = w.counters + align256((size_t)w.num_counters * 4);
-  w.part1 = w.part0 + (w.parts0 > 1 ? align256((size_t)w.parts0 * S * MT * 1024) : 0);
-  w.total = w.part1 + align256((size_t)w.parts1 * S * strips * 1024);
+  w.max_units = few::plan_max_units((int)S, (int)E, few_nb(T));
+  w.num_counters = 2 + w.max_units;
+  w.part = w.counters + (dtype == MOE_F32 ? 0 : align256((size_t)w.num_counters * 4));
+  w.total = w.part + (dtype == MOE_F32 ? 0 : align256(S * d * 4));
   return w;
 }
 
@@ -151,16 +164,10 @@ static bool few_tc_ok(const FewArgs& a) {
          aligned16(a.w_gate) && aligned16(a.w_up) && aligned16(a.w_down);
 }
 
-constexpr size_t kMaxSmem = 232448;  // dynamic shared memory a block may have on sm_100
-
 template <int MODE, int FMT, typename T, int NB>
-static int few_kernel_launch(const CUtensorMap* maps, fewtc::Params p, unsigned grid, int table_bytes,
+static int few_kernel_launch(const CUtensorMap* maps, const fewtc::Params& p, unsigned grid, int table_bytes,
                              cudaStream_t stream) {
   auto kern = fewtc::few_kernel<MODE, FMT, T, NB>;
-  const size_t stage = fewtc::kWBytes + NB * 128;
-  const size_t fixed = 1024 + fewtc::kCtlBytes + fewtc::kStagedBytes + (size_t)table_bytes;
-  p.stages = (int)std::min<size_t>(fewtc::kMaxStages, (kMaxSmem - fixed) / stage);
-  MOE_REQUIRE(fixed < kMaxSmem && p.stages > fewtc::kLag, "few rows: routing tables too large");
   const int dev = current_device();
   static unsigned long long attr_set = 0;  // per-device bitmask, one per instantiation
   {
@@ -170,8 +177,9 @@ static int few_kernel_launch(const CUtensorMap* maps, fewtc::Params p, unsigned 
       if (dev < 64) attr_set |= 1ull << dev;
     }
   }
-  MOE_CUDA_CHECK(launch_pdl(kern, dim3(grid), dim3(fewtc::kThreads), fixed + p.stages * stage, stream,
-                            maps[0], maps[1], maps[2], p));
+  const size_t smem = 1024 + (size_t)p.stages * p.stage_bytes + fewtc::kCtlBytes + fewtc::kStagedBytes + table_bytes;
+  MOE_CUDA_CHECK(launch_pdl(kern, dim3(grid), dim3(fewtc::kThreads), smem, stream, maps[0], maps[1],
+                            maps[2], p));
   return MOE_OK;
 }
 
@@ -189,19 +197,17 @@ static int zero_counters(int* counters, int n, cudaStream_t s) {
   return MOE_OK;
 }
 
-static int few_weight_map(CUtensorMap* map, const void* w, int dtype, int64_t inner, int64_t rows, int64_t E) {
+static int few_weight_map(CUtensorMap* map, const void* w, int dtype, int64_t inner, int64_t rows, int64_t E,
+                          int box_rows) {
   const uint64_t dims[3] = {(uint64_t)inner, (uint64_t)rows, (uint64_t)E};
-  const uint32_t box[3] = {(uint32_t)fewtc::BK, 128, 1};
+  const uint32_t box[3] = {(uint32_t)fewtc::BK, (uint32_t)box_rows, 1};
   return make_map(map, w, dtype, 3, dims, box);
 }
 
 static int few_tc_launch(const FewArgs& a, const few::Routing& r, const FewWorkspace& w) {
-  CUtensorMap maps[3];
-  int rc;
-  if ((rc = few_weight_map(&maps[0], a.w_gate, a.dtype, a.d, a.hidden, a.E))) return rc;
-  if ((rc = few_weight_map(&maps[1], a.w_up, a.dtype, a.d, a.hidden, a.E))) return rc;
-  if ((rc = few_weight_map(&maps[2], a.w_down, a.dtype, a.hidden, a.d, a.E))) return rc;
   uint8_t* ws = (uint8_t*)a.workspace;
+  const int nb = few_nb(a.num_tokens);
+  const int table = few::plan_bytes(r.num_tokens * r.K, r.E, nb);
   fewtc::Params p = {};
   p.r = r;
   p.d = (int)a.d;
@@ -209,15 +215,21 @@ static int few_tc_launch(const FewArgs& a, const few::Routing& r, const FewWorks
   p.x = a.x;
   p.y = a.out;
   p.h = ws + w.h;
-  p.rows = r.num_tokens * r.K;
-  p.parts0 = w.parts0;
-  p.parts1 = w.parts1;
-  p.part0 = (float*)(ws + w.part0);
-  p.part1 = (float*)(ws + w.part1);
+  p.parts = 1;
+  p.part = (float*)(ws + w.part);
   p.counters = (int*)(ws + w.counters);
   p.max_units = w.max_units;
-  const int nb = few_nb(a.num_tokens);
-  const int table = few::plan_bytes(r.num_tokens * r.K, r.E, nb);
+  // experts that the tokens are expected to touch when each picks K of E
+  const double touched =
+      a.topk >= a.E ? (double)a.E : a.E * (1.0 - pow(1.0 - (double)a.topk / a.E, (double)a.num_tokens));
+  p.shape[0] = few_shape(touched, a.hidden, true, nb);
+  p.shape[1] = few_shape(touched, a.d, false, nb);
+  int rc;
+  if ((rc = few_ring(p, 2, nb, table))) return rc;
+  CUtensorMap maps[3];
+  if ((rc = few_weight_map(&maps[0], a.w_gate, a.dtype, a.d, a.hidden, a.E, p.shape[0].box_rows))) return rc;
+  if ((rc = few_weight_map(&maps[1], a.w_up, a.dtype, a.d, a.hidden, a.E, p.shape[0].box_rows))) return rc;
+  if ((rc = few_weight_map(&maps[2], a.w_down, a.dtype, a.hidden, a.d, a.E, p.shape[1].box_rows))) return rc;
   const unsigned grid = (unsigned)num_sms(current_device());
   if (a.dtype == MOE_BF16)
     return few_kernel_nb<fewtc::kMoe, 1, __nv_bfloat16>(nb, maps, p, grid, table, a.stream);

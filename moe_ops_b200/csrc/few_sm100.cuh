@@ -7,42 +7,42 @@
 // operand (N = n rounded up to 16): one 64-deep block of 256 weight rows is a 32 KB stage, its
 // 8 MMAs take a fraction of the stage's HBM time, and no register touches a weight.
 //
-//   kMoe     phase 0: a tile is 128 columns of h: 128 gate rows (accumulator D0) and the same
-//            128 up rows (D1) of one unit (an expert's rows, at most NB); its epilogue forms
+//   kMoe     phase 0: a tile is up to 128 columns of h: those gate rows (accumulator D0) and the
+//            same up rows (D1) of one unit (an expert's rows, at most NB); its epilogue forms
 //            h = silu(gate) * up in fp32 and rounds it once to 16 bits (as an MMA operand it
 //            has to be).
-//            phase 1: a tile is 256 rows of Wd (D0, D1) times the unit's h.  Its fp32 results
-//            are stored, never rounded; the block that completes a 256-column strip of y adds
-//            p * result over the slots in order.
-//   kLinear  one phase: 256 weight rows times up to NB rows; bias, activation, residual.
+//            phase 1: a tile is up to 256 rows of Wd (D0, D1) times the unit's h.  Its fp32
+//            results are stored, never rounded; when all are there, y adds p * result over a
+//            token's slots in order.
+//   kLinear  one phase: up to 256 weight rows times up to NB rows; bias, activation, residual.
 //
-// Work split.  Every tile's contraction is cut into `parts` chunks (fixed by the host from the
-// sizes, so results do not depend on routing or timing), small enough for about
-// kChunksPerSm chunks per SM: SMs do not all stream equally fast, and with one equal share each
-// the slowest held the others up (one token, d = 4096, H = 11008: 15 us of 115).  An atomic
-// ticket hands the chunks out in order, phase 0's before phase 1's.  A block waits only for
-// chunks with smaller tickets, each of which a running block has taken and finishes without
-// waiting for a later one: the kernel makes progress whatever share of its blocks is resident.
-// Partial sums are fp32 and added in chunk order: those of h by the block that finishes a tile
-// last, those of the outputs in a final stage that all blocks share once the tickets are used
-// up.
+// Work split.  The host sets the tile height of each phase so that the tiles fill whole waves of
+// the SMs (TMA boxes may have any height; MMA rows past the box compute on stale shared memory
+// and are not stored).  Cutting the contraction instead, with partial sums in memory, costs a
+// fence, an atomic and a second pass per cut; while the weights saturate HBM each of these takes
+// microseconds (6 and 5 us measured for a block's first ones).  With equal tiles SMs need not
+// stream equally fast: those that end early leave their share of HBM to the others.  Only
+// kLinear with many rows and few columns cuts the contraction (`parts`, fixed by the sizes),
+// where low tiles would re-read the activations too often; the parts are fp32 and are added in
+// order at the end.
 //
-// The weight producer never waits for h, so the ring (about 200 KB per SM) fills with Wd while
-// the last h tiles are finished.  Phase 1 goes unit by unit in phase 0's order, so that the h
-// it needs first was finished first: the stream does not stop between the phases.
+// kMoe (and a cut kLinear) hands its chunks out by an atomic ticket, phase 0's before phase 1's.
+// A block waits only for phase-0 tiles, each of which a running block has taken and finishes
+// without waiting for anyone, and at the very end for all chunks: the kernel makes progress
+// whatever share of its blocks is resident.  The weight producer never waits for h, so the ring
+// fills with Wd while the last h tiles are finished; phase 1 goes unit by unit in phase 0's
+// order.  A finished h tile is published (fence and atomic) only when the next chunk's
+// accumulator is ready or there is nothing else to do, and output chunks are counted once per
+// block.
 //
 // Warp roles (256 threads, one block per SM):
 //   warp 0      weights: TMA boxes of 64 x 128, 128-byte swizzle; also fetches the tickets.
 //   warp 1      TMEM owner and MMA issuer.
 //   warps 2-3   activations: 16-byte cp.async into the same swizzle (rows are gathered: any
-//               token, any h row), handed over kLag stages later.
+//               token, any h row), which arrive on the stage's barrier when they land: these
+//               warps run ahead by the whole ring, as the weights do (handing stages over 3
+//               behind held the stream to 3.6 TB/s).
 //   warps 4-7   epilogue, one accumulator lane (weight row) per thread.
-//
-// While the weights saturate HBM a fence or an atomic takes microseconds (measured: 6 us and 5 us
-// for the first ones of a block), as long as a chunk's loads.  So they stay off the chunk's path:
-// there are several accumulator pairs, a finished h tile is published only when the next
-// chunk's accumulator is ready (its stores have long landed, the fence is short) or when there is
-// nothing else to do, and finished output chunks are counted once per block.
 //
 // Every wait is bounded; one that gives up sets the abort flag and device error 1.
 #pragma once
@@ -57,10 +57,8 @@ namespace fewtc {
 
 constexpr int kThreads = 256;
 constexpr int BK = 64;
-constexpr uint32_t kBoxBytes = 128 * 128;        // 128 weight rows x 64 16-bit columns
-constexpr uint32_t kWBytes = 2 * kBoxBytes;      // weights of a stage
-constexpr int kLag = 3;                          // stages between a cp.async and its hand-over
-constexpr int kMaxStages = 8;
+constexpr int kMaxStages = 12;
+constexpr int kMaxBlocksPerStage = 4;
 constexpr uint64_t kWaitNs = gmm::kWaitTimeoutNs;
 
 enum Mode { kMoe = 0, kLinear = 1 };
@@ -82,15 +80,18 @@ struct Params {
   // both
   const void* x;     // activations, rows of d (K) elements
   void* y;           // [T, d]; kLinear: [m, N]
-  int parts0, parts1;  // chunks per tile of each phase
-  float* part0;      // [parts0, rows, MT * 256] partials of phase 0 (parts0 > 1); rows: S or m
-  float* part1;      // [parts1, S, strips * 256] results of phase 1
-  int rows;          // S (kMoe) or m
-  int* counters;     // zeroed before the launch: ticket; finished chunks of the outputs; kMoe:
-                     // done[max_units] finished h tiles of a unit, tile[max_units * MT] finished
-                     // chunks of an h tile (parts0 > 1)
+  struct Shape {
+    int box_rows;    // weight rows of a TMA box (at most 128)
+    int boxes;       // boxes of a tile: accumulators D0, D1
+    int tiles;       // tiles of a unit
+    int blocks;      // 64-deep blocks of a stage
+  } shape[2];
+  int stage_bytes, stages;
+  int parts;         // kLinear: chunks that a tile's contraction is cut into
+  float* part;       // kMoe: [S, d] results of phase 1; kLinear: [parts, m, N] (parts > 1)
+  int* counters;     // zeroed before the launch (kLinear: parts > 1): ticket; finished chunks of
+                     // the outputs; kMoe: done[units] finished h tiles of a unit
   int max_units;
-  int stages;
 };
 
 constexpr int kTickets = 4;  // ticket ring
@@ -110,7 +111,7 @@ struct Ctl {
 };
 
 constexpr int kCtlBytes = (int)((sizeof(Ctl) + 15) / 16 * 16);
-constexpr int kStagedBytes = 8 * 256 * 4;  // accumulators of 8 rows on their way out
+constexpr int kStagedBytes = 16384;  // accumulators of 8 (at most 16) rows on their way out
 
 // Units of kLinear: at most NB consecutive rows of one group.
 struct RowUnits {
@@ -148,19 +149,20 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
            const __grid_constant__ CUtensorMap map2, const Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  constexpr uint32_t kStage = kWBytes + NB * 128;
   constexpr int kBufs = acc_bufs(NB);
   constexpr uint32_t kTmemCols = kBufs * 2 * NB;
   const int ST = p.stages;
-  Ctl& s = *reinterpret_cast<Ctl*>(smem + ST * kStage);
-  float* const staged = reinterpret_cast<float*>(smem + ST * kStage + kCtlBytes);  // [8][256]
-  uint8_t* plan_mem = smem + ST * kStage + kCtlBytes + kStagedBytes;
+  const uint32_t stage_bytes = (uint32_t)p.stage_bytes;
+  // After the ring, at least 16 KB that an MMA of a low box may read past the last stage.
+  Ctl& s = *reinterpret_cast<Ctl*>(smem + ST * stage_bytes);
+  float* const staged = reinterpret_cast<float*>(smem + ST * stage_bytes + kCtlBytes);  // [8][256]
+  uint8_t* plan_mem = smem + ST * stage_bytes + kCtlBytes + kStagedBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &s.abort;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
-      ptx::mbar_init(ptx::smem_u32(&s.full[i]), 3);
+      ptx::mbar_init(ptx::smem_u32(&s.full[i]), 1 + 64);  // weights, and each lane of warps 2-3
       ptx::mbar_init(ptx::smem_u32(&s.empty[i]), 1);
     }
     for (int i = 0; i < kBufs; ++i) {
@@ -193,6 +195,9 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
     pdl_wait();
     few::build_plan(plan, p.r, NB);
   } else {
+    // A cut product follows the kernel that zeroes its counters, which started after everything
+    // before it had ended: only the counters have to wait.
+    if (p.parts == 1) pdl_wait();
     ru.row = reinterpret_cast<int*>(plan_mem);
     ru.e = reinterpret_cast<int16_t*>(ru.row + p.max_units);
     ru.n = reinterpret_cast<uint16_t*>(ru.e + p.max_units);
@@ -237,29 +242,33 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
   ptx::tc_fence_after();
   const int U = MODE == kMoe ? *plan.num_units : s.num_units;
   const uint32_t tmem_base = s.tmem_base;
-  // Tiles per unit, 64-deep blocks per tile and chunks of each phase.
-  const int MT = MODE == kMoe ? (p.H + 127) / 128 : (p.N + 255) / 256;
-  const int strips = MODE == kMoe ? (p.d + 255) / 256 : 0;
+  // 64-deep blocks per tile and chunks of each phase.
   const int KB0 = ((MODE == kMoe ? p.d : p.K) + BK - 1) / BK, KB1 = (p.H + BK - 1) / BK;
-  const int G0 = U * MT * p.parts0, G1 = MODE == kMoe ? U * strips * p.parts1 : 0;
+  const int G0 = U * p.shape[0].tiles * (MODE == kLinear ? p.parts : 1);
+  const int G1 = MODE == kMoe ? U * p.shape[1].tiles : 0;
   int* const c_out = p.counters + 1;
   int* const c_done = p.counters + 2;
-  int* const c_tile = c_done + p.max_units;
+  // Without a cut, kLinear's blocks depend on nobody: tiles at a fixed stride, no counters.
+  const bool tickets = MODE == kMoe || p.parts > 1;
 
-  // Chunk t: unit u (expert e, first row row0, n rows), tile mt, blocks [kb0, kb0 + len).
+  // Chunk t: unit u (expert e, first row row0, n rows), weight rows [w0, w0 + boxes * box_rows),
+  // blocks [kb0, kb0 + len).
   struct Chunk {
-    int phase, u, mt, part, kb0, len, e, row0, n;
+    int phase, u, w0, part, kb0, len, e, row0, n;
   };
   auto decode = [&](int t) {
     Chunk c;
     c.phase = MODE == kMoe && t >= G0;
-    const int i = c.phase ? t - G0 : t;
-    const int parts = c.phase ? p.parts1 : p.parts0, tiles = c.phase ? strips : MT;
-    const int q = i / parts;
-    c.part = i - q * parts;
-    c.u = q / tiles;
-    c.mt = q - c.u * tiles;
-    part_range(c.phase ? KB1 : KB0, parts, c.part, c.kb0, c.len);
+    int q = c.phase ? t - G0 : t;
+    c.part = 0;
+    if (MODE == kLinear && p.parts > 1) {
+      c.part = q % p.parts;
+      q /= p.parts;
+    }
+    const auto& sh = p.shape[c.phase];
+    c.u = q / sh.tiles;
+    c.w0 = (q - c.u * sh.tiles) * sh.boxes * sh.box_rows;
+    part_range(c.phase ? KB1 : KB0, MODE == kLinear ? p.parts : 1, c.part, c.kb0, c.len);
     if constexpr (MODE == kMoe) {
       c.e = plan.unit_e[c.u]; c.row0 = plan.unit_pos[c.u]; c.n = plan.unit_n[c.u];
     } else {
@@ -274,11 +283,16 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
   };
   // This block's it-th ticket, for the warps that follow the producer; false at the end.
   auto ticket = [&](int it, Chunk& c) -> bool {
-    const int slot = it % kTickets;
-    if (!warp_wait(s.tk_full[slot], (it / kTickets) & 1)) return false;
-    const int t = *(volatile int*)&s.tk[slot];
-    __syncwarp();
-    if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&s.tk_empty[slot]));
+    int t;
+    if (tickets) {
+      const int slot = it % kTickets;
+      if (!warp_wait(s.tk_full[slot], (it / kTickets) & 1)) return false;
+      t = *(volatile int*)&s.tk[slot];
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&s.tk_empty[slot]));
+    } else {
+      t = blockIdx.x + it * gridDim.x;
+    }
     if (t >= G0 + G1) return false;
     c = decode(t);
     return true;
@@ -287,32 +301,46 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
   if (warp == 0) {
     // ---------------------------------------------------------- weights
     if (lane == 0) {
-      if (MODE == kLinear) pdl_wait();  // the counters are zeroed
+      if (MODE == kLinear && tickets) pdl_wait();  // the counters are zeroed
       int stage = 0;
       uint32_t parity = 1;
       bool ok = true;
       for (int it = 0; ok; ++it) {
-        const int slot = it % kTickets;
-        // The next ticket is taken when the last chunk's loads have been issued, so a slower
-        // SM takes fewer; its latency hides behind the ring.
-        if (!ptx::wait_bounded(ptx::smem_u32(&s.tk_empty[slot]), ((it / kTickets) & 1) ^ 1, abort_flag, kWaitNs)) break;
-        const int t = atomicAdd(p.counters, 1);
-        *(volatile int*)&s.tk[slot] = t;
-        ptx::mbar_arrive(ptx::smem_u32(&s.tk_full[slot]));
+        int t;
+        if (tickets) {
+          const int slot = it % kTickets;
+          // The next ticket is taken when the last chunk's loads have been issued, so a slower
+          // SM takes fewer; its latency hides behind the ring.
+          if (!ptx::wait_bounded(ptx::smem_u32(&s.tk_empty[slot]), ((it / kTickets) & 1) ^ 1, abort_flag, kWaitNs)) break;
+          t = atomicAdd(p.counters, 1);
+          *(volatile int*)&s.tk[slot] = t;
+          ptx::mbar_arrive(ptx::smem_u32(&s.tk_full[slot]));
+        } else {
+          t = blockIdx.x + it * gridDim.x;
+        }
         if (t >= G0 + G1) break;
         const Chunk c = decode(t);
         const bool gate_up = MODE == kMoe && !c.phase;
         const CUtensorMap* m0 = MODE == kMoe && c.phase ? &map2 : &map0;
         const CUtensorMap* m1 = gate_up ? &map1 : m0;
-        const int r0 = gate_up ? c.mt * 128 : c.mt * 256;
-        const int r1 = gate_up ? r0 : r0 + 128;
-        for (int kb = c.kb0; kb < c.kb0 + c.len; ++kb) {
+        const auto& sh = p.shape[c.phase];
+        const uint32_t box = (sh.box_rows + 7) / 8 * 1024;
+        const int r1 = c.w0 + (gate_up ? 0 : sh.box_rows);
+        const int boxes = gate_up ? 2 : sh.boxes;
+        for (int kb = c.kb0, left = c.len; left > 0; left -= sh.blocks) {
           if (!ptx::wait_bounded(ptx::smem_u32(&s.empty[stage]), parity, abort_flag, kWaitNs)) { ok = false; break; }
           const uint32_t bar = ptx::smem_u32(&s.full[stage]);
-          const uint32_t dst = ptx::smem_u32(smem) + stage * kStage;
-          ptx::mbar_arrive_expect_tx(bar, kWBytes);
-          ptx::tma_load_3d(dst, m0, bar, kb * BK, r0, c.e);
-          ptx::tma_load_3d(dst + kBoxBytes, m1, bar, kb * BK, r1, c.e);
+          uint32_t dst = ptx::smem_u32(smem) + stage * stage_bytes;
+          const int nb = min(left, sh.blocks);
+          ptx::mbar_arrive_expect_tx(bar, nb * boxes * sh.box_rows * 128);
+          for (int j = 0; j < nb; ++j, ++kb) {
+            ptx::tma_load_3d(dst, m0, bar, kb * BK, c.w0, c.e);
+            dst += box;
+            if (boxes == 2) {
+              ptx::tma_load_3d(dst, m1, bar, kb * BK, r1, c.e);
+              dst += box;
+            }
+          }
           if (++stage == ST) { stage = 0; parity ^= 1; }
         }
       }
@@ -330,18 +358,29 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
       if (!warp_wait(s.tmem_empty[buf], ((it / kBufs) & 1) ^ 1)) break;
       ptx::tc_fence_after();
       const uint32_t d0 = tmem_base + buf * 2 * NB;
-      for (int i = 0; i < c.len; ++i) {
+      const auto& sh = p.shape[c.phase];
+      const uint32_t box = (sh.box_rows + 7) / 8 * 1024;
+      const int boxes = MODE == kMoe && !c.phase ? 2 : sh.boxes;
+      for (int left = c.len; left > 0; left -= sh.blocks) {
         if (!warp_wait(s.full[stage], parity)) { ok = false; break; }
         ptx::tc_fence_after();
         if (lane == 0) {
-          const uint32_t sa = ptx::smem_u32(smem) + stage * kStage;
-          const uint32_t sb = sa + kWBytes;
+          ptx::fence_proxy_async_smem();  // the copies of warps 2-3 before the MMAs' reads
+          uint32_t sa = ptx::smem_u32(smem) + stage * stage_bytes;
+          uint32_t sb = sa + sh.blocks * boxes * box;
+          const int nb = min(left, sh.blocks);
+          for (int j = 0; j < nb; ++j) {
+            const uint32_t more = left != c.len || j > 0;
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            const uint64_t bd = ptx::make_sw128_desc(sb + kk * 32, 16, 1024);
-            ptx::mma_f16_ss<1>(d0, ptx::make_sw128_desc(sa + kk * 32, 16, 1024), bd, idesc, (i | kk) != 0);
-            ptx::mma_f16_ss<1>(d0 + NB, ptx::make_sw128_desc(sa + kBoxBytes + kk * 32, 16, 1024), bd,
-                               idesc, (i | kk) != 0);
+            for (int kk = 0; kk < 4; ++kk) {
+              const uint64_t bd = ptx::make_sw128_desc(sb + kk * 32, 16, 1024);
+              ptx::mma_f16_ss<1>(d0, ptx::make_sw128_desc(sa + kk * 32, 16, 1024), bd, idesc, more | kk);
+              if (boxes == 2)
+                ptx::mma_f16_ss<1>(d0 + NB, ptx::make_sw128_desc(sa + box + kk * 32, 16, 1024), bd,
+                                   idesc, more | kk);
+            }
+            sa += boxes * box;
+            sb += NB * 128;
           }
           ptx::mma_commit<1>(ptx::smem_u32(&s.empty[stage]));
         }
@@ -356,31 +395,11 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
     // ---------------------------------------------------------- activations
     const int l64 = (warp - 2) * 32 + lane;
     const int c16 = l64 & 7;  // 16-byte column of a 128-byte row
-    int stage = 0, held = 0, held_stage = 0;
+    int stage = 0;
     uint32_t parity = 1;
     bool ok = true;
     Chunk c;
-    // Hands over the oldest `count` stages whose copies have landed.
-    auto hand_over = [&](int count) {
-      ptx::fence_proxy_async_smem();
-      __syncwarp();
-      for (int i = 0; i < count; ++i) {
-        if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&s.full[held_stage]));
-        if (++held_stage == ST) held_stage = 0;
-      }
-      held -= count;
-    };
-    auto drain = [&]() {
-      if (held == 0) return;
-      ptx::cp_async_wait<0>();
-      hand_over(held);
-    };
-    for (int it = 0; ok; ++it) {
-      // Nothing is held back while this warp waits for a ticket (or, below, for h).
-      if (!__all_sync(0xffffffffu, ptx::mbar_try_wait(ptx::smem_u32(&s.tk_full[it % kTickets]),
-                                                      (it / kTickets) & 1)))
-        drain();
-      if (!ticket(it, c)) break;
+    for (int it = 0; ok && ticket(it, c); ++it) {
       const int cols = MODE == kLinear ? p.K : c.phase ? p.H : p.d;
       const T* rows[NB / 8];
 #pragma unroll
@@ -391,11 +410,11 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
         rows[i] = static_cast<const T*>(MODE == kMoe && c.phase ? p.h : p.x) + src * cols + c16 * 8;
       }
       if (MODE == kMoe && c.phase) {
-        // the unit's h: every one of its MT tiles finished
-        if (!__all_sync(0xffffffffu, ptx::ld_acquire_gpu(c_done + c.u) >= MT)) {
-          drain();
+        // the unit's h: every one of its tiles finished
+        const int want = p.shape[0].tiles;
+        if (!__all_sync(0xffffffffu, ptx::ld_acquire_gpu(c_done + c.u) >= want)) {
           const uint64_t t0 = ptx::globaltimer();
-          while (ptx::ld_acquire_gpu(c_done + c.u) < MT) {
+          while (ptx::ld_acquire_gpu(c_done + c.u) < want) {
             if (*abort_flag || ptx::globaltimer() - t0 > kWaitNs) { *abort_flag = 1; ok = false; break; }
             __nanosleep(32);
           }
@@ -403,72 +422,45 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
           if (!ok) break;
         }
       }
-      for (int kb = c.kb0; kb < c.kb0 + c.len; ++kb) {
+      const auto& sh = p.shape[c.phase];
+      const uint32_t a_bytes = sh.blocks * (MODE == kMoe && !c.phase ? 2 : sh.boxes) * ((sh.box_rows + 7) / 8 * 1024);
+      for (int kb = c.kb0, left = c.len; left > 0; left -= sh.blocks) {
         if (!warp_wait(s.empty[stage], parity)) { ok = false; break; }
-        const uint32_t dst = ptx::smem_u32(smem) + stage * kStage + kWBytes;
-        const bool in = kb * BK + c16 * 8 < cols;  // cols is a multiple of 8
+        uint32_t dst = ptx::smem_u32(smem) + stage * stage_bytes + a_bytes;
+        const int nb = min(left, sh.blocks);
+        for (int j = 0; j < nb; ++j, ++kb, dst += NB * 128) {
+          const bool in = kb * BK + c16 * 8 < cols;  // cols is a multiple of 8
 #pragma unroll
-        for (int i = 0; i < NB / 8; ++i) {
-          const int r = (l64 >> 3) + 8 * i;
-          if (r < c.n)
-            ptx::cp_async16(dst + r * 128 + ((c16 ^ (r & 7)) << 4),
-                            rows[i] + (in ? kb * BK : -(c16 * 8)), in ? 16u : 0u);
+          for (int i = 0; i < NB / 8; ++i) {
+            const int r = (l64 >> 3) + 8 * i;
+            if (r < c.n)
+              ptx::cp_async16(dst + r * 128 + ((c16 ^ (r & 7)) << 4),
+                              rows[i] + (in ? kb * BK : -(c16 * 8)), in ? 16u : 0u);
+          }
         }
-        ptx::cp_async_commit();
+        ptx::cp_async_arrive(ptx::smem_u32(&s.full[stage]));
         if (++stage == ST) { stage = 0; parity ^= 1; }
-        if (++held > kLag) {
-          ptx::cp_async_wait<kLag>();
-          hand_over(1);
-        }
       }
     }
-    drain();
+    ptx::cp_async_wait_all();
   } else {
     // ---------------------------------------------------------- epilogue
     const int row = (warp - 4) * 32 + lane;  // accumulator lane
     const bool lead = row == 0;
-    const int64_t ld0 = (int64_t)MT * 256, ld1 = (int64_t)strips * 256;
-    Chunk c, held = {};
-    bool pending = false;  // `held` is a phase-0 chunk of kMoe that is stored but not published
-    int outputs = 0;       // chunks of the outputs that this block has stored
-    // h of column `row` of a tile: D0 is its gate, D1 its up.
-    auto store_h = [&](const Chunk& k, int j, float gate, float up) {
-      const int col = k.mt * 128 + row;
-      if (col < p.H)
-        static_cast<T*>(p.h)[(int64_t)(k.row0 + j) * p.H + col] = from_f32<T>(gate * sigmoid_f32(gate) * up);
-    };
-    // Counts `held`; of a cut tile, the block that finishes it last adds the parts in order.
+    Chunk c;
+    int held_unit = -1;  // kMoe: the unit of an h tile that is stored but not published
+    int outputs = 0;     // chunks of the outputs that this block has stored
     auto publish = [&]() {
-      pending = false;
       ptx::fence_acq_rel_gpu();
       ptx::named_barrier(1, 128);
-      if (p.parts0 > 1) {
-        if (lead) s.flag = ptx::atom_add_gpu(c_tile + held.u * MT + held.mt, 1) + 1 == p.parts0;
-        ptx::named_barrier(1, 128);
-        if (!*(volatile int*)&s.flag) return;
-        ptx::fence_acq_rel_gpu();
-        const float* src = p.part0 + (int64_t)held.row0 * ld0 + held.mt * 256 + row;
-        const int64_t step = (int64_t)p.rows * ld0;
-#pragma unroll 1
-        for (int j = 0; j < held.n; ++j) {
-          float a = 0.f, g = 0.f;
-#pragma unroll 8
-          for (int q = 0; q < p.parts0; ++q) {
-            a += __ldcg(src + q * step + j * ld0);
-            g += __ldcg(src + q * step + j * ld0 + 128);
-          }
-          store_h(held, j, a, g);
-        }
-        ptx::fence_acq_rel_gpu();
-        ptx::named_barrier(1, 128);
-      }
-      if (lead) ptx::atom_add_gpu(c_done + held.u, 1);
+      if (lead) ptx::red_add_gpu(c_done + held_unit, 1);
+      held_unit = -1;
     };
     // The four warps meet at barriers, so each wait's outcome is agreed on by all of them.
     for (int it = 0;; ++it) {
       const int buf = it % kBufs;
       const uint32_t parity = (it / kBufs) & 1;
-      if (pending) {
+      if (MODE == kMoe && held_unit >= 0) {
         const bool ready = ptx::mbar_try_wait(ptx::smem_u32(&s.tk_full[it % kTickets]), (it / kTickets) & 1) &&
                            ptx::mbar_try_wait(ptx::smem_u32(&s.tmem_full[buf]), parity);
         if (!ptx::named_barrier_all(1, 128, ready)) publish();
@@ -476,13 +468,14 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
       const bool more = ticket(it, c);
       if (!ptx::named_barrier_all(1, 128, more)) break;
       if (!ptx::named_barrier_all(1, 128, warp_wait(s.tmem_full[buf], parity))) break;
-      if (pending) publish();
+      if (MODE == kMoe && held_unit >= 0) publish();
       ptx::tc_fence_after();
       const uint32_t tb = tmem_base + ((uint32_t)((warp - 4) * 32) << 16) + buf * 2 * NB;
-      const bool whole = !c.phase && p.parts0 == 1;
-      // Partial sums: this thread's two columns of the tile, row by row.
-      const int64_t ld = c.phase ? ld1 : ld0;
-      float* dst = (c.phase ? p.part1 : p.part0) + ((int64_t)c.part * p.rows + c.row0) * ld + c.mt * 256 + row;
+      const auto& sh = p.shape[c.phase];
+      const int limit = MODE == kLinear ? p.N : c.phase ? p.d : p.H;
+      // This thread's columns of the output: one per accumulator.
+      const int col0 = row < sh.box_rows ? c.w0 + row : limit;
+      const int col1 = row < sh.box_rows && sh.boxes == 2 ? c.w0 + sh.box_rows + row : limit;
 #pragma unroll 1
       for (int j0 = 0; j0 < c.n; j0 += 8) {
         uint32_t v0[8], v1[8];
@@ -498,44 +491,40 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
         const int m = min(8, c.n - j0);
 #pragma unroll 1
         for (int j = 0; j < m; ++j) {
-          const float a = staged[j * 256 + row], g = staged[j * 256 + 128 + row];
-          if (!whole) {
-            dst[(j0 + j) * ld] = a;
-            dst[(j0 + j) * ld + 128] = g;
-          } else if constexpr (MODE == kMoe) {
-            store_h(c, j0 + j, a, g);
+          const float a = staged[j * 256 + row], b = staged[j * 256 + 128 + row];
+          const int64_t r = c.row0 + j0 + j;
+          if (MODE == kMoe && !c.phase) {
+            if (col0 < limit) static_cast<T*>(p.h)[r * p.H + col0] = from_f32<T>(a * sigmoid_f32(a) * b);
+          } else if (MODE == kMoe || p.parts > 1) {
+            float* dst = p.part + (MODE == kMoe ? r : (int64_t)c.part * p.m + r) * limit;
+            if (col0 < limit) dst[col0] = a;
+            if (col1 < limit) dst[col1] = b;
           } else {
 #pragma unroll 1
-            for (int i = 0; i < 2; ++i)
-              linear_out<T>(p, c.e, c.row0 + j0 + j, c.mt * 256 + i * 128 + row, i ? g : a);
+            for (int i = 0; i < 2; ++i) linear_out<T>(p, c.e, r, i ? col1 : col0, i ? b : a);
           }
         }
       }
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&s.tmem_empty[buf]));
-      if (MODE == kMoe && !c.phase) {
-        held = c;
-        pending = true;
-      } else {
-        ++outputs;
-      }
+      if (MODE == kMoe && !c.phase) held_unit = c.u;
+      else ++outputs;
     }
     // Abandoned work is not published (the wait that gave up has set the abort flag).
-    if (pending && !ptx::named_barrier_all(1, 128, *abort_flag != 0)) publish();
-    if (MODE == kMoe || p.parts0 > 1) {
+    if (MODE == kMoe && held_unit >= 0 && ptx::named_barrier_all(1, 128, *abort_flag == 0)) publish();
+    if (tickets) {
       ptx::fence_acq_rel_gpu();
       ptx::named_barrier(1, 128);
-      if (lead && outputs > 0) ptx::atom_add_gpu(c_out, outputs);
+      if (lead && outputs > 0) ptx::red_add_gpu(c_out, outputs);
     }
   }
 
   // ------------------------------------------------------------ final stage
-  // Every ticket is taken.  64 columns of one output row at a time: 4 threads per column each
-  // add a quarter of the terms, then the quarters are added in order.
+  // Every ticket is taken.  Four neighbouring elements of an output row at a time; when there are
+  // many terms to add, 2 to 8 neighbouring lanes each add every split-th and then join.
   __syncthreads();
-  if (!*abort_flag && (MODE == kMoe || p.parts0 > 1)) {
-    float* red = reinterpret_cast<float*>(smem);  // the ring is idle
+  if (!*abort_flag && tickets) {
     if (threadIdx.x == 0) {
       const int want = MODE == kMoe ? G1 : G0;
       const uint64_t t0 = ptx::globaltimer();
@@ -546,49 +535,62 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
       }
     }
     __syncthreads();
-    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-    const int width = MODE == kMoe ? p.d : p.N;
-    const int groups = (width + 63) / 64;
-    const int out_rows = MODE == kMoe ? p.r.num_tokens : p.rows;
-    const int64_t ld = (int64_t)(MODE == kMoe ? strips : MT) * 256;
-    const int parts = MODE == kMoe ? p.parts1 : p.parts0;
-    const int64_t step = (int64_t)p.rows * ld;
-    const int items = *(volatile int*)&s.flag ? groups * out_rows : 0;
-    for (int i = blockIdx.x; i < items; i += gridDim.x) {
-      const int r = i / groups, g = i - r * groups, col = g * 64 + tx;
-      int unit = 0;
-      if constexpr (MODE == kLinear) {  // the row's unit: the last that starts at or before it
-        int hi = U - 1;
-        while (unit < hi) {
-          const int mid = (unit + hi + 1) >> 1;
-          if (ru.row[mid] <= r) unit = mid; else hi = mid - 1;
-        }
-        if (U == 0 || r < ru.row[unit] || r >= ru.row[unit] + ru.n[unit]) continue;  // in no group
-      }
-      float acc = 0.f;
-      if constexpr (MODE == kMoe) {
-        const int terms = p.r.K * parts;
+    const int width = MODE == kMoe ? p.d : p.N;  // a multiple of 8
+    const int out_rows = MODE == kMoe ? p.r.num_tokens : (int)p.m;
+    const int terms = MODE == kMoe ? p.r.K : p.parts;
+    const int split = terms <= 4 ? 1 : terms <= 8 ? 2 : terms <= 16 ? 4 : 8;
+    const int sub = lane & (split - 1);
+    const int quads = width / 4;
+    const long long items = (long long)quads * out_rows;
+    const long long stride = (long long)gridDim.x * kThreads / split;
+    // every lane of a warp makes the same number of turns (the join is a warp shuffle)
+    const long long first = (long long)(blockIdx.x * kThreads + warp * 32) / split;
+    for (long long i0 = first; *(volatile int*)&s.flag && i0 < items; i0 += stride) {
+      const long long i = i0 + lane / split;
+      const bool live = i < items;
+      const int r = live ? (int)(i / quads) : 0, col = live ? (int)(i - (long long)r * quads) * 4 : 0;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-        for (int j = ty; j < terms; j += 4) {
-          const int k = j / parts, sl = r * p.r.K + k, pos = plan.pos[sl];
-          if (pos >= 0)
-            acc = fmaf(plan.w[sl], __ldcg(p.part1 + (int64_t)(j - k * parts) * step + pos * ld + col), acc);
-        }
-      } else {
-#pragma unroll 4
-        for (int j = ty; j < parts; j += 4) acc += __ldcg(p.part0 + j * step + r * ld + col);
-      }
-      red[threadIdx.x] = acc;
-      __syncthreads();
-      if (ty == 0 && col < width) {
-        const float v = ((red[tx] + red[64 + tx]) + red[128 + tx]) + red[192 + tx];
+      for (int k = sub; k < terms; k += split) {
+        float w = 1.f;
+        int64_t at;
         if constexpr (MODE == kMoe) {
-          static_cast<T*>(p.y)[(int64_t)r * p.d + col] = from_f32<T>(v);
+          const int sl = r * terms + k, pos = plan.pos[sl];
+          if (pos < 0) continue;
+          w = plan.w[sl];
+          at = pos;
         } else {
-          linear_out<T>(p, ru.e[unit], r, col, v);
+          at = (int64_t)k * p.m + r;
         }
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part + at * width + col));
+        acc.x = fmaf(w, v.x, acc.x);
+        acc.y = fmaf(w, v.y, acc.y);
+        acc.z = fmaf(w, v.z, acc.z);
+        acc.w = fmaf(w, v.w, acc.w);
       }
-      __syncthreads();
+      for (int o = 1; o < split; o <<= 1) {
+        acc.x += __shfl_xor_sync(0xffffffffu, acc.x, o);
+        acc.y += __shfl_xor_sync(0xffffffffu, acc.y, o);
+        acc.z += __shfl_xor_sync(0xffffffffu, acc.z, o);
+        acc.w += __shfl_xor_sync(0xffffffffu, acc.w, o);
+      }
+      if (!live || sub != 0) continue;
+      int e = 0;
+      if constexpr (MODE == kLinear) {  // the row's unit: the last that starts at or before it
+        int lo = 0, hi = U - 1;
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (ru.row[mid] <= r) lo = mid; else hi = mid - 1;
+        }
+        if (U == 0 || r < ru.row[lo] || r >= ru.row[lo] + ru.n[lo]) continue;  // in no group
+        e = ru.e[lo];
+      }
+#pragma unroll 1
+      for (int q = 0; q < 4; ++q) {
+        const float v = q == 0 ? acc.x : q == 1 ? acc.y : q == 2 ? acc.z : acc.w;
+        if constexpr (MODE == kMoe) static_cast<T*>(p.y)[(int64_t)r * width + col + q] = from_f32<T>(v);
+        else linear_out<T>(p, e, r, col + q, v);
+      }
     }
   }
 

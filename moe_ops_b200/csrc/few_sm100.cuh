@@ -366,21 +366,31 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
         ptx::tc_fence_after();
         if (lane == 0) {
           ptx::fence_proxy_async_smem();  // the copies of warps 2-3 before the MMAs' reads
-          uint32_t sa = ptx::smem_u32(smem) + stage * stage_bytes;
-          uint32_t sb = sa + sh.blocks * boxes * box;
+          const uint32_t sa = ptx::smem_u32(smem) + stage * stage_bytes;
+          uint32_t da = ptx::sw128_desc_lo(sa), db = ptx::sw128_desc_lo(sa + sh.blocks * boxes * box);
           const int nb = min(left, sh.blocks);
-          for (int j = 0; j < nb; ++j) {
-            const uint32_t more = left != c.len || j > 0;
+          const uint32_t box16 = box >> 4;
+          uint32_t more = left != c.len;
+          if (boxes == 2) {
+            for (int j = 0; j < nb; ++j) {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-              const uint64_t bd = ptx::make_sw128_desc(sb + kk * 32, 16, 1024);
-              ptx::mma_f16_ss<1>(d0, ptx::make_sw128_desc(sa + kk * 32, 16, 1024), bd, idesc, more | kk);
-              if (boxes == 2)
-                ptx::mma_f16_ss<1>(d0 + NB, ptx::make_sw128_desc(sa + box + kk * 32, 16, 1024), bd,
-                                   idesc, more | kk);
+              for (int kk = 0; kk < 4; ++kk) {
+                ptx::mma_f16_sw128(d0, da + 2 * kk, db + 2 * kk, idesc, kk ? 1u : more);
+                ptx::mma_f16_sw128(d0 + NB, da + box16 + 2 * kk, db + 2 * kk, idesc, kk ? 1u : more);
+              }
+              da += 2 * box16;
+              db += NB * 8;
+              more = 1;
             }
-            sa += boxes * box;
-            sb += NB * 128;
+          } else {
+            for (int j = 0; j < nb; ++j) {
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                ptx::mma_f16_sw128(d0, da + 2 * kk, db + 2 * kk, idesc, kk ? 1u : more);
+              da += box16;
+              db += NB * 8;
+              more = 1;
+            }
           }
           ptx::mma_commit<1>(ptx::smem_u32(&s.empty[stage]));
         }

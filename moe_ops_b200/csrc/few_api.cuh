@@ -34,35 +34,61 @@ static size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 // crowded expert's weights once.
 static int few_nb(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
-// Tiles of a phase: `rows` weight rows per unit (per box: gate_up tiles hold two boxes of the same
-// rows), about `units` units.  As few waves of tiles over the SMs as a tile's height allows, and
-// tiles as high as then fill the waves; never lower than the activations' rows would make
-// worthwhile (a tile re-reads them all).
-static fewtc::Params::Shape few_shape(double units, int64_t rows, bool gate_up, int nb) {
-  fewtc::Params::Shape s = {};
-  const int64_t most = gate_up ? 128 : 256;
+// Tile height and cut of a phase.  `units` times `rows` weight rows (of each of gate and up) with
+// KB blocks of contraction, `n` rows of activations per unit.  Counted in SM cycles: a
+// 64-deep block of a tile takes the larger of its weights at an SM's share of HBM (26 bytes per
+// cycle), weights and activations at the rate an SM reads L2 (50), and 4 MMAs (90 each); a chunk
+// costs about 1000 more, and adding parts up at the end 6000 and a pass over them.  All SMs are
+// taken to run equally long, waves x chunk; heights that fill 1 to 4 waves are compared.
+struct FewSplit {
+  fewtc::Params::Shape shape;
+  int parts;
+};
+static FewSplit few_split(double units, int64_t rows, int64_t KB, double n, bool gate_up, bool may_cut) {
   const double sms = num_sms(current_device());
-  const double waves = ceil(units * (double)rows / ((double)most * sms));
-  int64_t tiles = std::max<int64_t>(1, (int64_t)(sms * waves / units));
-  int64_t height = std::max((rows + tiles - 1) / tiles, std::min<int64_t>(rows, std::max(16, nb / 2)));
-  height = std::min(height, most);
-  s.boxes = !gate_up && height > 128 ? 2 : 1;
-  s.box_rows = (int)((height + s.boxes - 1) / s.boxes);
-  s.tiles = (int)((rows + s.boxes * s.box_rows - 1) / (s.boxes * s.box_rows));
-  return s;
+  const int64_t most = std::min<int64_t>(gate_up ? 128 : 256, (rows + 7) / 8 * 8);
+  double best = 1e30;
+  FewSplit f = {};
+  for (const int64_t parts : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32}) {
+    if (parts > 1 && !may_cut) break;
+    const int64_t len = (KB + parts - 1) / parts;
+    if ((KB + len - 1) / len != parts) continue;  // equal chunks, none empty
+    if (parts > 1 && len < 4) break;
+    for (int w = 1; w <= 5; ++w) {
+      int64_t height = (int64_t)(units * parts * rows / (sms * w)) + 1;
+      height = std::min(most, std::max<int64_t>(16, (height + 7) / 8 * 8));
+      if (w == 5) height = most;
+      const int64_t tiles = (rows + height - 1) / height;
+      const double weights = (gate_up ? 256.0 : 128.0) * height;
+      const double block = std::max({weights / 26, (weights + n * 128) / 50, 360.0});
+      double cost = ceil(units * tiles * parts / sms - 1e-6) * (len * block + 1000);
+      if (parts > 1) cost += 6000 + parts * units * n * rows * 8 / (sms * 30);
+      if (cost < best) {
+        best = cost;
+        f.parts = (int)parts;
+        f.shape.rows = (int)height;
+        f.shape.tiles = (int)tiles;
+      }
+    }
+  }
+  f.shape.block_bytes = (gate_up ? 2 : 1) * f.shape.rows * 128;  // heights are multiples of 8
+  f.shape.n = (f.shape.block_bytes / 128 + 15) / 16 * 16;
+  return f;
 }
 
-// Ring geometry: as many 64-deep blocks per stage as about 40 KB hold, then as many stages as
-// shared memory holds.
+// Ring geometry: as many 64-deep blocks per stage as about 36 KB hold, then as many stages as
+// shared memory holds; and the accumulators.
 static int few_ring(fewtc::Params& p, int phases, int nb, int table_bytes) {
-  int bytes = 0;
+  int bytes = 0, cols = 16;
   for (int i = 0; i < phases; ++i) {
     auto& s = p.shape[i];
-    const int boxes = phases == 2 && i == 0 ? 2 : s.boxes;
-    const int block = boxes * ((s.box_rows + 7) / 8 * 1024) + nb * 128;
-    s.blocks = std::max(1, std::min(fewtc::kMaxBlocksPerStage, 40960 / block));
+    const int block = s.block_bytes + nb * 128;
+    s.blocks = std::max(1, std::min(fewtc::kMaxBlocksPerStage, 36864 / block));
     bytes = std::max(bytes, s.blocks * block);
+    cols = std::max(cols, (s.n + 31) / 32 * 32);
   }
+  p.acc_cols = cols;
+  p.bufs = std::min(4, 512 / cols);
   p.stage_bytes = bytes;
   const size_t fixed = 1024 + fewtc::kCtlBytes + fewtc::kStagedBytes + (size_t)table_bytes;
   MOE_REQUIRE(fixed < kMaxSmem, "few rows: routing tables too large");
@@ -76,6 +102,7 @@ static int few_ring(fewtc::Params& p, int phases, int nb, int table_bytes) {
 struct FewWorkspace {
   size_t logits, h, counters, part, total;
   int num_counters, max_units;
+  FewSplit split0, split1;
 };
 static FewWorkspace few_workspace(int64_t T, int64_t d, int64_t H, int64_t E, int64_t K, int dtype) {
   FewWorkspace w = {};
@@ -83,10 +110,19 @@ static FewWorkspace few_workspace(int64_t T, int64_t d, int64_t H, int64_t E, in
   w.logits = 0;
   w.h = align256((size_t)T * E * 4);
   w.counters = w.h + align256(S * H * 4);
+  if (dtype == MOE_F32 || d == 0 || H == 0) {
+    w.total = w.counters;
+    return w;
+  }
+  // experts that the tokens are expected to touch when each picks K of E, and their rows
+  const double touched = K >= E ? (double)E : E * (1.0 - pow(1.0 - (double)K / E, (double)T));
+  const double n = std::min<double>(few_nb(T), S / touched);
+  w.split0 = few_split(touched, H, (d + fewtc::BK - 1) / fewtc::BK, n, true, false);
+  w.split1 = few_split(touched, d, (H + fewtc::BK - 1) / fewtc::BK, n, false, true);
   w.max_units = few::plan_max_units((int)S, (int)E, few_nb(T));
   w.num_counters = 2 + w.max_units;
-  w.part = w.counters + (dtype == MOE_F32 ? 0 : align256((size_t)w.num_counters * 4));
-  w.total = w.part + (dtype == MOE_F32 ? 0 : align256(S * d * 4));
+  w.part = w.counters + align256((size_t)w.num_counters * 4);
+  w.total = w.part + align256((size_t)w.split1.parts * S * d * 4);
   return w;
 }
 
@@ -198,9 +234,9 @@ static int zero_counters(int* counters, int n, cudaStream_t s) {
 }
 
 static int few_weight_map(CUtensorMap* map, const void* w, int dtype, int64_t inner, int64_t rows, int64_t E,
-                          int box_rows) {
+                          int rows_of_box) {
   const uint64_t dims[3] = {(uint64_t)inner, (uint64_t)rows, (uint64_t)E};
-  const uint32_t box[3] = {(uint32_t)fewtc::BK, (uint32_t)box_rows, 1};
+  const uint32_t box[3] = {(uint32_t)fewtc::BK, (uint32_t)rows_of_box, 1};
   return make_map(map, w, dtype, 3, dims, box);
 }
 
@@ -215,21 +251,18 @@ static int few_tc_launch(const FewArgs& a, const few::Routing& r, const FewWorks
   p.x = a.x;
   p.y = a.out;
   p.h = ws + w.h;
-  p.parts = 1;
+  p.parts = w.split1.parts;
   p.part = (float*)(ws + w.part);
   p.counters = (int*)(ws + w.counters);
   p.max_units = w.max_units;
-  // experts that the tokens are expected to touch when each picks K of E
-  const double touched =
-      a.topk >= a.E ? (double)a.E : a.E * (1.0 - pow(1.0 - (double)a.topk / a.E, (double)a.num_tokens));
-  p.shape[0] = few_shape(touched, a.hidden, true, nb);
-  p.shape[1] = few_shape(touched, a.d, false, nb);
+  p.shape[0] = w.split0.shape;
+  p.shape[1] = w.split1.shape;
   int rc;
   if ((rc = few_ring(p, 2, nb, table))) return rc;
   CUtensorMap maps[3];
-  if ((rc = few_weight_map(&maps[0], a.w_gate, a.dtype, a.d, a.hidden, a.E, p.shape[0].box_rows))) return rc;
-  if ((rc = few_weight_map(&maps[1], a.w_up, a.dtype, a.d, a.hidden, a.E, p.shape[0].box_rows))) return rc;
-  if ((rc = few_weight_map(&maps[2], a.w_down, a.dtype, a.hidden, a.d, a.E, p.shape[1].box_rows))) return rc;
+  if ((rc = few_weight_map(&maps[0], a.w_gate, a.dtype, a.d, a.hidden, a.E, p.shape[0].rows))) return rc;
+  if ((rc = few_weight_map(&maps[1], a.w_up, a.dtype, a.d, a.hidden, a.E, p.shape[0].rows))) return rc;
+  if ((rc = few_weight_map(&maps[2], a.w_down, a.dtype, a.hidden, a.d, a.E, p.shape[1].rows))) return rc;
   const unsigned grid = (unsigned)num_sms(current_device());
   if (a.dtype == MOE_BF16)
     return few_kernel_nb<fewtc::kMoe, 1, __nv_bfloat16>(nb, maps, p, grid, table, a.stream);

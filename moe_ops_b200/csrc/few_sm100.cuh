@@ -2,29 +2,29 @@
 // MoE layer (kMoe) and linear / grouped_linear for a few rows (kLinear).
 //
 // With n rows (1 to 64) per weight matrix the product does 2 n flops per 2-byte weight, far
-// below the ridge: the kernel is a stream over the weights and everything else hides behind
-// it.  So the weights are the MMA's A operand (M = 128 weight rows) and the activations its B
-// operand (N = n rounded up to 16): one 64-deep block of 256 weight rows is a 32 KB stage, its
-// 8 MMAs take a fraction of the stage's HBM time, and no register touches a weight.
+// below the ridge: the kernel is a stream over the weights and everything else hides behind it.
+// The weights are the MMA's B operand (N = the tile's weight rows, up to 256) and the activations
+// its A operand (M = 128 rows, of which n hold data; the others compute on stale shared memory
+// and are not stored).  A tcgen05.mma takes about 90 cycles to issue however small it is
+// (measured the same for M = 64 and 128, N = 16 to 128), so an instruction should cover many
+// weights: 256 rows of 16 elements are 8 KB, 64 bytes per cycle against the 26 that an SM's share
+// of HBM delivers.  As the A operand (128 rows) the same weights need twice the instructions,
+// which bounded tiles of 75 rows at 4.2 TB/s.
 //
-//   kMoe     phase 0: a tile is up to 128 columns of h: those gate rows (accumulator D0) and the
-//            same up rows (D1) of one unit (an expert's rows, at most NB); its epilogue forms
+//   kMoe     phase 0: a tile is up to 128 columns of h: those gate rows and the same up rows of
+//            one unit (an expert's rows of activations, at most NB); its epilogue forms
 //            h = silu(gate) * up in fp32 and rounds it once to 16 bits (as an MMA operand it
 //            has to be).
-//            phase 1: a tile is up to 256 rows of Wd (D0, D1) times the unit's h.  Its fp32
-//            results are stored, never rounded; when all are there, y adds p * result over a
-//            token's slots in order.
+//            phase 1: a tile is up to 256 rows of Wd times the unit's h.  Its fp32 results are
+//            stored, never rounded; when all are there, y adds p * result over a token's slots.
 //   kLinear  one phase: up to 256 weight rows times up to NB rows; bias, activation, residual.
 //
-// Work split.  The host sets the tile height of each phase so that the tiles fill whole waves of
-// the SMs (TMA boxes may have any height; MMA rows past the box compute on stale shared memory
-// and are not stored).  Cutting the contraction instead, with partial sums in memory, costs a
-// fence, an atomic and a second pass per cut; while the weights saturate HBM each of these takes
-// microseconds (6 and 5 us measured for a block's first ones).  With equal tiles SMs need not
-// stream equally fast: those that end early leave their share of HBM to the others.  Only
-// kLinear with many rows and few columns cuts the contraction (`parts`, fixed by the sizes),
-// where low tiles would re-read the activations too often; the parts are fp32 and are added in
-// order at the end.
+// Work split.  The host picks each phase's tile height and the number of chunks that a tile's
+// contraction is cut into (`parts`) from the sizes alone, so that the chunks fill whole waves of
+// the SMs (results depend on neither routing nor timing).  Phase 0 is never cut: adding up
+// parts of h before phase 1 costs a fence, an atomic and a second pass per cut, and while the
+// weights saturate HBM each of these takes microseconds (6 and 5 us measured for a block's first
+// ones).  Parts of the outputs are fp32 and cost little: all are added at the end, in order.
 //
 // kMoe (and a cut kLinear) hands its chunks out by an atomic ticket, phase 0's before phase 1's.
 // A block waits only for phase-0 tiles, each of which a running block has taken and finishes
@@ -36,13 +36,14 @@
 // block.
 //
 // Warp roles (256 threads, one block per SM):
-//   warp 0      weights: TMA boxes of 64 x 128, 128-byte swizzle; also fetches the tickets.
+//   warp 0      weights: TMA boxes 64 elements wide, 128-byte swizzle; also fetches the tickets.
 //   warp 1      TMEM owner and MMA issuer.
 //   warps 2-3   activations: 16-byte cp.async into the same swizzle (rows are gathered: any
 //               token, any h row), which arrive on the stage's barrier when they land: these
 //               warps run ahead by the whole ring, as the weights do (handing stages over 3
 //               behind held the stream to 3.6 TB/s).
-//   warps 4-7   epilogue, one accumulator lane (weight row) per thread.
+//   warps 4-7   epilogue: accumulators (a lane per row of activations) through shared memory, so
+//               that stores run along the output's columns.
 //
 // Every wait is bounded; one that gives up sets the abort flag and device error 1.
 #pragma once
@@ -81,14 +82,16 @@ struct Params {
   const void* x;     // activations, rows of d (K) elements
   void* y;           // [T, d]; kLinear: [m, N]
   struct Shape {
-    int box_rows;    // weight rows of a TMA box (at most 128)
-    int boxes;       // boxes of a tile: accumulators D0, D1
+    int rows;        // weight rows of a tile = of its TMA box (a gate/up tile: of each of its two)
     int tiles;       // tiles of a unit
     int blocks;      // 64-deep blocks of a stage
+    int block_bytes; // weights of a block (heights are multiples of 8 rows)
+    int n;           // N of the MMA
   } shape[2];
   int stage_bytes, stages;
-  int parts;         // kLinear: chunks that a tile's contraction is cut into
-  float* part;       // kMoe: [S, d] results of phase 1; kLinear: [parts, m, N] (parts > 1)
+  int acc_cols, bufs;  // TMEM columns of an accumulator, and their number (at most 4)
+  int parts;         // chunks that a tile's contraction is cut into (kMoe: in phase 1)
+  float* part;       // kMoe: [parts, S, d] results of phase 1; kLinear: [parts, m, N] (parts > 1)
   int* counters;     // zeroed before the launch (kLinear: parts > 1): ticket; finished chunks of
                      // the outputs; kMoe: done[units] finished h tiles of a unit
   int max_units;
@@ -96,12 +99,9 @@ struct Params {
 
 constexpr int kTickets = 4;  // ticket ring
 
-// Accumulator pairs of a unit size: 256 TMEM columns, 512 for NB = 64.
-__host__ __device__ constexpr int acc_bufs(int nb) { return nb == 16 ? 8 : 4; }
-
 struct Ctl {
   uint64_t full[kMaxStages], empty[kMaxStages];
-  uint64_t tmem_full[8], tmem_empty[8];
+  uint64_t tmem_full[4], tmem_empty[4];
   uint64_t tk_full[kTickets], tk_empty[kTickets];
   int tk[kTickets];
   uint32_t tmem_base;
@@ -111,7 +111,10 @@ struct Ctl {
 };
 
 constexpr int kCtlBytes = (int)((sizeof(Ctl) + 15) / 16 * 16);
-constexpr int kStagedBytes = 16384;  // accumulators of 8 (at most 16) rows on their way out
+// Accumulators on their way out: two buffers of 64 rows x 32 columns (rows 33 apart: no bank
+// conflicts).
+constexpr int kStagePitch = 33;
+constexpr int kStagedBytes = 2 * 64 * kStagePitch * 4;
 
 // Units of kLinear: at most NB consecutive rows of one group.
 struct RowUnits {
@@ -149,13 +152,12 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
            const __grid_constant__ CUtensorMap map2, const Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  constexpr int kBufs = acc_bufs(NB);
-  constexpr uint32_t kTmemCols = kBufs * 2 * NB;
+  constexpr uint32_t kTmemCols = 512;
   const int ST = p.stages;
   const uint32_t stage_bytes = (uint32_t)p.stage_bytes;
-  // After the ring, at least 16 KB that an MMA of a low box may read past the last stage.
+  // After the ring, at least the 14 KB that an MMA reads past the activations of the last stage.
   Ctl& s = *reinterpret_cast<Ctl*>(smem + ST * stage_bytes);
-  float* const staged = reinterpret_cast<float*>(smem + ST * stage_bytes + kCtlBytes);  // [8][256]
+  float* const staged = reinterpret_cast<float*>(smem + ST * stage_bytes + kCtlBytes);
   uint8_t* plan_mem = smem + ST * stage_bytes + kCtlBytes + kStagedBytes;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &s.abort;
@@ -165,7 +167,7 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
       ptx::mbar_init(ptx::smem_u32(&s.full[i]), 1 + 64);  // weights, and each lane of warps 2-3
       ptx::mbar_init(ptx::smem_u32(&s.empty[i]), 1);
     }
-    for (int i = 0; i < kBufs; ++i) {
+    for (int i = 0; i < 4; ++i) {
       ptx::mbar_init(ptx::smem_u32(&s.tmem_full[i]), 1);
       ptx::mbar_init(ptx::smem_u32(&s.tmem_empty[i]), 4);
     }
@@ -245,30 +247,28 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
   // 64-deep blocks per tile and chunks of each phase.
   const int KB0 = ((MODE == kMoe ? p.d : p.K) + BK - 1) / BK, KB1 = (p.H + BK - 1) / BK;
   const int G0 = U * p.shape[0].tiles * (MODE == kLinear ? p.parts : 1);
-  const int G1 = MODE == kMoe ? U * p.shape[1].tiles : 0;
+  const int G1 = MODE == kMoe ? U * p.shape[1].tiles * p.parts : 0;
   int* const c_out = p.counters + 1;
   int* const c_done = p.counters + 2;
   // Without a cut, kLinear's blocks depend on nobody: tiles at a fixed stride, no counters.
   const bool tickets = MODE == kMoe || p.parts > 1;
 
-  // Chunk t: unit u (expert e, first row row0, n rows), weight rows [w0, w0 + boxes * box_rows),
-  // blocks [kb0, kb0 + len).
+  // Chunk t: unit u (expert e, first row row0, n rows), weight rows from w0, blocks
+  // [kb0, kb0 + len) of the contraction.
   struct Chunk {
     int phase, u, w0, part, kb0, len, e, row0, n;
   };
   auto decode = [&](int t) {
     Chunk c;
     c.phase = MODE == kMoe && t >= G0;
-    int q = c.phase ? t - G0 : t;
-    c.part = 0;
-    if (MODE == kLinear && p.parts > 1) {
-      c.part = q % p.parts;
-      q /= p.parts;
-    }
+    const int q = c.phase ? t - G0 : t;
     const auto& sh = p.shape[c.phase];
-    c.u = q / sh.tiles;
-    c.w0 = (q - c.u * sh.tiles) * sh.boxes * sh.box_rows;
-    part_range(c.phase ? KB1 : KB0, MODE == kLinear ? p.parts : 1, c.part, c.kb0, c.len);
+    const int parts = MODE == kMoe && !c.phase ? 1 : p.parts;
+    const int tile = q / parts;
+    c.part = q - tile * parts;
+    c.u = tile / sh.tiles;
+    c.w0 = (tile - c.u * sh.tiles) * sh.rows;
+    part_range(c.phase ? KB1 : KB0, parts, c.part, c.kb0, c.len);
     if constexpr (MODE == kMoe) {
       c.e = plan.unit_e[c.u]; c.row0 = plan.unit_pos[c.u]; c.n = plan.unit_n[c.u];
     } else {
@@ -322,24 +322,17 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
         const Chunk c = decode(t);
         const bool gate_up = MODE == kMoe && !c.phase;
         const CUtensorMap* m0 = MODE == kMoe && c.phase ? &map2 : &map0;
-        const CUtensorMap* m1 = gate_up ? &map1 : m0;
         const auto& sh = p.shape[c.phase];
-        const uint32_t box = (sh.box_rows + 7) / 8 * 1024;
-        const int r1 = c.w0 + (gate_up ? 0 : sh.box_rows);
-        const int boxes = gate_up ? 2 : sh.boxes;
         for (int kb = c.kb0, left = c.len; left > 0; left -= sh.blocks) {
           if (!ptx::wait_bounded(ptx::smem_u32(&s.empty[stage]), parity, abort_flag, kWaitNs)) { ok = false; break; }
           const uint32_t bar = ptx::smem_u32(&s.full[stage]);
           uint32_t dst = ptx::smem_u32(smem) + stage * stage_bytes;
           const int nb = min(left, sh.blocks);
-          ptx::mbar_arrive_expect_tx(bar, nb * boxes * sh.box_rows * 128);
+          ptx::mbar_arrive_expect_tx(bar, nb * (gate_up ? 2 : 1) * sh.rows * 128);
           for (int j = 0; j < nb; ++j, ++kb) {
             ptx::tma_load_3d(dst, m0, bar, kb * BK, c.w0, c.e);
-            dst += box;
-            if (boxes == 2) {
-              ptx::tma_load_3d(dst, m1, bar, kb * BK, r1, c.e);
-              dst += box;
-            }
+            if (gate_up) ptx::tma_load_3d(dst + sh.block_bytes / 2, &map1, bar, kb * BK, c.w0, c.e);
+            dst += sh.block_bytes;
           }
           if (++stage == ST) { stage = 0; parity ^= 1; }
         }
@@ -348,49 +341,33 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
     __syncwarp();
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA
-    int stage = 0;
-    uint32_t parity = 0;
+    const uint32_t ring = ptx::smem_u32(smem);
+    int stage = 0, buf = 0;
+    uint32_t parity = 0, buf_parity = 1;
     bool ok = true;
     Chunk c;
     for (int it = 0; ok && ticket(it, c); ++it) {
-      const uint32_t idesc = ptx::make_idesc_f16(FMT, 0, 0, 128, (c.n + 15) / 16 * 16);
-      const int buf = it % kBufs;
-      if (!warp_wait(s.tmem_empty[buf], ((it / kBufs) & 1) ^ 1)) break;
-      ptx::tc_fence_after();
-      const uint32_t d0 = tmem_base + buf * 2 * NB;
       const auto& sh = p.shape[c.phase];
-      const uint32_t box = (sh.box_rows + 7) / 8 * 1024;
-      const int boxes = MODE == kMoe && !c.phase ? 2 : sh.boxes;
+      const uint32_t idesc = ptx::make_idesc_f16(FMT, 0, 0, 128, sh.n);
+      if (!warp_wait(s.tmem_empty[buf], buf_parity)) break;
+      ptx::tc_fence_after();
+      const uint32_t d = tmem_base + buf * p.acc_cols;
       for (int left = c.len; left > 0; left -= sh.blocks) {
         if (!warp_wait(s.full[stage], parity)) { ok = false; break; }
         ptx::tc_fence_after();
         if (lane == 0) {
           ptx::fence_proxy_async_smem();  // the copies of warps 2-3 before the MMAs' reads
-          const uint32_t sa = ptx::smem_u32(smem) + stage * stage_bytes;
-          uint32_t da = ptx::sw128_desc_lo(sa), db = ptx::sw128_desc_lo(sa + sh.blocks * boxes * box);
+          const uint32_t sw = ring + stage * stage_bytes;
+          uint32_t dw = ptx::sw128_desc_lo(sw), da = ptx::sw128_desc_lo(sw + sh.blocks * sh.block_bytes);
           const int nb = min(left, sh.blocks);
-          const uint32_t box16 = box >> 4;
           uint32_t more = left != c.len;
-          if (boxes == 2) {
-            for (int j = 0; j < nb; ++j) {
+          for (int j = 0; j < nb; ++j) {
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk) {
-                ptx::mma_f16_sw128(d0, da + 2 * kk, db + 2 * kk, idesc, kk ? 1u : more);
-                ptx::mma_f16_sw128(d0 + NB, da + box16 + 2 * kk, db + 2 * kk, idesc, kk ? 1u : more);
-              }
-              da += 2 * box16;
-              db += NB * 8;
-              more = 1;
-            }
-          } else {
-            for (int j = 0; j < nb; ++j) {
-#pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
-                ptx::mma_f16_sw128(d0, da + 2 * kk, db + 2 * kk, idesc, kk ? 1u : more);
-              da += box16;
-              db += NB * 8;
-              more = 1;
-            }
+            for (int kk = 0; kk < 4; ++kk)
+              ptx::mma_f16_sw128(d, da + 2 * kk, dw + 2 * kk, idesc, kk ? 1u : more);
+            dw += sh.block_bytes >> 4;
+            da += NB * 8;
+            more = 1;
           }
           ptx::mma_commit<1>(ptx::smem_u32(&s.empty[stage]));
         }
@@ -400,6 +377,7 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
       if (!ok) break;
       if (lane == 0) ptx::mma_commit<1>(ptx::smem_u32(&s.tmem_full[buf]));
       __syncwarp();
+      if (++buf == p.bufs) { buf = 0; buf_parity ^= 1; }
     }
   } else if (warp < 4) {
     // ---------------------------------------------------------- activations
@@ -433,10 +411,10 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
         }
       }
       const auto& sh = p.shape[c.phase];
-      const uint32_t a_bytes = sh.blocks * (MODE == kMoe && !c.phase ? 2 : sh.boxes) * ((sh.box_rows + 7) / 8 * 1024);
+      const uint32_t w_bytes = sh.blocks * sh.block_bytes;
       for (int kb = c.kb0, left = c.len; left > 0; left -= sh.blocks) {
         if (!warp_wait(s.empty[stage], parity)) { ok = false; break; }
-        uint32_t dst = ptx::smem_u32(smem) + stage * stage_bytes + a_bytes;
+        uint32_t dst = ptx::smem_u32(smem) + stage * stage_bytes + w_bytes;
         const int nb = min(left, sh.blocks);
         for (int j = 0; j < nb; ++j, ++kb, dst += NB * 128) {
           const bool in = kb * BK + c16 * 8 < cols;  // cols is a multiple of 8
@@ -455,8 +433,10 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
     ptx::cp_async_wait_all();
   } else {
     // ---------------------------------------------------------- epilogue
-    const int row = (warp - 4) * 32 + lane;  // accumulator lane
-    const bool lead = row == 0;
+    const int quarter = warp - 4, tid = threadIdx.x - 128;
+    const bool lead = tid == 0;
+    int buf = 0, half = 0;
+    uint32_t parity = 0;
     Chunk c;
     int held_unit = -1;  // kMoe: the unit of an h tile that is stored but not published
     int outputs = 0;     // chunks of the outputs that this block has stored
@@ -468,8 +448,6 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
     };
     // The four warps meet at barriers, so each wait's outcome is agreed on by all of them.
     for (int it = 0;; ++it) {
-      const int buf = it % kBufs;
-      const uint32_t parity = (it / kBufs) & 1;
       if (MODE == kMoe && held_unit >= 0) {
         const bool ready = ptx::mbar_try_wait(ptx::smem_u32(&s.tk_full[it % kTickets]), (it / kTickets) & 1) &&
                            ptx::mbar_try_wait(ptx::smem_u32(&s.tmem_full[buf]), parity);
@@ -480,45 +458,57 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
       if (!ptx::named_barrier_all(1, 128, warp_wait(s.tmem_full[buf], parity))) break;
       if (MODE == kMoe && held_unit >= 0) publish();
       ptx::tc_fence_after();
-      const uint32_t tb = tmem_base + ((uint32_t)((warp - 4) * 32) << 16) + buf * 2 * NB;
+      const uint32_t tb = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * p.acc_cols;
       const auto& sh = p.shape[c.phase];
+      const bool gate_up = MODE == kMoe && !c.phase;
       const int limit = MODE == kLinear ? p.N : c.phase ? p.d : p.H;
-      // This thread's columns of the output: one per accumulator.
-      const int col0 = row < sh.box_rows ? c.w0 + row : limit;
-      const int col1 = row < sh.box_rows && sh.boxes == 2 ? c.w0 + sh.box_rows + row : limit;
+      // Columns of the tile's output, `wide` at a time: with 32, or 16 gate and 16 up.
+      const int wide = gate_up ? 16 : 32, cols = min(sh.rows, limit - c.w0);
+      const int up = sh.block_bytes / 256;  // accumulator column of the first up row
+      const int tc = tid & (wide - 1), tr = tid / wide, rows_step = 128 / wide;
 #pragma unroll 1
-      for (int j0 = 0; j0 < c.n; j0 += 8) {
-        uint32_t v0[8], v1[8];
-        ptx::tmem_ld_32x32b_x8(tb + j0, v0);
-        ptx::tmem_ld_32x32b_x8(tb + NB + j0, v1);
-        ptx::tmem_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          staged[j * 256 + row] = __uint_as_float(v0[j]);
-          staged[j * 256 + 128 + row] = __uint_as_float(v1[j]);
-        }
-        // each thread reads back what it wrote
-        const int m = min(8, c.n - j0);
-#pragma unroll 1
-        for (int j = 0; j < m; ++j) {
-          const float a = staged[j * 256 + row], b = staged[j * 256 + 128 + row];
-          const int64_t r = c.row0 + j0 + j;
-          if (MODE == kMoe && !c.phase) {
-            if (col0 < limit) static_cast<T*>(p.h)[r * p.H + col0] = from_f32<T>(a * sigmoid_f32(a) * b);
-          } else if (MODE == kMoe || p.parts > 1) {
-            float* dst = p.part + (MODE == kMoe ? r : (int64_t)c.part * p.m + r) * limit;
-            if (col0 < limit) dst[col0] = a;
-            if (col1 < limit) dst[col1] = b;
+      for (int c0 = 0; c0 < cols; c0 += wide, half ^= 1) {
+        float* st = staged + half * 64 * kStagePitch;
+        if (quarter * 32 < c.n) {
+          uint32_t v[32];
+          if (gate_up) {
+            ptx::tmem_ld_32x32b_x16(tb + c0, v);
+            ptx::tmem_ld_32x32b_x16(tb + up + c0, v + 16);
           } else {
+            ptx::tmem_ld_32x32b_x32(tb + c0, v);
+          }
+          ptx::tmem_wait_ld();
+          if (quarter * 32 + lane < c.n) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              st[(quarter * 32 + lane) * kStagePitch + j] = __uint_as_float(v[j]);
+          }
+        }
+        // One barrier per turn: this buffer is written again two turns later, after everybody has
+        // passed the next turn's barrier.
+        ptx::named_barrier(1, 128);
+        const int col = c0 + tc;
+        if (col < cols) {
 #pragma unroll 1
-            for (int i = 0; i < 2; ++i) linear_out<T>(p, c.e, r, i ? col1 : col0, i ? b : a);
+          for (int j = tr; j < c.n; j += rows_step) {
+            const float a = st[j * kStagePitch + tc];
+            const int64_t r = c.row0 + j;
+            if (gate_up) {
+              static_cast<T*>(p.h)[r * p.H + c.w0 + col] =
+                  from_f32<T>(a * sigmoid_f32(a) * st[j * kStagePitch + 16 + tc]);
+            } else if (tickets) {
+              p.part[(c.part * (int64_t)(MODE == kMoe ? S : p.m) + r) * limit + c.w0 + col] = a;
+            } else {
+              linear_out<T>(p, c.e, r, c.w0 + col, a);
+            }
           }
         }
       }
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&s.tmem_empty[buf]));
-      if (MODE == kMoe && !c.phase) held_unit = c.u;
+      if (++buf == p.bufs) { buf = 0; parity ^= 1; }
+      if (gate_up) held_unit = c.u;
       else ++outputs;
     }
     // Abandoned work is not published (the wait that gave up has set the abort flag).
@@ -547,7 +537,7 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
     __syncthreads();
     const int width = MODE == kMoe ? p.d : p.N;  // a multiple of 8
     const int out_rows = MODE == kMoe ? p.r.num_tokens : (int)p.m;
-    const int terms = MODE == kMoe ? p.r.K : p.parts;
+    const int terms = MODE == kMoe ? p.r.K * p.parts : p.parts;
     const int split = terms <= 4 ? 1 : terms <= 8 ? 2 : terms <= 16 ? 4 : 8;
     const int sub = lane & (split - 1);
     const int quads = width / 4;
@@ -565,10 +555,10 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
         float w = 1.f;
         int64_t at;
         if constexpr (MODE == kMoe) {
-          const int sl = r * terms + k, pos = plan.pos[sl];
+          const int slot = k / p.parts, sl = r * p.r.K + slot, pos = plan.pos[sl];
           if (pos < 0) continue;
           w = plan.w[sl];
-          at = pos;
+          at = (int64_t)(k - slot * p.parts) * S + pos;
         } else {
           at = (int64_t)k * p.m + r;
         }

@@ -97,8 +97,8 @@ static int linear_tiles(const LinearArgs& a) {
 
 // The few-row kernel's split, counters and partials.
 struct FewLinear {
-  int nb, max_units, parts, grid;
-  fewtc::Params::Shape shape;
+  int nb, max_units, grid;
+  FewSplit split;
   size_t part, total;
 };
 static FewLinear few_linear_plan(int64_t m, int64_t n, int64_t k, int E, bool dense) {
@@ -108,22 +108,12 @@ static FewLinear few_linear_plan(int64_t m, int64_t n, int64_t k, int E, bool de
   // groups that are likely to have a row, when the rows pick groups at random
   const double live = E <= 1 ? 1.0 : E * (1.0 - pow(1.0 - 1.0 / E, (double)m));
   const double units = dense ? (double)((m + f.nb - 1) / f.nb) : std::max(live, (double)m / f.nb);
-  const int64_t KB = (k + fewtc::BK - 1) / fewtc::BK;
-  // Every tile reads its unit's rows: cut the contraction rather than make tiles lower than
-  // twice the rows of a unit (16 rows and fewer cost little).
-  f.parts = 1;
-  const double rows = std::min<double>(f.nb, dense ? (double)m : (double)m / live);
-  if (rows > 16) {
-    const double height = units * n / num_sms(current_device());
-    f.parts = (int)std::min<int64_t>(std::max<int64_t>(1, (int64_t)(2 * rows / height)), std::max<int64_t>(1, KB / 4));
-    const int64_t len = (KB + f.parts - 1) / f.parts;  // equal chunks, none empty
-    f.parts = (int)((KB + len - 1) / len);
-  }
-  f.shape = few_shape(units * f.parts, n, false, f.nb);
+  f.split = few_split(units, n, (k + fewtc::BK - 1) / fewtc::BK, std::min<double>(f.nb, (double)m / units),
+                      false, true);
   f.part = 256;
-  f.total = f.part + (f.parts > 1 ? (size_t)f.parts * m * n * 4 : 0);
+  f.total = f.part + (f.split.parts > 1 ? (size_t)f.split.parts * m * n * 4 : 0);
   f.grid = num_sms(current_device());
-  if (dense) f.grid = (int)std::min<int64_t>(f.grid, (int64_t)units * f.shape.tiles * f.parts);
+  if (dense) f.grid = (int)std::min<int64_t>(f.grid, (int64_t)units * f.split.shape.tiles * f.split.parts);
   return f;
 }
 
@@ -135,7 +125,7 @@ static int few_linear(const LinearArgs& a, void* workspace) {
   const FewLinear f = few_linear_plan(a.m, a.n, a.k, a.E, a.offsets == nullptr);
   CUtensorMap map;
   int rc;
-  if ((rc = few_weight_map(&map, a.B, a.dtype, a.k, a.n, a.E, f.shape.box_rows))) return rc;
+  if ((rc = few_weight_map(&map, a.B, a.dtype, a.k, a.n, a.E, f.split.shape.rows))) return rc;
   uint8_t* ws = (uint8_t*)workspace;
   fewtc::Params p = {};
   p.offsets = a.offsets;
@@ -152,12 +142,12 @@ static int few_linear(const LinearArgs& a, void* workspace) {
   p.y = a.out;
   p.counters = (int*)ws;
   p.part = (float*)(ws + f.part);
-  p.parts = f.parts;
+  p.parts = f.split.parts;
   p.max_units = f.max_units;
-  p.shape[0] = f.shape;
+  p.shape[0] = f.split.shape;
   const int table = fewtc::row_units_bytes(f.max_units);
   if ((rc = few_ring(p, 1, f.nb, table))) return rc;
-  if (f.parts > 1 && (rc = zero_counters(p.counters, 2, a.stream))) return rc;
+  if (f.split.parts > 1 && (rc = zero_counters(p.counters, 2, a.stream))) return rc;
   const CUtensorMap maps[3] = {map, map, map};
   if (a.dtype == MOE_BF16)
     return few_kernel_nb<fewtc::kLinear, 1, __nv_bfloat16>(f.nb, maps, p, (unsigned)f.grid, table, a.stream);

@@ -37,8 +37,8 @@ static int few_nb(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 // Tile height and cut of a phase.  `units` times `rows` weight rows (of each of gate and up) with
 // KB blocks of contraction, `n` rows of activations per unit.  Counted in SM cycles: a
 // 64-deep block of a tile takes the larger of its weights at an SM's share of HBM (26 bytes per
-// cycle), weights and activations at the rate an SM reads L2 (50), and 4 MMAs (90 each); a chunk
-// costs about 1000 more, and adding parts up at the end 6000 and a pass over them.  All SMs are
+// cycle), weights and activations at the rate an SM reads L2 (50), and its MMAs (75 each, and
+// 250 for every stage of about 32 KB); a chunk costs about 1000 more, and adding parts up at the end 6000 and a pass over them.  All SMs are
 // taken to run equally long, waves x chunk; heights that fill 1 to 4 waves are compared.
 struct FewSplit {
   fewtc::Params::Shape shape;
@@ -46,7 +46,7 @@ struct FewSplit {
 };
 static FewSplit few_split(double units, int64_t rows, int64_t KB, double n, bool gate_up, bool may_cut) {
   const double sms = num_sms(current_device());
-  const int64_t most = std::min<int64_t>(gate_up ? 128 : 256, (rows + 7) / 8 * 8);
+  const int64_t most = std::min<int64_t>(gate_up ? 128 : 256, rows);
   double best = 1e30;
   FewSplit f = {};
   for (const int64_t parts : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32}) {
@@ -56,11 +56,12 @@ static FewSplit few_split(double units, int64_t rows, int64_t KB, double n, bool
     if (parts > 1 && len < 4) break;
     for (int w = 1; w <= 5; ++w) {
       int64_t height = (int64_t)(units * parts * rows / (sms * w)) + 1;
-      height = std::min(most, std::max<int64_t>(16, (height + 7) / 8 * 8));
+      height = std::min(most, std::max<int64_t>(16, height));
       if (w == 5) height = most;
       const int64_t tiles = (rows + height - 1) / height;
       const double weights = (gate_up ? 256.0 : 128.0) * height;
-      const double block = std::max({weights / 26, (weights + n * 128) / 50, 360.0});
+      const int m_tiles = gate_up ? (height > 64 ? 2 : 1) : (height > 128 ? 2 : 1);
+      const double block = std::max({weights / 26, (weights + n * 128) / 50, 300.0 * m_tiles + std::min(250.0, weights / 128)});
       double cost = ceil(units * tiles * parts / sms - 1e-6) * (len * block + 1000);
       if (parts > 1) cost += 6000 + parts * units * n * rows * 8 / (sms * 30);
       if (cost < best) {
@@ -71,24 +72,23 @@ static FewSplit few_split(double units, int64_t rows, int64_t KB, double n, bool
       }
     }
   }
-  f.shape.block_bytes = (gate_up ? 2 : 1) * f.shape.rows * 128;  // heights are multiples of 8
-  f.shape.n = (f.shape.block_bytes / 128 + 15) / 16 * 16;
+  const int h = (f.shape.rows + 7) / 8 * 8;  // boxes start at multiples of 1 KB
+  f.shape.m_tiles = h > (gate_up ? 64 : 128) ? 2 : 1;
+  f.shape.second = gate_up ? std::max(64, h) * 128 : h > 128 ? 16384 : 0;
+  f.shape.block_bytes = gate_up ? f.shape.second + h * 128 : h * 128;
   return f;
 }
 
 // Ring geometry: as many 64-deep blocks per stage as about 36 KB hold, then as many stages as
-// shared memory holds; and the accumulators.
+// shared memory holds.
 static int few_ring(fewtc::Params& p, int phases, int nb, int table_bytes) {
-  int bytes = 0, cols = 16;
+  int bytes = 0;
   for (int i = 0; i < phases; ++i) {
     auto& s = p.shape[i];
     const int block = s.block_bytes + nb * 128;
     s.blocks = std::max(1, std::min(fewtc::kMaxBlocksPerStage, 36864 / block));
     bytes = std::max(bytes, s.blocks * block);
-    cols = std::max(cols, (s.n + 31) / 32 * 32);
   }
-  p.acc_cols = cols;
-  p.bufs = std::min(4, 512 / cols);
   p.stage_bytes = bytes;
   const size_t fixed = 1024 + fewtc::kCtlBytes + fewtc::kStagedBytes + (size_t)table_bytes;
   MOE_REQUIRE(fixed < kMaxSmem, "few rows: routing tables too large");

@@ -3,16 +3,17 @@
 //
 // With n rows (1 to 64) per weight matrix the product does 2 n flops per 2-byte weight, far
 // below the ridge: the kernel is a stream over the weights and everything else hides behind it.
-// The weights are the MMA's B operand (N = the tile's weight rows, up to 256) and the activations
-// its A operand (M = 128 rows, of which n hold data; the others compute on stale shared memory
-// and are not stored).  A tcgen05.mma takes about 90 cycles to issue however small it is
-// (measured the same for M = 64 and 128, N = 16 to 128), so an instruction should cover many
-// weights: 256 rows of 16 elements are 8 KB, 64 bytes per cycle against the 26 that an SM's share
-// of HBM delivers.  As the A operand (128 rows) the same weights need twice the instructions,
-// which bounded tiles of 75 rows at 4.2 TB/s.
+// The weights are the MMA's A operand (M = 128 weight rows) and the activations its B operand
+// (N = n rounded up to 16).  A tcgen05.mma takes about 80 cycles here however small it is (the
+// same measured for M = 64 and 128, N = 16 to 112), 51 bytes of weights per cycle when its 128
+// rows are all in use, against the 26 that an SM's share of HBM delivers: M tiles should be full.
+// (With the roles swapped, 256 weight rows as N, an instruction covers twice the weights but
+// multiplies them with 128 rows, nearly all of them padding: the power that takes made 32 tokens
+// at d = 7168 5 to 20 % slower.)
 //
 //   kMoe     phase 0: a tile is up to 128 columns of h: those gate rows and the same up rows of
-//            one unit (an expert's rows of activations, at most NB); its epilogue forms
+//            one unit (an expert's rows of activations, at most NB), in one M tile (up to 64
+//            columns: gate in its first half, up in its second) or two.  Its epilogue forms
 //            h = silu(gate) * up in fp32 and rounds it once to 16 bits (as an MMA operand it
 //            has to be).
 //            phase 1: a tile is up to 256 rows of Wd times the unit's h.  Its fp32 results are
@@ -21,7 +22,9 @@
 //
 // Work split.  The host picks each phase's tile height and the number of chunks that a tile's
 // contraction is cut into (`parts`) from the sizes alone, so that the chunks fill whole waves of
-// the SMs (results depend on neither routing nor timing).  Phase 0 is never cut: adding up
+// the SMs (results depend on neither routing nor timing).  Each chunk starts its contraction at
+// another block, so that SMs that start together do not all read the same columns of rows that
+// lie a power of two apart (1 token, d = 4096: 120 -> 112 us).  Phase 0 is never cut: adding up
 // parts of h before phase 1 costs a fence, an atomic and a second pass per cut, and while the
 // weights saturate HBM each of these takes microseconds (6 and 5 us measured for a block's first
 // ones).  Parts of the outputs are fp32 and cost little: all are added at the end, in order.
@@ -42,8 +45,7 @@
 //               token, any h row), which arrive on the stage's barrier when they land: these
 //               warps run ahead by the whole ring, as the weights do (handing stages over 3
 //               behind held the stream to 3.6 TB/s).
-//   warps 4-7   epilogue: accumulators (a lane per row of activations) through shared memory, so
-//               that stores run along the output's columns.
+//   warps 4-7   epilogue, one accumulator lane (weight row) per thread.
 //
 // Every wait is bounded; one that gives up sets the abort flag and device error 1.
 #pragma once
@@ -85,11 +87,11 @@ struct Params {
     int rows;        // weight rows of a tile = of its TMA box (a gate/up tile: of each of its two)
     int tiles;       // tiles of a unit
     int blocks;      // 64-deep blocks of a stage
-    int block_bytes; // weights of a block (heights are multiples of 8 rows)
-    int n;           // N of the MMA
+    int m_tiles;     // M tiles of a tile: 1 or 2
+    int second;      // bytes from a block's first box to its second box or M tile (0: none)
+    int block_bytes; // weights of a block
   } shape[2];
   int stage_bytes, stages;
-  int acc_cols, bufs;  // TMEM columns of an accumulator, and their number (at most 4)
   int parts;         // chunks that a tile's contraction is cut into (kMoe: in phase 1)
   float* part;       // kMoe: [parts, S, d] results of phase 1; kLinear: [parts, m, N] (parts > 1)
   int* counters;     // zeroed before the launch (kLinear: parts > 1): ticket; finished chunks of
@@ -111,10 +113,8 @@ struct Ctl {
 };
 
 constexpr int kCtlBytes = (int)((sizeof(Ctl) + 15) / 16 * 16);
-// Accumulators on their way out: two buffers of 64 rows x 32 columns (rows 33 apart: no bank
-// conflicts).
-constexpr int kStagePitch = 33;
-constexpr int kStagedBytes = 2 * 64 * kStagePitch * 4;
+// Accumulators on their way out: two buffers of 8 rows of activations x 256 weight rows.
+constexpr int kStagedBytes = 2 * 8 * 256 * 4;
 
 // Units of kLinear: at most NB consecutive rows of one group.
 struct RowUnits {
@@ -146,20 +146,25 @@ __device__ __forceinline__ void linear_out(const Params& p, int e, int64_t row, 
   static_cast<T*>(p.y)[at] = from_f32<T>(y);
 }
 
+// A value that is the same in every lane, in a form that tells the compiler so.
+template <typename V>
+__device__ __forceinline__ V warp_uniform(V v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 template <int MODE, int FMT, typename T, int NB>
 __global__ void __launch_bounds__(kThreads, 1)
 few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUtensorMap map1,
            const __grid_constant__ CUtensorMap map2, const Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  constexpr uint32_t kTmemCols = 512;
+  constexpr int kBufs = 4;  // accumulators: 2 M tiles of NB columns each
+  constexpr uint32_t kTmemCols = kBufs * 2 * NB;
   const int ST = p.stages;
   const uint32_t stage_bytes = (uint32_t)p.stage_bytes;
-  // After the ring, at least the 14 KB that an MMA reads past the activations of the last stage.
+  // After the ring, at least the 16 KB that an MMA of a low tile may read past the last stage.
   Ctl& s = *reinterpret_cast<Ctl*>(smem + ST * stage_bytes);
   float* const staged = reinterpret_cast<float*>(smem + ST * stage_bytes + kCtlBytes);
   uint8_t* plan_mem = smem + ST * stage_bytes + kCtlBytes + kStagedBytes;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_uniform((int)(threadIdx.x >> 5)), lane = threadIdx.x & 31;
   volatile int* abort_flag = &s.abort;
 
   if (threadIdx.x == 0) {
@@ -256,7 +261,7 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
   // Chunk t: unit u (expert e, first row row0, n rows), weight rows from w0, blocks
   // [kb0, kb0 + len) of the contraction.
   struct Chunk {
-    int phase, u, w0, part, kb0, len, e, row0, n;
+    int phase, u, w0, part, kb0, len, e, row0, n, turn;
   };
   auto decode = [&](int t) {
     Chunk c;
@@ -269,6 +274,7 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
     c.u = tile / sh.tiles;
     c.w0 = (tile - c.u * sh.tiles) * sh.rows;
     part_range(c.phase ? KB1 : KB0, parts, c.part, c.kb0, c.len);
+    c.turn = (int)((unsigned)t * 37u % (unsigned)c.len);
     if constexpr (MODE == kMoe) {
       c.e = plan.unit_e[c.u]; c.row0 = plan.unit_pos[c.u]; c.n = plan.unit_n[c.u];
     } else {
@@ -323,16 +329,17 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
         const bool gate_up = MODE == kMoe && !c.phase;
         const CUtensorMap* m0 = MODE == kMoe && c.phase ? &map2 : &map0;
         const auto& sh = p.shape[c.phase];
-        for (int kb = c.kb0, left = c.len; left > 0; left -= sh.blocks) {
+        for (int kb = c.kb0 + c.turn, left = c.len; left > 0; left -= sh.blocks) {
           if (!ptx::wait_bounded(ptx::smem_u32(&s.empty[stage]), parity, abort_flag, kWaitNs)) { ok = false; break; }
           const uint32_t bar = ptx::smem_u32(&s.full[stage]);
           uint32_t dst = ptx::smem_u32(smem) + stage * stage_bytes;
           const int nb = min(left, sh.blocks);
           ptx::mbar_arrive_expect_tx(bar, nb * (gate_up ? 2 : 1) * sh.rows * 128);
-          for (int j = 0; j < nb; ++j, ++kb) {
+          for (int j = 0; j < nb; ++j) {
             ptx::tma_load_3d(dst, m0, bar, kb * BK, c.w0, c.e);
-            if (gate_up) ptx::tma_load_3d(dst + sh.block_bytes / 2, &map1, bar, kb * BK, c.w0, c.e);
+            if (gate_up) ptx::tma_load_3d(dst + sh.second, &map1, bar, kb * BK, c.w0, c.e);
             dst += sh.block_bytes;
+            if (++kb == c.kb0 + c.len) kb = c.kb0;
           }
           if (++stage == ST) { stage = 0; parity ^= 1; }
         }
@@ -341,43 +348,69 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
     __syncwarp();
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA
-    const uint32_t ring = ptx::smem_u32(smem);
+    // The whole warp runs this code and one lane issues.  tcgen05.mma takes its operands from
+    // uniform registers: every value and branch here goes through warp_uniform(), which lets the
+    // compiler keep them there.
+    const uint32_t issue = lane == 0;
+    const uint32_t ring = warp_uniform(ptx::smem_u32(smem)), tmem = warp_uniform(tmem_base);
+    const int g0 = warp_uniform(G0), g = warp_uniform(G0 + G1);
+    auto wait = [&](uint64_t& bar, uint32_t par) { return warp_uniform((int)warp_wait(bar, par)) != 0; };
     int stage = 0, buf = 0;
     uint32_t parity = 0, buf_parity = 1;
     bool ok = true;
-    Chunk c;
-    for (int it = 0; ok && ticket(it, c); ++it) {
-      const auto& sh = p.shape[c.phase];
-      const uint32_t idesc = ptx::make_idesc_f16(FMT, 0, 0, 128, sh.n);
-      if (!warp_wait(s.tmem_empty[buf], buf_parity)) break;
+    for (int it = 0; ok; ++it) {
+      int t;
+      if (tickets) {
+        const int slot = it % kTickets;
+        if (!wait(s.tk_full[slot], (it / kTickets) & 1)) break;
+        t = warp_uniform(*(volatile int*)&s.tk[slot]);
+        if (issue) ptx::mbar_arrive(ptx::smem_u32(&s.tk_empty[slot]));
+        __syncwarp();
+      } else {
+        t = blockIdx.x + it * gridDim.x;
+      }
+      if (t >= g) break;
+      const bool second = MODE == kMoe && t >= g0;
+      const int parts = MODE == kMoe && !second ? 1 : p.parts;
+      int kb0, len;
+      part_range(second ? KB1 : KB0, parts, (second ? t - g0 : t) % parts, kb0, len);
+      const int blocks = second ? p.shape[1].blocks : p.shape[0].blocks;
+      const uint32_t block_bytes = second ? p.shape[1].block_bytes : p.shape[0].block_bytes;
+      const int m_tiles = second ? p.shape[1].m_tiles : p.shape[0].m_tiles;
+      const uint32_t next = (uint32_t)(second ? p.shape[1].second : p.shape[0].second) >> 4;
+      const int u = ((second ? t - g0 : t) / parts) / (second ? p.shape[1].tiles : p.shape[0].tiles);
+      const int n = warp_uniform(MODE == kMoe ? (int)plan.unit_n[u] : (int)ru.n[u]);
+      const uint32_t idesc = ptx::make_idesc_f16(FMT, 0, 0, 128, (n + 15) / 16 * 16);
+      if (!wait(s.tmem_empty[buf], buf_parity)) break;
       ptx::tc_fence_after();
-      const uint32_t d = tmem_base + buf * p.acc_cols;
-      for (int left = c.len; left > 0; left -= sh.blocks) {
-        if (!warp_wait(s.full[stage], parity)) { ok = false; break; }
+      const uint32_t d = tmem + buf * 2 * NB;
+      uint32_t more = 0;
+      for (int left = len; left > 0; left -= blocks) {
+        if (!wait(s.full[stage], parity)) { ok = false; break; }
         ptx::tc_fence_after();
-        if (lane == 0) {
-          ptx::fence_proxy_async_smem();  // the copies of warps 2-3 before the MMAs' reads
-          const uint32_t sw = ring + stage * stage_bytes;
-          uint32_t dw = ptx::sw128_desc_lo(sw), da = ptx::sw128_desc_lo(sw + sh.blocks * sh.block_bytes);
-          const int nb = min(left, sh.blocks);
-          uint32_t more = left != c.len;
-          for (int j = 0; j < nb; ++j) {
+        ptx::fence_proxy_async_smem();  // the copies of warps 2-3 before the MMAs' reads
+        const uint32_t sw = ring + stage * stage_bytes;
+        uint32_t dw = ptx::sw128_desc_lo(sw), da = ptx::sw128_desc_lo(sw + blocks * block_bytes);
+        const int nb = min(left, blocks);
+        for (int j = 0; j < nb; ++j) {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              ptx::mma_f16_sw128(d, da + 2 * kk, dw + 2 * kk, idesc, kk ? 1u : more);
-            dw += sh.block_bytes >> 4;
-            da += NB * 8;
-            more = 1;
+          for (int kk = 0; kk < 4; ++kk) {
+            ptx::mma_f16_sw128(issue, d, dw + 2 * kk, da + 2 * kk, idesc, kk ? 1u : more);
+            if (m_tiles == 2)
+              ptx::mma_f16_sw128(issue, d + NB, dw + next + 2 * kk, da + 2 * kk, idesc, kk ? 1u : more);
           }
-          ptx::mma_commit<1>(ptx::smem_u32(&s.empty[stage]));
+          dw += block_bytes >> 4;
+          da += NB * 8;
+          more = 1;
         }
+        if (issue) ptx::mma_commit<1>(ptx::smem_u32(&s.empty[stage]));
         __syncwarp();
         if (++stage == ST) { stage = 0; parity ^= 1; }
       }
       if (!ok) break;
-      if (lane == 0) ptx::mma_commit<1>(ptx::smem_u32(&s.tmem_full[buf]));
+      if (issue) ptx::mma_commit<1>(ptx::smem_u32(&s.tmem_full[buf]));
       __syncwarp();
-      if (++buf == p.bufs) { buf = 0; buf_parity ^= 1; }
+      if (++buf == kBufs) { buf = 0; buf_parity ^= 1; }
     }
   } else if (warp < 4) {
     // ---------------------------------------------------------- activations
@@ -412,11 +445,11 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
       }
       const auto& sh = p.shape[c.phase];
       const uint32_t w_bytes = sh.blocks * sh.block_bytes;
-      for (int kb = c.kb0, left = c.len; left > 0; left -= sh.blocks) {
+      for (int kb = c.kb0 + c.turn, left = c.len; left > 0; left -= sh.blocks) {
         if (!warp_wait(s.empty[stage], parity)) { ok = false; break; }
         uint32_t dst = ptx::smem_u32(smem) + stage * stage_bytes + w_bytes;
         const int nb = min(left, sh.blocks);
-        for (int j = 0; j < nb; ++j, ++kb, dst += NB * 128) {
+        for (int j = 0; j < nb; ++j, dst += NB * 128) {
           const bool in = kb * BK + c16 * 8 < cols;  // cols is a multiple of 8
 #pragma unroll
           for (int i = 0; i < NB / 8; ++i) {
@@ -425,6 +458,7 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
               ptx::cp_async16(dst + r * 128 + ((c16 ^ (r & 7)) << 4),
                               rows[i] + (in ? kb * BK : -(c16 * 8)), in ? 16u : 0u);
           }
+          if (++kb == c.kb0 + c.len) kb = c.kb0;
         }
         ptx::cp_async_arrive(ptx::smem_u32(&s.full[stage]));
         if (++stage == ST) { stage = 0; parity ^= 1; }
@@ -433,8 +467,8 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
     ptx::cp_async_wait_all();
   } else {
     // ---------------------------------------------------------- epilogue
-    const int quarter = warp - 4, tid = threadIdx.x - 128;
-    const bool lead = tid == 0;
+    const int row = threadIdx.x - 128;  // accumulator lane
+    const bool lead = row == 0;
     int buf = 0, half = 0;
     uint32_t parity = 0;
     Chunk c;
@@ -458,56 +492,53 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
       if (!ptx::named_barrier_all(1, 128, warp_wait(s.tmem_full[buf], parity))) break;
       if (MODE == kMoe && held_unit >= 0) publish();
       ptx::tc_fence_after();
-      const uint32_t tb = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * p.acc_cols;
+      const uint32_t tb = tmem_base + ((uint32_t)((warp - 4) * 32) << 16) + buf * 2 * NB;
       const auto& sh = p.shape[c.phase];
       const bool gate_up = MODE == kMoe && !c.phase;
+      const bool pair = gate_up && sh.m_tiles == 1;  // gate in lanes 0-63, up in lanes 64-127
       const int limit = MODE == kLinear ? p.N : c.phase ? p.d : p.H;
-      // Columns of the tile's output, `wide` at a time: with 32, or 16 gate and 16 up.
-      const int wide = gate_up ? 16 : 32, cols = min(sh.rows, limit - c.w0);
-      const int up = sh.block_bytes / 256;  // accumulator column of the first up row
-      const int tc = tid & (wide - 1), tr = tid / wide, rows_step = 128 / wide;
+      // This thread's columns of the output: one per M tile; of a pair, column row % 64 of every
+      // second row of activations.
+      const int at = pair ? row & 63 : row;
+      const int col0 = at < sh.rows ? c.w0 + at : limit;
+      const int col1 = !gate_up && 128 + at < sh.rows ? c.w0 + 128 + at : limit;
 #pragma unroll 1
-      for (int c0 = 0; c0 < cols; c0 += wide, half ^= 1) {
-        float* st = staged + half * 64 * kStagePitch;
-        if (quarter * 32 < c.n) {
-          uint32_t v[32];
-          if (gate_up) {
-            ptx::tmem_ld_32x32b_x16(tb + c0, v);
-            ptx::tmem_ld_32x32b_x16(tb + up + c0, v + 16);
-          } else {
-            ptx::tmem_ld_32x32b_x32(tb + c0, v);
-          }
-          ptx::tmem_wait_ld();
-          if (quarter * 32 + lane < c.n) {
+      for (int j0 = 0; j0 < c.n; j0 += 8, half ^= 1) {
+        float* st = staged + half * 8 * 256;
+        uint32_t v0[8], v1[8];
+        ptx::tmem_ld_32x32b_x8(tb + j0, v0);
+        ptx::tmem_ld_32x32b_x8(tb + NB + j0, v1);
+        ptx::tmem_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              st[(quarter * 32 + lane) * kStagePitch + j] = __uint_as_float(v[j]);
-          }
+        for (int j = 0; j < 8; ++j) {
+          st[j * 256 + row] = __uint_as_float(v0[j]);
+          st[j * 256 + 128 + row] = __uint_as_float(v1[j]);
         }
-        // One barrier per turn: this buffer is written again two turns later, after everybody has
-        // passed the next turn's barrier.
-        ptx::named_barrier(1, 128);
-        const int col = c0 + tc;
-        if (col < cols) {
+        const int m = min(8, c.n - j0);
+        // A pair's halves meet here (this buffer is written again two turns later, after the next
+        // turn's barrier); otherwise each thread reads back what it wrote.
+        if (pair) ptx::named_barrier(1, 128);
+        const int up = pair ? 64 : 128;
 #pragma unroll 1
-          for (int j = tr; j < c.n; j += rows_step) {
-            const float a = st[j * kStagePitch + tc];
-            const int64_t r = c.row0 + j;
-            if (gate_up) {
-              static_cast<T*>(p.h)[r * p.H + c.w0 + col] =
-                  from_f32<T>(a * sigmoid_f32(a) * st[j * kStagePitch + 16 + tc]);
-            } else if (tickets) {
-              p.part[(c.part * (int64_t)(MODE == kMoe ? S : p.m) + r) * limit + c.w0 + col] = a;
-            } else {
-              linear_out<T>(p, c.e, r, c.w0 + col, a);
-            }
+        for (int j = pair ? row >> 6 : 0; j < m; j += pair ? 2 : 1) {
+          const float a = st[j * 256 + at], b = st[j * 256 + up + at];
+          const int64_t r = c.row0 + j0 + j;
+          if (gate_up) {
+            if (col0 < limit) static_cast<T*>(p.h)[r * p.H + col0] = from_f32<T>(a * sigmoid_f32(a) * b);
+          } else if (tickets) {
+            float* dst = p.part + (c.part * (int64_t)(MODE == kMoe ? S : p.m) + r) * limit;
+            if (col0 < limit) dst[col0] = a;
+            if (col1 < limit) dst[col1] = b;
+          } else {
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i) linear_out<T>(p, c.e, r, i ? col1 : col0, i ? b : a);
           }
         }
       }
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(ptx::smem_u32(&s.tmem_empty[buf]));
-      if (++buf == p.bufs) { buf = 0; parity ^= 1; }
+      if (++buf == kBufs) { buf = 0; parity ^= 1; }
       if (gate_up) held_unit = c.u;
       else ++outputs;
     }

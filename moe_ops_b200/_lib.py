@@ -151,6 +151,30 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+class _Here:
+    """A context that changes nothing."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(t: torch.Tensor):
+    """torch.cuda.device(t.device), without its cost when that device is current already."""
+    index = t.device.index
+    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+
+
+def raw_stream(t: torch.Tensor) -> int:
+    """stream_of without building a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
 def check(status: int, what: str) -> None:
     if status != 0:
         msg = load().moe_last_error_string().decode(errors="replace")

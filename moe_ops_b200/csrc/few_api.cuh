@@ -34,48 +34,73 @@ static size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 // crowded expert's weights once.
 static int few_nb(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 
-// Tile height and cut of a phase.  `units` times `rows` weight rows (of each of gate and up) with
-// KB blocks of contraction, `n` rows of activations per unit.  Counted in SM cycles: a
-// 64-deep block of a tile takes the larger of its weights at an SM's share of HBM (26 bytes per
-// cycle), weights and activations at the rate an SM reads L2 (50), and its MMAs (75 each, and
-// 250 for every stage of about 32 KB); a chunk costs about 1000 more, and adding parts up at the end 6000 and a pass over them.  All SMs are
-// taken to run equally long, waves x chunk; heights that fill 1 to 4 waves are compared.
 struct FewSplit {
   fewtc::Params::Shape shape;
   int parts;
 };
-static FewSplit few_split(double units, int64_t rows, int64_t KB, double n, bool gate_up, bool may_cut) {
-  const double sms = num_sms(current_device());
-  const int64_t most = std::min<int64_t>(gate_up ? 128 : 256, rows);
-  double best = 1e30;
+static FewSplit few_tiles(int64_t rows, int64_t height, int64_t KB, int64_t parts, bool gate_up) {
   FewSplit f = {};
-  for (const int64_t parts : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32}) {
-    if (parts > 1 && !may_cut) break;
-    const int64_t len = (KB + parts - 1) / parts;
-    if ((KB + len - 1) / len != parts) continue;  // equal chunks, none empty
-    if (parts > 1 && len < 4) break;
-    for (int w = 1; w <= 5; ++w) {
-      int64_t height = (int64_t)(units * parts * rows / (sms * w)) + 1;
-      height = std::min(most, std::max<int64_t>(16, height));
-      if (w == 5) height = most;
-      const int64_t tiles = (rows + height - 1) / height;
-      const double weights = (gate_up ? 256.0 : 128.0) * height;
-      const int m_tiles = gate_up ? (height > 64 ? 2 : 1) : (height > 128 ? 2 : 1);
-      const double block = std::max({weights / 26, (weights + n * 128) / 50, 300.0 * m_tiles + std::min(250.0, weights / 128)});
-      double cost = ceil(units * tiles * parts / sms - 1e-6) * (len * block + 1000);
-      if (parts > 1) cost += 6000 + parts * units * n * rows * 8 / (sms * 30);
-      if (cost < best) {
-        best = cost;
-        f.parts = (int)parts;
-        f.shape.rows = (int)height;
-        f.shape.tiles = (int)tiles;
-      }
-    }
-  }
+  const int64_t len = (KB + parts - 1) / parts;  // equal chunks, none empty
+  f.parts = (int)((KB + len - 1) / len);
+  f.shape.rows = (int)std::min(height, rows);
+  f.shape.tiles = (int)((rows + f.shape.rows - 1) / f.shape.rows);
   const int h = (f.shape.rows + 7) / 8 * 8;  // boxes start at multiples of 1 KB
   f.shape.m_tiles = h > (gate_up ? 64 : 128) ? 2 : 1;
   f.shape.second = gate_up ? std::max(64, h) * 128 : h > 128 ? 16384 : 0;
   f.shape.block_bytes = gate_up ? f.shape.second + h * 128 : h * 128;
+  return f;
+}
+
+// kMoe.  Full M tiles throughout.  Phase 0: 128 columns of h to a tile from 4 waves of tiles on,
+// else 64 (measured, all of a call: 32 tokens d = 7168 E = 256 H = 2048, 17 waves, 2019 us against
+// 2260; 1 token d = 4096 H = 11008, 1.2 waves, 122 against 109).  Phase 1: 256 rows from 2 waves
+// on, else 128 rows, and the contraction cut into chunks of 8 blocks or more: SMs leave phase 0
+// at different times and small chunks even that out (the 1-token call: 4 waves of chunks 106 us,
+// one wave 123 us; 16 tokens: 256 rows cut in 5 961 us, 128 rows uncut 987 us).
+static FewSplit few_split0(double units, int64_t H, int64_t d) {
+  const int64_t KB = (d + fewtc::BK - 1) / fewtc::BK;
+  const double waves = units * ((H + 127) / 128) / num_sms(current_device());
+  return few_tiles(H, waves >= 4 ? 128 : 64, KB, 1, true);
+}
+static FewSplit few_split1(double units, int64_t d, int64_t H) {
+  const int64_t KB = (H + fewtc::BK - 1) / fewtc::BK;
+  const double sms = num_sms(current_device());
+  const bool high = units * ((d + 255) / 256) >= 2 * sms;
+  const int64_t height = high ? 256 : 128;
+  const int64_t parts = (int64_t)((high ? 12 : 4) * sms / (units * ((d + height - 1) / height)));
+  return few_tiles(d, height, KB, std::max<int64_t>(1, std::min(parts, KB / 8)), false);
+}
+
+// kLinear: `units` units of `n` rows, counted in SM cycles.  A 64-deep block of a tile takes the
+// larger of its weights at an SM's share of HBM (26 bytes per cycle), weights and activations at
+// the rate an SM reads L2 (50), and its MMAs (75 each, and up to 250 a stage); a chunk costs
+// about 1000 more, and adding parts up at the end 6000 and a pass over them.  Heights that fill
+// 1 to 4 waves of the SMs are compared, and whole ones.  (37 rows, K = 7168, N = 4096: picks 148
+// chunks of 111 rows and a quarter of K, 26.7 us; 128 rows 30 us, 128 rows and a fifth 37 us.)
+static FewSplit few_split_linear(double units, int64_t rows, int64_t KB, double n) {
+  const double sms = num_sms(current_device());
+  double best = 1e30;
+  FewSplit f = {};
+  for (const int64_t parts : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16}) {
+    const int64_t len = (KB + parts - 1) / parts;
+    if ((KB + len - 1) / len != parts) continue;
+    if (parts > 1 && len < 4) break;
+    for (int w = 1; w <= 5; ++w) {
+      int64_t height = (int64_t)(units * parts * rows / (sms * w)) + 1;
+      if (w == 5) height = 256;
+      height = std::min<int64_t>(256, std::max<int64_t>(16, std::min(height, rows)));
+      const int64_t tiles = (rows + height - 1) / height;
+      const double weights = 128.0 * height;
+      const double block = std::max({weights / 26, (weights + n * 128) / 50,
+                                     300.0 * (height > 128 ? 2 : 1) + std::min(250.0, weights / 128)});
+      double cost = ceil(units * tiles * parts / sms - 1e-6) * (len * block + 1000);
+      if (parts > 1) cost += 6000 + parts * units * n * rows * 8 / (sms * 30);
+      if (cost < best) {
+        best = cost;
+        f = few_tiles(rows, height, KB, parts, false);
+      }
+    }
+  }
   return f;
 }
 
@@ -114,11 +139,10 @@ static FewWorkspace few_workspace(int64_t T, int64_t d, int64_t H, int64_t E, in
     w.total = w.counters;
     return w;
   }
-  // experts that the tokens are expected to touch when each picks K of E, and their rows
+  // experts that the tokens are expected to touch when each picks K of E
   const double touched = K >= E ? (double)E : E * (1.0 - pow(1.0 - (double)K / E, (double)T));
-  const double n = std::min<double>(few_nb(T), S / touched);
-  w.split0 = few_split(touched, H, (d + fewtc::BK - 1) / fewtc::BK, n, true, false);
-  w.split1 = few_split(touched, d, (H + fewtc::BK - 1) / fewtc::BK, n, false, true);
+  w.split0 = few_split0(touched, H, d);
+  w.split1 = few_split1(touched, d, H);
   w.max_units = few::plan_max_units((int)S, (int)E, few_nb(T));
   w.num_counters = 2 + w.max_units;
   w.part = w.counters + align256((size_t)w.num_counters * 4);

@@ -156,8 +156,11 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
            const __grid_constant__ CUtensorMap map2, const Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  constexpr int kBufs = 4;  // accumulators: 2 M tiles of NB columns each
-  constexpr uint32_t kTmemCols = kBufs * 2 * NB;
+  // Accumulator sets: 2 M tiles x 2 accumulators of NB columns, or 4 of one M tile, which the
+  // epilogue adds.  An MMA that adds to the one before it starts later (linear, 1 row, one M tile:
+  // 26.6 us with one accumulator, 24.0 us with four).
+  constexpr int kBufs = NB == 64 ? 2 : 4;
+  constexpr uint32_t kTmemCols = kBufs * 4 * NB;
   const int ST = p.stages;
   const uint32_t stage_bytes = (uint32_t)p.stage_bytes;
   // After the ring, at least the 16 KB that an MMA of a low tile may read past the last stage.
@@ -383,7 +386,7 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
       const uint32_t idesc = ptx::make_idesc_f16(FMT, 0, 0, 128, (n + 15) / 16 * 16);
       if (!wait(s.tmem_empty[buf], buf_parity)) break;
       ptx::tc_fence_after();
-      const uint32_t d = tmem + buf * 2 * NB;
+      const uint32_t d = tmem + buf * 4 * NB;
       uint32_t more = 0;
       for (int left = len; left > 0; left -= blocks) {
         if (!wait(s.full[stage], parity)) { ok = false; break; }
@@ -393,11 +396,17 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
         uint32_t dw = ptx::sw128_desc_lo(sw), da = ptx::sw128_desc_lo(sw + blocks * block_bytes);
         const int nb = min(left, blocks);
         for (int j = 0; j < nb; ++j) {
+          if (m_tiles == 2) {
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            ptx::mma_f16_sw128(issue, d, dw + 2 * kk, da + 2 * kk, idesc, kk ? 1u : more);
-            if (m_tiles == 2)
-              ptx::mma_f16_sw128(issue, d + NB, dw + next + 2 * kk, da + 2 * kk, idesc, kk ? 1u : more);
+            for (int kk = 0; kk < 4; ++kk) {
+              ptx::mma_f16_sw128(issue, d + (kk & 1) * NB, dw + 2 * kk, da + 2 * kk, idesc, kk > 1 ? 1u : more);
+              ptx::mma_f16_sw128(issue, d + (2 + (kk & 1)) * NB, dw + next + 2 * kk, da + 2 * kk, idesc,
+                                 kk > 1 ? 1u : more);
+            }
+          } else {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              ptx::mma_f16_sw128(issue, d + kk * NB, dw + 2 * kk, da + 2 * kk, idesc, more);
           }
           dw += block_bytes >> 4;
           da += NB * 8;
@@ -492,7 +501,7 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
       if (!ptx::named_barrier_all(1, 128, warp_wait(s.tmem_full[buf], parity))) break;
       if (MODE == kMoe && held_unit >= 0) publish();
       ptx::tc_fence_after();
-      const uint32_t tb = tmem_base + ((uint32_t)((warp - 4) * 32) << 16) + buf * 2 * NB;
+      const uint32_t tb = tmem_base + ((uint32_t)((warp - 4) * 32) << 16) + buf * 4 * NB;
       const auto& sh = p.shape[c.phase];
       const bool gate_up = MODE == kMoe && !c.phase;
       const bool pair = gate_up && sh.m_tiles == 1;  // gate in lanes 0-63, up in lanes 64-127
@@ -505,14 +514,16 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
 #pragma unroll 1
       for (int j0 = 0; j0 < c.n; j0 += 8, half ^= 1) {
         float* st = staged + half * 8 * 256;
-        uint32_t v0[8], v1[8];
-        ptx::tmem_ld_32x32b_x8(tb + j0, v0);
-        ptx::tmem_ld_32x32b_x8(tb + NB + j0, v1);
+        uint32_t v[4][8];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ptx::tmem_ld_32x32b_x8(tb + q * NB + j0, v[q]);
         ptx::tmem_wait_ld();
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          st[j * 256 + row] = __uint_as_float(v0[j]);
-          st[j * 256 + 128 + row] = __uint_as_float(v1[j]);
+          const float a = __uint_as_float(v[0][j]) + __uint_as_float(v[1][j]);
+          const float b = __uint_as_float(v[2][j]) + __uint_as_float(v[3][j]);
+          st[j * 256 + row] = sh.m_tiles == 2 ? a : a + b;
+          st[j * 256 + 128 + row] = b;
         }
         const int m = min(8, c.n - j0);
         // A pair's halves meet here (this buffer is written again two turns later, after the next

@@ -108,8 +108,8 @@ static FewLinear few_linear_plan(int64_t m, int64_t n, int64_t k, int E, bool de
   // groups that are likely to have a row, when the rows pick groups at random
   const double live = E <= 1 ? 1.0 : E * (1.0 - pow(1.0 - 1.0 / E, (double)m));
   const double units = dense ? (double)((m + f.nb - 1) / f.nb) : std::max(live, (double)m / f.nb);
-  f.split = few_split(units, n, (k + fewtc::BK - 1) / fewtc::BK, std::min<double>(f.nb, (double)m / units),
-                      false, true);
+  f.split = few_split_linear(units, n, (k + fewtc::BK - 1) / fewtc::BK,
+                             std::min<double>(f.nb, (double)m / units));
   f.part = 256;
   f.total = f.part + (f.split.parts > 1 ? (size_t)f.split.parts * m * n * 4 : 0);
   f.grid = num_sms(current_device());
@@ -121,8 +121,12 @@ static bool few_linear_ok(const LinearArgs& a) {
   return linear_tc_ok(a) && !a.b_mn && a.m <= few_linear_max_rows(a.E);
 }
 
-static int few_linear(const LinearArgs& a, void* workspace) {
+static int few_linear(const LinearArgs& a, void* workspace, size_t workspace_bytes) {
   const FewLinear f = few_linear_plan(a.m, a.n, a.k, a.E, a.offsets == nullptr);
+  if (!workspace || workspace_bytes < f.total)
+    return set_error(MOE_ERR_WORKSPACE, "linear: workspace has %zu bytes, needs %zu",
+                     workspace ? workspace_bytes : (size_t)0, f.total);
+  MOE_REQUIRE(aligned16(workspace), "linear: workspace must be 16-byte aligned");
   CUtensorMap map;
   int rc;
   if ((rc = few_weight_map(&map, a.B, a.dtype, a.k, a.n, a.E, f.split.shape.rows))) return rc;
@@ -199,14 +203,9 @@ int moe_linear_fwd(const void* A, const void* B, const void* bias, const void* r
   if (m_total == 0 || n == 0) return MOE_OK;
   LinearArgs a = {A, B, bias, residual, out, preact, offsets, num_offsets == num_experts + 1,
                   m_total, n, k, num_experts, !trans_b, activation, dtype, (cudaStream_t)stream};
-  const size_t need = moe_linear_workspace_bytes(m_total, n, k, num_experts, trans_b, dtype);
-  if (need && (!workspace || workspace_bytes < need))
-    return set_error(MOE_ERR_WORKSPACE, "linear: workspace has %zu bytes, needs %zu",
-                     workspace ? workspace_bytes : (size_t)0, need);
-  MOE_REQUIRE(!need || aligned16(workspace), "linear: workspace must be 16-byte aligned");
   if (num_experts > 0) {
     if (few_linear_ok(a)) {
-      rc = few_linear(a, workspace);
+      rc = few_linear(a, workspace, workspace_bytes);
     } else if (linear_tc_ok(a)) {
       rc = linear_tiles(a);
     } else {

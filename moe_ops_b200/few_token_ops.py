@@ -18,6 +18,7 @@ part of a call is of the order of the kernel's time.
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -53,6 +54,11 @@ def _no_grad_only(*tensors) -> None:
                            "or use MoELayer / moe_layer_forward")
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(T: int, d: int, H: int, E: int, K: int, code: int) -> int:
+    return _lib.load().moe_few_tokens_workspace_bytes(T, d, H, E, K, code)
+
+
 def _run(x, route, w_gate, w_up, w_down, dims, K: int, given: bool) -> torch.Tensor:
     T, d, E, H = dims
     code = _lib.dtype_code(x.dtype)
@@ -61,12 +67,12 @@ def _run(x, route, w_gate, w_up, w_down, dims, K: int, given: bool) -> torch.Ten
     lib = _lib.load()
     y = torch.empty((T, d), device=x.device, dtype=x.dtype)
     fn = lib.moe_few_experts_fwd if given else lib.moe_few_tokens_fwd
-    with torch.cuda.device(x.device):
-        ws_bytes = lib.moe_few_tokens_workspace_bytes(T, d, H, E, K, code)
+    with _lib.on_device(x):
+        ws_bytes = _workspace_bytes(T, d, H, E, K, code)
         ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8)
         st = fn(x.data_ptr(), _lib.ptr(route[0]), _lib.ptr(route[1]), w_gate.data_ptr(),
                 w_up.data_ptr(), w_down.data_ptr(), code, T, d, H, E, K, y.data_ptr(),
-                ws.data_ptr(), ws_bytes, _lib.stream_of(x))
+                ws.data_ptr(), ws_bytes, _lib.raw_stream(x))
     _lib.check(st, "moe_few_experts" if given else "moe_few_tokens")
     _lib.count_launches(2)
     return y

@@ -23,6 +23,7 @@ the host's part of a call is of the order of the kernel's time.
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -37,16 +38,21 @@ def _check(x, w, bias, residual, out_shape, bias_shape, activation) -> int:
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)} (got {activation!r})")
-    _lib.dtype_code(x.dtype)
-    for name, t, shape in (("weight", w, None), ("bias", bias, bias_shape),
-                           ("residual", residual, out_shape)):
-        if t is None:
-            continue
-        if t.dtype != x.dtype or t.device != x.device:
-            raise ValueError(f"{name} must have the input's dtype and device")
-        if shape is not None and tuple(t.shape) != tuple(shape):
-            raise ValueError(f"{name} must be {list(shape)} (got {list(t.shape)})")
+    dtype, device = x.dtype, x.device
+    _lib.dtype_code(dtype)
+    if w.dtype != dtype or w.device != device:
+        raise ValueError("weight must have the input's dtype and device")
+    if bias is not None and (bias.dtype != dtype or bias.device != device or bias.shape != bias_shape):
+        raise ValueError(f"bias must be {list(bias_shape)} of the input's dtype and device")
+    if residual is not None and (residual.dtype != dtype or residual.device != device
+                                 or residual.shape != out_shape):
+        raise ValueError(f"residual must be {list(out_shape)} of the input's dtype and device")
     return act
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(m: int, n: int, k: int, E: int, trans_b: int, code: int) -> int:
+    return _lib.load().moe_linear_workspace_bytes(m, n, k, E, trans_b, code)
 
 
 def _forward(x, w, bias, residual, offsets, act: int, trans_b: bool, E: int, n: int, want_z: bool):
@@ -56,13 +62,13 @@ def _forward(x, w, bias, residual, offsets, act: int, trans_b: bool, E: int, n: 
     z = torch.empty_like(y) if want_z else None
     lib = _lib.load()
     code = _lib.dtype_code(x.dtype)
-    with torch.cuda.device(x.device):
-        ws_bytes = lib.moe_linear_workspace_bytes(m, n, k, E, int(trans_b), code)
+    with _lib.on_device(x):
+        ws_bytes = _workspace_bytes(m, n, k, E, int(trans_b), code)
         ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8) if ws_bytes else None
         st = lib.moe_linear_fwd(
             x.data_ptr(), w.data_ptr(), _lib.ptr(bias), _lib.ptr(residual), y.data_ptr(), _lib.ptr(z),
             _lib.ptr(offsets), 0 if offsets is None else offsets.numel(), m, n, k, E, int(trans_b),
-            act, code, _lib.ptr(ws), ws_bytes, _lib.stream_of(x))
+            act, code, _lib.ptr(ws), ws_bytes, _lib.raw_stream(x))
     _lib.check(st, "moe_linear_fwd")
     _lib.count_launches(1)
     return y, z
@@ -79,11 +85,11 @@ def _act_bwd(dy, z, offsets, E: int, act: int, want_bias: bool, bias_shape):
     lib = _lib.load()
     ws_bytes = lib.moe_linear_act_bwd_workspace_bytes(m, n, E) if want_bias else 0
     ws = torch.empty(ws_bytes, device=dy.device, dtype=torch.uint8)
-    with torch.cuda.device(dy.device):
+    with _lib.on_device(dy):
         st = lib.moe_linear_act_bwd(
             dy.data_ptr(), _lib.ptr(z), dz.data_ptr() if act else None, _lib.ptr(db),
             _lib.ptr(offsets), 0 if offsets is None else offsets.numel(), m, n, E, act, code,
-            ws.data_ptr() if ws_bytes else None, ws_bytes, _lib.stream_of(dy))
+            ws.data_ptr() if ws_bytes else None, ws_bytes, _lib.raw_stream(dy))
     _lib.check(st, "moe_linear_act_bwd")
     _lib.count_launches(1 + int(want_bias))
     return dz, db
@@ -94,15 +100,15 @@ def _gemm(fn: str, a, b, shape, offsets, m, n, k, E, trans_b):
     if out.numel() == 0 or (n if fn == "moe_gmm_dgrad" else m) == 0:
         return out.zero_()
     lib = _lib.load()
-    with torch.cuda.device(a.device):
+    with _lib.on_device(a):
         st = getattr(lib, fn)(
             a.data_ptr(), b.data_ptr(), out.data_ptr(), _lib.ptr(offsets),
             0 if offsets is None else offsets.numel(), m, n, k, E, int(trans_b),
-            _lib.dtype_code(a.dtype), _lib.stream_of(a))
+            _lib.dtype_code(a.dtype), _lib.raw_stream(a))
         _lib.check(st, fn)
         if fn == "moe_gmm_dgrad" and offsets is not None:
             _lib.check(lib.moe_zero_tail_rows(out.data_ptr(), offsets.data_ptr(), offsets.numel(), m,
-                                              k, _lib.dtype_code(a.dtype), _lib.stream_of(a)),
+                                              k, _lib.dtype_code(a.dtype), _lib.raw_stream(a)),
                        "moe_zero_tail_rows")
     _lib.count_launches(1)
     return out
@@ -159,13 +165,16 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"x [..., K] and weight [N, K] do not match: {list(x.shape)}, {list(weight.shape)}")
     n, k = weight.shape
-    out_shape = x.shape[:-1] + (n,)
+    if x.dim() == 2:
+        x2, out_shape = x, (x.shape[0], n)
+    else:
+        out_shape = x.shape[:-1] + (n,)
+        x2 = x.reshape(out_shape[:-1].numel(), k)
     act = _check(x, weight, bias, residual, out_shape, (n,), activation)
-    x2 = x.reshape(-1, k) if k else x.reshape(out_shape[:-1].numel(), 0)
     r2 = None if residual is None else residual.reshape(x2.shape[0], n).contiguous()
     y = _apply(x2.contiguous(), weight.contiguous(), None if bias is None else bias.contiguous(), r2,
                None, act, True, 1, n)
-    return y.view(out_shape)
+    return y if x.dim() == 2 else y.view(out_shape)
 
 
 def grouped_linear(A: torch.Tensor, B: torch.Tensor, offsets: torch.Tensor,

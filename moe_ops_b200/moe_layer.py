@@ -11,15 +11,20 @@ Same structure as the reference's example layer SingleGpuMoE (tests/test_moe.py:
               projection's dgrad carries the SwiGLU backward in its epilogue)
     out     = unpermute(down, row_id_map, w, T, K)
 
+Optionally a shared expert beside the routed ones, whose second projection adds their output
+in its epilogue (``linear``), and the few-token kernels for decoding (``moe_few_tokens``).
+
 Weights: w_router [E, d], w_gate / w_up [E, H, d], w_down [E, d, H] (trans_b=True layout).
 """
 from __future__ import annotations
 
 import torch
 
+from .few_token_ops import MAX_TOKENS, MAX_TOPK, moe_few_tokens
 from .fused_topk_softmax_ops import fused_topk_softmax
 from .gate_up_ops import grouped_swiglu_mlp
 from .fused_permute_ops import gathered_path_ok, grouped_swiglu_mlp_gathered, permute_index
+from .linear_ops import linear
 from .permute_ops import permute, permute_with_capacity
 from .unpermute_ops import unpermute
 
@@ -56,7 +61,10 @@ class MoELayer(torch.nn.Module):
     """Single-GPU SwiGLU MoE layer (parameters as in the reference's SingleGpuMoE)."""
 
     def __init__(self, d_model: int, num_experts: int, top_k: int, hidden: int,
-                 fp32_routing: bool = False, device=None, dtype=None):
+                 fp32_routing: bool = False, device=None, dtype=None, shared_hidden: int = 0,
+                 shared_activation: str = "silu"):
+        """shared_hidden > 0 adds a shared expert that every token passes through:
+        act(x . w_shared_in^T + b_shared_in) . w_shared_out^T + b_shared_out."""
         super().__init__()
         kw = dict(device=device, dtype=dtype)
         self.num_experts = num_experts
@@ -66,11 +74,22 @@ class MoELayer(torch.nn.Module):
         self.w_gate = torch.nn.Parameter(torch.empty(num_experts, hidden, d_model, **kw))
         self.w_up = torch.nn.Parameter(torch.empty(num_experts, hidden, d_model, **kw))
         self.w_down = torch.nn.Parameter(torch.empty(num_experts, d_model, hidden, **kw))
+        self.shared_activation = shared_activation
+        if shared_hidden > 0:
+            self.w_shared_in = torch.nn.Parameter(torch.empty(shared_hidden, d_model, **kw))
+            self.b_shared_in = torch.nn.Parameter(torch.empty(shared_hidden, **kw))
+            self.w_shared_out = torch.nn.Parameter(torch.empty(d_model, shared_hidden, **kw))
+            self.b_shared_out = torch.nn.Parameter(torch.empty(d_model, **kw))
+        self.shared_hidden = shared_hidden
         self.router_bias = None  # optional fixed per-expert logit bias [E]
         # > 0: expert capacity = ceil(capacity_factor * T * K / E) slots (token dropping)
         self.capacity_factor = 0.0
         # True: the expert GEMMs gather their rows from x (no permuted copy is written)
         self.fused_permute = False
+        # > 0: calls of up to that many tokens (at most 128) without gradients and without
+        # token dropping run moe_few_tokens; its router logits are not rounded to x's dtype, so
+        # experts whose logits are close may rank differently than in the assembled layer
+        self.few_tokens = 0
 
     @torch.no_grad()
     def init_normal(self, std: float = 0.02, generator=None) -> "MoELayer":
@@ -78,7 +97,25 @@ class MoELayer(torch.nn.Module):
             p.normal_(0.0, std, generator=generator)
         return self
 
+    def _use_few_tokens(self, x: torch.Tensor) -> bool:
+        if not 0 < x.shape[0] <= min(self.few_tokens, MAX_TOKENS) or self.capacity_factor > 0:
+            return False
+        if self.top_k > MAX_TOPK:
+            return False
+        return not torch.is_grad_enabled() or not (
+            x.requires_grad or any(p.requires_grad for p in self.parameters()))
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        out = self._routed(x)
+        if self.shared_hidden > 0:
+            h = linear(x, self.w_shared_in, self.b_shared_in, self.shared_activation)
+            out = linear(h, self.w_shared_out, self.b_shared_out, residual=out)
+        return out
+
+    def _routed(self, x: torch.Tensor) -> torch.Tensor:
+        if self._use_few_tokens(x):
+            return moe_few_tokens(x, self.w_router, self.w_gate, self.w_up, self.w_down, self.top_k,
+                                  router_bias=self.router_bias)
         cap = 0
         if self.capacity_factor > 0:
             cap = -(-int(self.capacity_factor * x.shape[0] * self.top_k) // self.num_experts)

@@ -29,25 +29,16 @@ struct LinearEpilogue {
   }
 };
 
-// ------------------------------------------------------------------ backward, elementwise
-// One pass over dout and z: dz written (unless the activation is none: dz is dout) and the
-// column sums of dz taken from its fp32 values before they are rounded.  A block owns
-// kDzRows consecutive rows of one group and kDzCols columns; its column sums go to
-// partial[chunk, n] and dbias_kernel adds the chunks of a group in order, so the result does
-// not depend on the order blocks run in.  HBM-bound: 2 reads + 1 write of m * n elements.
-constexpr int kDzRows = 128;
-constexpr int kDzThreads = 256;
-
-// Chunk c of the concatenation of every group's ceil(rows / kDzRows) chunks: its group, rows
-// and, in `first`, the group's first chunk.  `prefix` [E + 1] lives in shared memory.
-__device__ __forceinline__ void dz_prefix(int* prefix, const int32_t* offsets, int plus_one, int E,
-                                          int64_t m) {
+// Row chunks: every group's rows in pieces of `size`, one after the other.  prefix [E + 1] (shared
+// memory) receives the first chunk of each group; ends with a __syncthreads().
+__device__ __forceinline__ void row_chunks(int* prefix, const int32_t* offsets, int plus_one, int E,
+                                           int64_t m, int size) {
   if (threadIdx.x < 32) {
     int run = 0;
     for (int e0 = 0; e0 < E; e0 += 32) {
       const int e = e0 + (int)threadIdx.x;
       int c = 0;
-      if (e < E) c = (int)((simt::group_range(offsets, plus_one, e, m).rows + kDzRows - 1) / kDzRows);
+      if (e < E) c = (int)((simt::group_range(offsets, plus_one, e, m).rows + size - 1) / size);
       int inc = c;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -61,6 +52,65 @@ __device__ __forceinline__ void dz_prefix(int* prefix, const int32_t* offsets, i
   }
   __syncthreads();
 }
+// The group of chunk c: the last whose first chunk is not after it.
+__device__ __forceinline__ int chunk_group(const int* prefix, int E, int c) {
+  int lo = 0, hi = E - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (prefix[mid] <= c) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// A few rows on the CUDA cores: one warp per weight row and up to kWarpRows rows of A, lanes along
+// the contraction, so each weight is read once per kWarpRows rows and the latency does not grow
+// with K tile by tile.
+constexpr int kWarpRows = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+linear_rows_kernel(const T* __restrict__ A, const T* __restrict__ B, const LinearEpilogue<T> epi,
+                   const int32_t* __restrict__ offsets, int plus_one, int E, int64_t m, int64_t N, int64_t K) {
+  extern __shared__ int prefix[];
+  row_chunks(prefix, offsets, plus_one, E, m, kWarpRows);
+  const int lane = threadIdx.x & 31;
+  const int64_t total = (int64_t)prefix[E] * N, warps = (int64_t)gridDim.x * 8;
+  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < total; i += warps) {
+    const int c = (int)(i / N);
+    const int64_t n = i - (int64_t)c * N;
+    const int g = chunk_group(prefix, E, c);
+    const simt::GroupRange gr = simt::group_range(offsets, plus_one, g, m);
+    const int64_t r0 = gr.start + (int64_t)(c - prefix[g]) * kWarpRows;
+    const int rows = (int)min((int64_t)kWarpRows, gr.start + gr.rows - r0);
+    const T* w = B + ((int64_t)g * N + n) * K;
+    const T* a = A + r0 * K;
+    float acc[kWarpRows] = {};
+#pragma unroll 4
+    for (int64_t k = lane; k < K; k += 32) {
+      const float wv = to_f32(w[k]);
+#pragma unroll
+      for (int q = 0; q < kWarpRows; ++q)
+        if (q < rows) acc[q] = fmaf(to_f32(a[q * K + k]), wv, acc[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < kWarpRows; ++q) {
+      if (q >= rows) break;
+      float v = acc[q];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane == q) epi(v, g, r0 + q, n, N);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ backward, elementwise
+// One pass over dout and z: dz written (unless the activation is none: dz is dout) and the
+// column sums of dz taken from its fp32 values before they are rounded.  A block owns
+// kDzRows consecutive rows of one group and kDzCols columns; its column sums go to
+// partial[chunk, n] and dbias_kernel adds the chunks of a group in order, so the result does
+// not depend on the order blocks run in.  HBM-bound: 2 reads + 1 write of m * n elements.
+constexpr int kDzRows = 128;
+constexpr int kDzThreads = 256;
 
 template <typename T, int V>
 struct Pack {
@@ -76,16 +126,12 @@ dz_kernel(const T* __restrict__ dout, const T* __restrict__ z, T* __restrict__ d
           int64_t m, int64_t N, int act) {
   extern __shared__ int prefix[];
   __shared__ float red[8][32 * V + 1];
-  dz_prefix(prefix, offsets, plus_one, E, m);
+  row_chunks(prefix, offsets, plus_one, E, m, kDzRows);
   const int chunks = prefix[E];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t n = ((int64_t)blockIdx.x * 32 + tx) * V;
   for (int c = blockIdx.y; c < chunks; c += gridDim.y) {
-    int lo = 0, hi = E - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (prefix[mid] <= c) lo = mid; else hi = mid - 1;
-    }
+    const int lo = chunk_group(prefix, E, c);
     const simt::GroupRange gr = simt::group_range(offsets, plus_one, lo, m);
     const int64_t r0 = gr.start + (int64_t)(c - prefix[lo]) * kDzRows;
     const int64_t r1 = min(r0 + kDzRows, gr.start + gr.rows);
@@ -133,7 +179,7 @@ dbias_kernel(const float* __restrict__ partial, T* __restrict__ dbias,
   extern __shared__ int prefix[];
   __shared__ float red[8][33];
   pdl_wait();
-  dz_prefix(prefix, offsets, plus_one, E, m);
+  row_chunks(prefix, offsets, plus_one, E, m, kDzRows);
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t n = (int64_t)blockIdx.x * 32 + tx;
   for (int g = blockIdx.y; g < E; g += gridDim.y) {

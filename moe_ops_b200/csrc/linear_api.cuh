@@ -26,12 +26,24 @@ struct LinearArgs {
   cudaStream_t stream;
 };
 
+// Rows per group up to which a warp per weight row is taken over 64 x 64 tiles (which need at least
+// a slice of 32 in K per step, and 64 rows to be full).
+constexpr int kLinearWarpRows = 16;
+
 template <typename T>
 static int linear_simt(const LinearArgs& a) {
+  const LinearEpilogue<T> epi{(T*)a.out, (T*)a.preact, (const T*)a.bias, (const T*)a.residual, a.act};
+  if (!a.b_mn && a.E <= gmm::kMaxGroups && a.m <= (int64_t)kLinearWarpRows * a.E) {
+    const int64_t warps = ((a.m + kWarpRows - 1) / kWarpRows + (a.offsets ? a.E : 0)) * a.n;
+    const unsigned grid = (unsigned)std::min<int64_t>((warps + 7) / 8, 8 * num_sms(current_device()));
+    linear_rows_kernel<T><<<grid, 256, (size_t)(a.E + 1) * 4, a.stream>>>(
+        (const T*)a.A, (const T*)a.B, epi, a.offsets, a.plus_one, a.E, a.m, a.n, a.k);
+    MOE_LAUNCH_CHECK();
+    return MOE_OK;
+  }
   const dim3 grid((unsigned)((a.m + simt::TM - 1) / simt::TM), (unsigned)((a.n + simt::TN - 1) / simt::TN),
                   (unsigned)a.E);
   MOE_REQUIRE(grid.y <= 65535 && grid.z <= 65535, "linear: too large for the CUDA-core path");
-  const LinearEpilogue<T> epi{(T*)a.out, (T*)a.preact, (const T*)a.bias, (const T*)a.residual, a.act};
   simt::gmm_rows_simt_kernel<T><<<grid, 256, 0, a.stream>>>(
       (const T*)a.A, (const T*)a.B, epi, a.offsets, a.plus_one, a.m, a.n, a.k, a.b_mn);
   MOE_LAUNCH_CHECK();

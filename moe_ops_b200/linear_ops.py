@@ -27,6 +27,7 @@ import functools
 from typing import Optional
 
 import torch
+import torch.nn.functional as F
 
 from . import _lib
 
@@ -142,7 +143,25 @@ class _Linear(torch.autograd.Function):
         return dx, dw, db, dy if want_r else None, None, None, None, None, None
 
 
+# 16-bit operands whose rows are not 16-byte multiples: from this many multiplications on they are
+# copied into rows that are (zeros behind) for the tensor cores; below, the CUDA cores take
+# them as they are.
+_PAD_FROM = 1 << 24
+
+
+def _padded(x, w, bias, residual, offsets, act, trans_b, E, n):
+    k = x.shape[1]
+    dn, dk = -n % 8, -k % 8
+    w = F.pad(w, (0, dk, 0, dn) if trans_b else (0, dn, 0, dk))
+    y = _apply(F.pad(x, (0, dk)), w, None if bias is None else F.pad(bias, (0, dn)),
+               None if residual is None else F.pad(residual, (0, dn)), offsets, act, trans_b, E, n + dn)
+    return y[:, :n].contiguous()
+
+
 def _apply(x, w, bias, residual, offsets, act, trans_b, E, n):
+    m, k = x.shape
+    if (n % 8 or k % 8) and x.dtype != torch.float32 and m * n * k >= _PAD_FROM:
+        return _padded(x, w, bias, residual, offsets, act, trans_b, E, n)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias, residual)):
         return _Linear.apply(x, w, bias, residual, offsets, act, trans_b, E, n)
     return _forward(x, w, bias, residual, offsets, act, trans_b, E, n, False)[0]

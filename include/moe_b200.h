@@ -371,19 +371,18 @@ int moe_linear_fwd(const void* A, const void* B, const void* bias, const void* r
                    void* preact, const int32_t* offsets, int32_t num_offsets, int64_t m_total,
                    int64_t n, int64_t k, int32_t num_experts, int trans_b, int activation, int dtype,
                    void* workspace, size_t workspace_bytes, void* stream);
-/* The elementwise part of its backward: grad_preact = grad_out * act'(preact) and grad_bias
- * [E, n] = its sum over each expert's rows (from the unrounded products, in a fixed order; NULL:
- * not wanted).  For MOE_ACT_NONE grad_preact is grad_out itself: it is not written, and preact
- * and grad_preact may be NULL.  The products' gradients are moe_gmm_dgrad and moe_gmm_wgrad on
- * grad_preact (which take offsets NULL, num_offsets 0, num_experts 1 for a dense product). */
-size_t moe_linear_act_bwd_workspace_bytes(int64_t m_total, int64_t n, int32_t num_experts);
-int moe_linear_act_bwd(const void* grad_out, const void* preact, void* grad_preact, void* grad_bias,
-                       const int32_t* offsets, int32_t num_offsets, int64_t m_total, int64_t n,
-                       int32_t num_experts, int activation, int dtype, void* workspace,
-                       size_t workspace_bytes, void* stream);
-/* Zeroes the rows of out [m_total, n] behind the last offset. */
-int moe_zero_tail_rows(void* out, const int32_t* offsets, int32_t num_offsets, int64_t m_total,
-                       int64_t n, int dtype, void* stream);
+/* Its backward: dz = grad_out * act'(preact), then grad_A [m_total, k] = dz . op(B)^T, grad_B (B's
+ * shape) = A^T . dz per expert and grad_bias [E, n] = the sum of dz over each expert's rows (from
+ * its unrounded values, in a fixed order).  Each of the three may be NULL.  preact is
+ * moe_linear_fwd's (not read for MOE_ACT_NONE).  Rows of grad_A behind the last offset are zero;
+ * the residual's gradient is grad_out itself.  Workspace: moe_linear_bwd_workspace_bytes(...)
+ * bytes, 16-byte aligned. */
+size_t moe_linear_bwd_workspace_bytes(int64_t m_total, int64_t n, int32_t num_experts, int activation,
+                                      int dtype);
+int moe_linear_bwd(const void* grad_out, const void* A, const void* B, const void* preact, void* grad_A,
+                   void* grad_B, void* grad_bias, const int32_t* offsets, int32_t num_offsets,
+                   int64_t m_total, int64_t n, int64_t k, int32_t num_experts, int trans_b,
+                   int activation, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

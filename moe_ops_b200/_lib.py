@@ -90,10 +90,10 @@ SIGNATURES = {
     "moe_linear_fwd": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i32, _c_i64,
                                 _c_i64, _c_i64, _c_i32, _c_int, _c_int, _c_int, _c_ptr, _c_size, _c_ptr]),
     "moe_linear_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64, _c_i32, _c_int, _c_int]),
-    "moe_linear_act_bwd_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i32]),
-    "moe_linear_act_bwd": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i32, _c_i64, _c_i64,
-                                    _c_i32, _c_int, _c_int, _c_ptr, _c_size, _c_ptr]),
-    "moe_zero_tail_rows": (_c_int, [_c_ptr, _c_ptr, _c_i32, _c_i64, _c_i64, _c_int, _c_ptr]),
+    "moe_linear_bwd_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i32, _c_int, _c_int]),
+    "moe_linear_bwd": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i32,
+                                _c_i64, _c_i64, _c_i64, _c_i32, _c_int, _c_int, _c_int, _c_ptr,
+                                _c_size, _c_ptr]),
     "moe_few_tokens_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64, _c_i32, _c_i32, _c_int]),
     "moe_few_tokens_fwd": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_i64,
                                     _c_i64, _c_i64, _c_i32, _c_i32, _c_ptr, _c_ptr, _c_size, _c_ptr]),

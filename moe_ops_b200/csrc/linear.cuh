@@ -6,6 +6,7 @@
 #pragma once
 
 #include "activation.cuh"
+#include "few_tokens.cuh"
 #include "gmm_simt.cuh"
 
 namespace moe {
@@ -67,39 +68,48 @@ __device__ __forceinline__ int chunk_group(const int* prefix, int E, int c) {
 // with K tile by tile.
 constexpr int kWarpRows = 8;
 
-template <typename T>
+// VEC: 16-byte loads (rows that are 16-byte multiples).
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
 linear_rows_kernel(const T* __restrict__ A, const T* __restrict__ B, const LinearEpilogue<T> epi,
-                   const int32_t* __restrict__ offsets, int plus_one, int E, int64_t m, int64_t N, int64_t K) {
+                   const int32_t* __restrict__ offsets, int plus_one, int E, int64_t m, int N, int K) {
   extern __shared__ int prefix[];
   row_chunks(prefix, offsets, plus_one, E, m, kWarpRows);
+  constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
   const int lane = threadIdx.x & 31;
   const int64_t total = (int64_t)prefix[E] * N, warps = (int64_t)gridDim.x * 8;
   for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < total; i += warps) {
-    const int c = (int)(i / N);
-    const int64_t n = i - (int64_t)c * N;
+    const int c = (int)(i / N), n = (int)(i - (int64_t)c * N);
     const int g = chunk_group(prefix, E, c);
     const simt::GroupRange gr = simt::group_range(offsets, plus_one, g, m);
     const int64_t r0 = gr.start + (int64_t)(c - prefix[g]) * kWarpRows;
     const int rows = (int)min((int64_t)kWarpRows, gr.start + gr.rows - r0);
     const T* w = B + ((int64_t)g * N + n) * K;
-    const T* a = A + r0 * K;
-    float acc[kWarpRows] = {};
-#pragma unroll 4
-    for (int64_t k = lane; k < K; k += 32) {
-      const float wv = to_f32(w[k]);
+    const T* a[kWarpRows];  // a row past the chunk repeats its first: loads need no branch
 #pragma unroll
-      for (int q = 0; q < kWarpRows; ++q)
-        if (q < rows) acc[q] = fmaf(to_f32(a[q * K + k]), wv, acc[q]);
+    for (int q = 0; q < kWarpRows; ++q) a[q] = A + (r0 + (q < rows ? q : 0)) * K;
+    float acc[kWarpRows] = {};
+#pragma unroll 2
+    for (int k = lane * V; k < K; k += 32 * V) {
+      float wv[V];
+      few::load_vec<T, VEC>(w + k, wv);
+#pragma unroll
+      for (int q = 0; q < kWarpRows; ++q) {
+        float av[V];
+        few::load_vec<T, VEC>(a[q] + k, av);
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[q] = fmaf(av[j], wv[j], acc[q]);
+      }
     }
+    float mine = 0.f;
 #pragma unroll
     for (int q = 0; q < kWarpRows; ++q) {
-      if (q >= rows) break;
       float v = acc[q];
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (lane == q) epi(v, g, r0 + q, n, N);
+      if (lane == q) mine = v;
     }
+    if (lane < rows) epi(mine, g, r0 + lane, n, N);
   }
 }
 

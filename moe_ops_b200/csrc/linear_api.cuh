@@ -7,8 +7,19 @@
 
 namespace moe {
 
-// Rows up to which the few-row kernel takes a product.
-static int64_t few_linear_max_rows(int E) { return E <= 1 ? 64 : 64; }
+// When the few-row kernel takes a product over the row tiles of 128 x 256: up to 16 rows, and up to
+// 192 rows of a dense product whose tiles would keep no more than an eighth of the SMs busy over
+// a long contraction.  Measured, row tiles / few rows in us (bf16, dense unless said):
+//   1 row   4096 -> 11008   41 / 25       64 rows  4096 -> 11008  39 / 46
+//   37 rows 7168 -> 4096    49 / 27       64 rows  7168 -> 2048   48 / 25
+//   64 rows 2048 -> 7168    23 / 35       192 rows 7168 -> 2048   49 / 40
+//   64 rows 1024 -> 1024    16 / 29       256 rows 7168 -> 2048   49 / 60
+//   16 rows, 8 groups, 4096 -> 2048  43 / 33;  64 rows 45 / 52
+static bool few_linear_wins(int64_t m, int64_t n, int64_t k, bool dense) {
+  if (m <= 16) return true;
+  return dense && m <= 192 && k >= 4096 &&
+         (m + 127) / 128 * ((n + 255) / 256) * 8 <= num_sms(current_device());
+}
 
 struct LinearArgs {
   const void* A;
@@ -33,11 +44,17 @@ constexpr int kLinearWarpRows = 16;
 template <typename T>
 static int linear_simt(const LinearArgs& a) {
   const LinearEpilogue<T> epi{(T*)a.out, (T*)a.preact, (const T*)a.bias, (const T*)a.residual, a.act};
-  if (!a.b_mn && a.E <= gmm::kMaxGroups && a.m <= (int64_t)kLinearWarpRows * a.E) {
+  if (!a.b_mn && a.E <= gmm::kMaxGroups && a.m <= (int64_t)kLinearWarpRows * a.E && a.n < (1 << 30) &&
+      a.k < (1 << 30)) {
     const int64_t warps = ((a.m + kWarpRows - 1) / kWarpRows + (a.offsets ? a.E : 0)) * a.n;
     const unsigned grid = (unsigned)std::min<int64_t>((warps + 7) / 8, 8 * num_sms(current_device()));
-    linear_rows_kernel<T><<<grid, 256, (size_t)(a.E + 1) * 4, a.stream>>>(
-        (const T*)a.A, (const T*)a.B, epi, a.offsets, a.plus_one, a.E, a.m, a.n, a.k);
+    const size_t smem = (size_t)(a.E + 1) * 4;
+    if ((a.k * sizeof(T)) % 16 == 0 && aligned16(a.A) && aligned16(a.B))
+      linear_rows_kernel<T, true><<<grid, 256, smem, a.stream>>>(
+          (const T*)a.A, (const T*)a.B, epi, a.offsets, a.plus_one, a.E, a.m, (int)a.n, (int)a.k);
+    else
+      linear_rows_kernel<T, false><<<grid, 256, smem, a.stream>>>(
+          (const T*)a.A, (const T*)a.B, epi, a.offsets, a.plus_one, a.E, a.m, (int)a.n, (int)a.k);
     MOE_LAUNCH_CHECK();
     return MOE_OK;
   }
@@ -130,7 +147,7 @@ static FewLinear few_linear_plan(int64_t m, int64_t n, int64_t k, int E, bool de
 }
 
 static bool few_linear_ok(const LinearArgs& a) {
-  return linear_tc_ok(a) && !a.b_mn && a.m <= few_linear_max_rows(a.E);
+  return linear_tc_ok(a) && !a.b_mn && few_linear_wins(a.m, a.n, a.k, a.offsets == nullptr);
 }
 
 static int few_linear(const LinearArgs& a, void* workspace, size_t workspace_bytes) {
@@ -192,18 +209,65 @@ static int check_linear(const void* a, const void* b, const void* out, const int
   return check_gmm_args(out, out, out, offsets, num_offsets, out ? m : 0, n, k, E, dtype);
 }
 
+// Workspace of the backward: dz [m, n] (unless there is no activation), then the bias gradient's
+// partial sums.
+struct BwdWorkspace {
+  size_t partial, total;
+};
+static BwdWorkspace bwd_workspace(int64_t m, int64_t n, int E, int act, int dtype) {
+  BwdWorkspace w;
+  w.partial = act == MOE_ACT_NONE ? 0 : align256((size_t)m * n * dtype_size(dtype));
+  w.total = w.partial + (size_t)((m + kDzRows - 1) / kDzRows + E) * n * 4 + 16;
+  return w;
+}
+
+// dz = grad_out * act'(preact) (written unless act is none) and grad_bias (may be NULL).
+static int act_bwd(const void* grad_out, const void* preact, void* dz, void* grad_bias,
+                   const int32_t* offsets, int num_offsets, int64_t m, int64_t n, int E, int activation,
+                   int dtype, float* partial, cudaStream_t s) {
+  MOE_REQUIRE(E <= gmm::kMaxGroups, "linear_bwd: more than %d experts", gmm::kMaxGroups);
+  const bool act = activation != MOE_ACT_NONE;
+  const int plus_one = num_offsets == E + 1;
+  if (!grad_bias) partial = nullptr;
+  const int64_t chunks = (m + kDzRows - 1) / kDzRows + (offsets ? E : 0);
+  const size_t smem = (size_t)(E + 1) * 4;
+  const bool vec = (n * dtype_size(dtype)) % 16 == 0 && aligned16(grad_out) &&
+                   (!act || (aligned16(preact) && aligned16(dz)));
+  int rc = MOE_DISPATCH_DTYPE(dtype, T, [&] {
+    constexpr int V = 16 / (int)sizeof(T);
+    const int cols = 32 * (vec ? V : 1);
+    const dim3 grid((unsigned)((n + cols - 1) / cols), (unsigned)std::min<int64_t>(chunks, 32768));
+    if (vec)
+      dz_kernel<T, V><<<grid, kDzThreads, smem, s>>>((const T*)grad_out, (const T*)preact, (T*)dz, partial,
+                                                     offsets, plus_one, E, m, n, activation);
+    else
+      dz_kernel<T, 1><<<grid, kDzThreads, smem, s>>>((const T*)grad_out, (const T*)preact, (T*)dz, partial,
+                                                     offsets, plus_one, E, m, n, activation);
+    MOE_LAUNCH_CHECK();
+    return (int)MOE_OK;
+  });
+  if (rc || !grad_bias) return rc;
+  return MOE_DISPATCH_DTYPE(dtype, T, [&] {
+    const dim3 grid((unsigned)((n + 31) / 32), (unsigned)std::min(E, 1024));
+    MOE_CUDA_CHECK(launch_pdl(dbias_kernel<T>, grid, dim3(kDzThreads), smem, s, (const float*)partial,
+                              (T*)grad_bias, offsets, plus_one, E, m, n));
+    return (int)MOE_OK;
+  });
+}
+
 }  // namespace moe
 
 extern "C" {
 
 size_t moe_linear_workspace_bytes(int64_t m_total, int64_t n, int64_t k, int32_t num_experts,
                                   int trans_b, int dtype) {
-  if (m_total <= 0 || n <= 0 || k <= 0 || num_experts <= 0 || !trans_b || dtype == MOE_F32 ||
-      m_total > few_linear_max_rows(num_experts))
-    return 0;
-  // whether the product is dense only changes the split: the larger of the two
-  return std::max(few_linear_plan(m_total, n, k, num_experts, false).total,
-                  few_linear_plan(m_total, n, k, num_experts, true).total);
+  if (m_total <= 0 || n <= 0 || k <= 0 || num_experts <= 0 || !trans_b || dtype == MOE_F32) return 0;
+  size_t need = 0;  // of a grouped and, with one expert, of a dense product
+  if (few_linear_wins(m_total, n, k, false))
+    need = few_linear_plan(m_total, n, k, num_experts, false).total;
+  if (num_experts == 1 && few_linear_wins(m_total, n, k, true))
+    need = std::max(need, few_linear_plan(m_total, n, k, 1, true).total);
+  return need;
 }
 
 int moe_linear_fwd(const void* A, const void* B, const void* bias, const void* residual, void* out,
@@ -234,69 +298,53 @@ int moe_linear_fwd(const void* A, const void* B, const void* bias, const void* r
   return MOE_OK;
 }
 
-size_t moe_linear_act_bwd_workspace_bytes(int64_t m_total, int64_t n, int32_t num_experts) {
-  if (m_total <= 0 || n <= 0 || num_experts <= 0) return 16;
-  return (size_t)((m_total + kDzRows - 1) / kDzRows + num_experts) * n * 4 + 16;
+size_t moe_linear_bwd_workspace_bytes(int64_t m_total, int64_t n, int32_t num_experts, int activation,
+                                      int dtype) {
+  if (m_total <= 0 || n <= 0 || num_experts <= 0 || !dtype_ok(dtype)) return 16;
+  return bwd_workspace(m_total, n, num_experts, activation, dtype).total;
 }
 
-int moe_linear_act_bwd(const void* grad_out, const void* preact, void* grad_preact, void* grad_bias,
-                       const int32_t* offsets, int32_t num_offsets, int64_t m_total, int64_t n,
-                       int32_t num_experts, int activation, int dtype, void* workspace,
-                       size_t workspace_bytes, void* stream) {
+int moe_linear_bwd(const void* grad_out, const void* A, const void* B, const void* preact, void* grad_A,
+                   void* grad_B, void* grad_bias, const int32_t* offsets, int32_t num_offsets,
+                   int64_t m_total, int64_t n, int64_t k, int32_t num_experts, int trans_b,
+                   int activation, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_linear(nullptr, nullptr, grad_out, offsets, num_offsets, m_total, n, 0, num_experts,
                         activation, dtype);
   if (rc) return rc;
-  const bool act = activation != MOE_ACT_NONE;
-  MOE_REQUIRE(!act || m_total == 0 || (preact && grad_preact), "linear_act_bwd: NULL operand");
+  MOE_REQUIRE(k >= 0, "linear_bwd: negative size");
+  const bool act = activation != MOE_ACT_NONE, any = m_total > 0 && n > 0 && num_experts > 0;
+  MOE_REQUIRE(!any || !act || preact, "linear_bwd: preact is NULL");
+  MOE_REQUIRE(!any || k == 0 || ((!grad_A || B) && (!grad_B || A)), "linear_bwd: NULL operand");
   cudaStream_t s = (cudaStream_t)stream;
-  if (n == 0 || num_experts == 0) return MOE_OK;
-  if (m_total == 0) {
-    if (grad_bias)
-      MOE_CUDA_CHECK(cudaMemsetAsync(grad_bias, 0, (size_t)num_experts * n * dtype_size(dtype), s));
+  const int es = dtype_size(dtype);
+  if (!any) {  // sums over nothing
+    if (grad_A && m_total > 0 && k > 0) MOE_CUDA_CHECK(cudaMemsetAsync(grad_A, 0, (size_t)m_total * k * es, s));
+    if (grad_B && num_experts * n * k > 0)
+      MOE_CUDA_CHECK(cudaMemsetAsync(grad_B, 0, (size_t)num_experts * n * k * es, s));
+    if (grad_bias && num_experts * n > 0)
+      MOE_CUDA_CHECK(cudaMemsetAsync(grad_bias, 0, (size_t)num_experts * n * es, s));
     return MOE_OK;
   }
-  if (!act && !grad_bias) return MOE_OK;
-  MOE_REQUIRE(num_experts <= gmm::kMaxGroups, "linear_act_bwd: more than %d experts", gmm::kMaxGroups);
-  if (grad_bias && (!workspace || workspace_bytes <
-                                      moe_linear_act_bwd_workspace_bytes(m_total, n, num_experts)))
-    return set_error(MOE_ERR_WORKSPACE, "linear_act_bwd: workspace too small");
-  const int plus_one = num_offsets == num_experts + 1;
-  const int E = num_experts;
-  float* partial = grad_bias ? (float*)workspace : nullptr;
-  const int64_t chunks = (m_total + kDzRows - 1) / kDzRows + (offsets ? E : 0);
-  const size_t smem = (size_t)(E + 1) * 4;
-  const int es = dtype_size(dtype);
-  const bool vec = (n * es) % 16 == 0 && aligned16(grad_out) && (!act || (aligned16(preact) && aligned16(grad_preact)));
-  rc = MOE_DISPATCH_DTYPE(dtype, T, [&] {
-    constexpr int V = 16 / (int)sizeof(T);
-    const int cols = 32 * (vec ? V : 1);
-    const dim3 grid((unsigned)((n + cols - 1) / cols), (unsigned)std::min<int64_t>(chunks, 32768));
-    if (vec)
-      dz_kernel<T, V><<<grid, kDzThreads, smem, s>>>((const T*)grad_out, (const T*)preact,
-                                                     (T*)grad_preact, partial, offsets, plus_one, E,
-                                                     m_total, n, activation);
-    else
-      dz_kernel<T, 1><<<grid, kDzThreads, smem, s>>>((const T*)grad_out, (const T*)preact,
-                                                     (T*)grad_preact, partial, offsets, plus_one, E,
-                                                     m_total, n, activation);
-    MOE_LAUNCH_CHECK();
-    return (int)MOE_OK;
-  });
-  if (rc || !grad_bias) return rc;
-  return MOE_DISPATCH_DTYPE(dtype, T, [&] {
-    const dim3 grid((unsigned)((n + 31) / 32), (unsigned)std::min(E, 1024));
-    MOE_CUDA_CHECK(launch_pdl(dbias_kernel<T>, grid, dim3(kDzThreads), smem, s, (const float*)partial,
-                              (T*)grad_bias, offsets, plus_one, E, m_total, n));
-    return (int)MOE_OK;
-  });
-}
-
-int moe_zero_tail_rows(void* out, const int32_t* offsets, int32_t num_offsets, int64_t m_total,
-                       int64_t n, int dtype, void* stream) {
-  MOE_REQUIRE(dtype_ok(dtype), "zero_tail_rows: bad dtype %d", dtype);
-  MOE_REQUIRE(offsets && num_offsets > 0 && m_total >= 0 && n >= 0 && (out || m_total == 0 || n == 0),
-              "zero_tail_rows: bad arguments");
-  return tail_rows(out, nullptr, offsets, num_offsets - 1, m_total, n, dtype, (cudaStream_t)stream);
+  const BwdWorkspace w = bwd_workspace(m_total, n, num_experts, activation, dtype);
+  if ((act || grad_bias) && (!workspace || workspace_bytes < w.total))
+    return set_error(MOE_ERR_WORKSPACE, "linear_bwd: workspace has %zu bytes, needs %zu",
+                     workspace ? workspace_bytes : (size_t)0, w.total);
+  MOE_REQUIRE(!(act || grad_bias) || aligned16(workspace), "linear_bwd: workspace must be 16-byte aligned");
+  void* dz = act ? workspace : const_cast<void*>(grad_out);
+  if (act || grad_bias) {
+    rc = act_bwd(grad_out, preact, dz, grad_bias, offsets, num_offsets, m_total, n, num_experts,
+                 activation, dtype, (float*)((uint8_t*)workspace + w.partial), s);
+    if (rc) return rc;
+  }
+  if (grad_A && k > 0) {
+    rc = moe_gmm_dgrad(dz, B, grad_A, offsets, num_offsets, m_total, n, k, num_experts, trans_b, dtype, stream);
+    if (rc) return rc;
+    rc = tail_rows(grad_A, nullptr, offsets, num_offsets - 1, m_total, k, dtype, s);
+    if (rc) return rc;
+  }
+  if (grad_B && k > 0)
+    return moe_gmm_wgrad(A, dz, grad_B, offsets, num_offsets, m_total, n, k, num_experts, trans_b, dtype, stream);
+  return MOE_OK;
 }
 
 }  // extern "C"

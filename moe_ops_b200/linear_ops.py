@@ -75,44 +75,29 @@ def _forward(x, w, bias, residual, offsets, act: int, trans_b: bool, E: int, n: 
     return y, z
 
 
-def _act_bwd(dy, z, offsets, E: int, act: int, want_bias: bool, bias_shape):
-    """(dz, dbias): one pass over dy and z."""
-    m, n = dy.shape
-    code = _lib.dtype_code(dy.dtype)
-    dz = torch.empty_like(dy) if act else dy
-    db = torch.empty(bias_shape, device=dy.device, dtype=dy.dtype) if want_bias else None
-    if not act and db is None:
-        return dz, None
-    lib = _lib.load()
-    ws_bytes = lib.moe_linear_act_bwd_workspace_bytes(m, n, E) if want_bias else 0
-    ws = torch.empty(ws_bytes, device=dy.device, dtype=torch.uint8)
-    with _lib.on_device(dy):
-        st = lib.moe_linear_act_bwd(
-            dy.data_ptr(), _lib.ptr(z), dz.data_ptr() if act else None, _lib.ptr(db),
-            _lib.ptr(offsets), 0 if offsets is None else offsets.numel(), m, n, E, act, code,
-            ws.data_ptr() if ws_bytes else None, ws_bytes, _lib.raw_stream(dy))
-    _lib.check(st, "moe_linear_act_bwd")
-    _lib.count_launches(1 + int(want_bias))
-    return dz, db
+@functools.lru_cache(maxsize=4096)
+def _bwd_workspace_bytes(m: int, n: int, E: int, act: int, code: int) -> int:
+    return _lib.load().moe_linear_bwd_workspace_bytes(m, n, E, act, code)
 
 
-def _gemm(fn: str, a, b, shape, offsets, m, n, k, E, trans_b):
-    out = torch.empty(shape, device=a.device, dtype=a.dtype)
-    if out.numel() == 0 or (n if fn == "moe_gmm_dgrad" else m) == 0:
-        return out.zero_()
+def _backward(dy, x, w, z, offsets, act: int, trans_b: bool, E: int, n: int, bias_shape, wanted):
+    """(dx, dw, dbias), None where not wanted."""
+    m, k = x.shape
+    dx = torch.empty_like(x) if wanted[0] else None
+    dw = torch.empty_like(w) if wanted[1] else None
+    db = torch.empty(bias_shape, device=x.device, dtype=x.dtype) if wanted[2] else None
+    code = _lib.dtype_code(x.dtype)
     lib = _lib.load()
-    with _lib.on_device(a):
-        st = getattr(lib, fn)(
-            a.data_ptr(), b.data_ptr(), out.data_ptr(), _lib.ptr(offsets),
-            0 if offsets is None else offsets.numel(), m, n, k, E, int(trans_b),
-            _lib.dtype_code(a.dtype), _lib.raw_stream(a))
-        _lib.check(st, fn)
-        if fn == "moe_gmm_dgrad" and offsets is not None:
-            _lib.check(lib.moe_zero_tail_rows(out.data_ptr(), offsets.data_ptr(), offsets.numel(), m,
-                                              k, _lib.dtype_code(a.dtype), _lib.raw_stream(a)),
-                       "moe_zero_tail_rows")
-    _lib.count_launches(1)
-    return out
+    with _lib.on_device(x):
+        ws_bytes = _bwd_workspace_bytes(m, n, E, act, code) if act or wanted[2] else 0
+        ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8) if ws_bytes else None
+        st = lib.moe_linear_bwd(
+            dy.data_ptr(), x.data_ptr(), w.data_ptr(), _lib.ptr(z), _lib.ptr(dx), _lib.ptr(dw),
+            _lib.ptr(db), _lib.ptr(offsets), 0 if offsets is None else offsets.numel(), m, n, k, E,
+            int(trans_b), act, code, _lib.ptr(ws), ws_bytes, _lib.raw_stream(x))
+    _lib.check(st, "moe_linear_bwd")
+    _lib.count_launches(sum(wanted) + int(act != 0))
+    return dx, dw, db
 
 
 class _Linear(torch.autograd.Function):
@@ -129,18 +114,11 @@ class _Linear(torch.autograd.Function):
     def backward(ctx, dy):
         x, w, z, offsets = ctx.saved_tensors
         act, trans_b, E, n, bias_shape = ctx.cfg
-        m, k = x.shape
-        want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
+        wanted = ctx.needs_input_grad[:3]
         dx = dw = db = None
-        if want_x or want_w or want_b:
-            dyc = dy.contiguous()
-            dz, db = _act_bwd(dyc, z, offsets, E, act if (want_x or want_w or want_b) else 0, want_b,
-                              bias_shape)
-            if want_x:
-                dx = _gemm("moe_gmm_dgrad", dz, w, (m, k), offsets, m, n, k, E, trans_b)
-            if want_w:
-                dw = _gemm("moe_gmm_wgrad", x, dz, w.shape, offsets, m, n, k, E, trans_b)
-        return dx, dw, db, dy if want_r else None, None, None, None, None, None
+        if any(wanted):
+            dx, dw, db = _backward(dy.contiguous(), x, w, z, offsets, act, trans_b, E, n, bias_shape, wanted)
+        return dx, dw, db, dy if ctx.needs_input_grad[3] else None, None, None, None, None, None
 
 
 # 16-bit operands whose rows are not 16-byte multiples: from this many multiplications on they are

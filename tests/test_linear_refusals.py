@@ -30,14 +30,19 @@ def test_c_abi_refusals(lib):
     assert ws > 0 and lib.moe_linear_workspace_bytes(100000, 8, 8, 1, 1, 2) == 0
     st, msg = fwd(ws=ws - 1)
     assert st == 4 and b"workspace" in msg
-    need = lib.moe_linear_act_bwd_workspace_bytes(300, 64, 3)
-    assert need >= 3 * 64 * 4
-    st = lib.moe_linear_act_bwd(p, p, p, p, None, 0, 300, 64, 1, 4, 2, p, 8, None)
-    assert st == 4 and b"workspace" in lib.moe_last_error_string()
-    st = lib.moe_linear_act_bwd(p, None, p, None, None, 0, 300, 64, 1, 4, 2, None, 0, None)
-    assert st == 1
-    assert lib.moe_zero_tail_rows(p, None, 0, 4, 8, 2, None) == 1
-    assert lib.moe_zero_tail_rows(p, p, 1, 4, 8, 9, None) == 1
+    need = lib.moe_linear_bwd_workspace_bytes(300, 64, 3, 4, 2)
+    assert need >= 300 * 64 * 2 + 3 * 64 * 4
+
+    def bwd(z=p, b=p, off=None, num=0, E=1, act=4, ws=need, dtype=2, k=8):
+        st = lib.moe_linear_bwd(p, p, b, z, p, p, p, off, num, 300, 64, k, E, 1, act, dtype, p, ws, None)
+        return st, lib.moe_last_error_string()
+
+    for kw, status, word in ((dict(ws=8), 4, b"workspace"), (dict(z=None), 1, b"preact"),
+                             (dict(b=None), 1, b"NULL"), (dict(act=9), 1, b"activation"),
+                             (dict(dtype=5), 1, b"dtype"), (dict(E=3), 1, b"num_offsets"),
+                             (dict(k=-1), 1, b"negative")):
+        st, msg = bwd(**kw)
+        assert st == status and word in msg, (kw, st, msg)
 
 
 def test_python_refusals():

@@ -141,7 +141,7 @@ __device__ __forceinline__ void linear_out(const Params& p, int e, int64_t row, 
   if (p.bias) z += to_f32(static_cast<const T*>(p.bias)[(int64_t)e * p.N + col]);
   const int64_t at = row * p.N + col;
   if (p.preact) static_cast<T*>(p.preact)[at] = from_f32<T>(z);
-  float y = act_fwd_rt(p.act, z);
+  float y = act_fwd_rt<true>(p.act, z);
   if (p.residual) y += to_f32(static_cast<const T*>(p.residual)[at]);
   static_cast<T*>(p.y)[at] = from_f32<T>(y);
 }

@@ -870,7 +870,7 @@ gmm_sm100_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           if (p.preact) pack32_16b<OutT>(v, wz);
           MOE_SWITCH_ACT(p.act, ACT, {
             _Pragma("unroll") for (int i = 0; i < 32; ++i)
-              v[i] = __float_as_uint(act_fwd<ACT>(__uint_as_float(v[i])) + to_f32(rv[i]));
+              v[i] = __float_as_uint(act_fwd<ACT, true>(__uint_as_float(v[i])) + to_f32(rv[i]));
           })
           pack32_16b<OutT>(v, wy);
           if (c + 1 < nchunks) ptx::tmem_ld_32x32b_x32(tbase + (c + 1) * 32, v);

@@ -24,7 +24,7 @@ struct LinearEpilogue {
     float z = acc;
     if (bias) z += to_f32(bias[(int64_t)g * N + n]);
     if (preact) preact[at] = from_f32<T>(z);
-    float y = act_fwd_rt(act, z);
+    float y = act_fwd_rt<sizeof(T) == 2>(act, z);
     if (residual) y += to_f32(residual[at]);
     out[at] = from_f32<T>(y);
   }
@@ -157,7 +157,7 @@ dz_kernel(const T* __restrict__ dout, const T* __restrict__ z, T* __restrict__ d
           _Pragma("unroll") for (int j = 0; j < V; ++j) {
             float v = to_f32(d.p.v[j]);
             if constexpr (ACT != MOE_ACT_NONE) {
-              v *= act_bwd<ACT>(to_f32(zz.p.v[j]));
+              v *= act_bwd<ACT, sizeof(T) == 2>(to_f32(zz.p.v[j]));
               o.p.v[j] = from_f32<T>(v);
             }
             sum[j] += v;

@@ -234,3 +234,31 @@ def test_side_stream_and_graph_replay(cuda_dev):
     torch.cuda.synchronize()
     assert torch.equal(graphs[0][1], want_p.flip(0))
     assert _lib.read_device_error() == 0
+
+
+def test_two_streams_at_once(cuda_dev):
+    """Eager calls that overlap on two streams, both persistent over all SMs."""
+    a = make(cuda_dev, 9, 1024, 32, 1024, BF, seed=21)
+    b = make(cuda_dev, 3, 512, 8, 2048, BF, seed=22)
+    want_a, want_b = M.moe_few_tokens(**a, top_k=4), M.moe_few_tokens(**b, top_k=2)
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(20):
+        with torch.cuda.stream(s1):
+            got.append((M.moe_few_tokens(**a, top_k=4), want_a))
+        with torch.cuda.stream(s2):
+            got.append((M.moe_few_tokens(**b, top_k=2), want_b))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, w) for y, w in got)
+    assert _lib.read_device_error() == 0
+
+
+def test_a_row_does_not_depend_on_its_batch(cuda_dev):
+    """The same token alone and among others, with the sizes' split held (same T): other rows'
+    values change nothing."""
+    p = make(cuda_dev, 8, 512, 16, 512, BF, seed=23)
+    y = M.moe_few_tokens(**p, top_k=2)
+    q = dict(p, x=p["x"].clone())
+    q["x"][1:] = torch.randn_like(q["x"][1:])
+    assert torch.equal(M.moe_few_tokens(**q, top_k=2)[0], y[0])

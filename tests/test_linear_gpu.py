@@ -274,6 +274,51 @@ def test_shapes_strides_and_empty(cuda_dev):
     assert torch.equal(we.grad, torch.zeros_like(w)) and torch.equal(be.grad, torch.zeros_like(b))
 
 
+@pytest.mark.parametrize("E,trans_b", [(0, True), (3, True), (3, False)])
+def test_large_unaligned_products_are_padded(cuda_dev, E, trans_b):
+    """16-bit rows that are no 16-byte multiples, large enough for the padded path."""
+    m, k, n = 140, 401, 333
+    x, w, b, r, dy = make(cuda_dev, m, k, n, BF, 8, E=E, trans_b=trans_b)
+    off = torch.tensor([0, 50, 50, 131], device=cuda_dev, dtype=torch.int32) if E else None
+    run_case(x, w, b, r, dy, "silu", BF, offsets=off, trans_b=trans_b)
+
+
+def test_large_products_off_a_boundary(cuda_dev):
+    m, k, n = 140, 400, 336
+    x, w, b, r, dy = make(cuda_dev, m, k, n, FP, 9)
+
+    def shifted(t):
+        flat = torch.empty(t.numel() + 1, device=cuda_dev, dtype=t.dtype)
+        v = flat[1:].view(t.shape)
+        v.copy_(t)
+        return v
+
+    got = M.linear(shifted(x), shifted(w), bias=shifted(b), activation="gelu", residual=shifted(r))
+    assert torch.equal(got, M.linear(x, w, bias=b, activation="gelu", residual=r))
+
+
+def test_no_experts_and_no_rows(cuda_dev):
+    x, w, b, r, dy = make(cuda_dev, 6, 64, 72, BF, 10, E=2)
+    none = torch.zeros(1, device=cuda_dev, dtype=torch.int32)
+    leaf = x.clone().requires_grad_(True)
+    y = M.grouped_linear(leaf, w[:0], none, bias=b[:0], activation="silu", residual=r)
+    assert torch.equal(y.detach(), r)
+    y.sum().backward()
+    assert torch.equal(leaf.grad, torch.zeros_like(x))
+    off = torch.zeros(3, device=cuda_dev, dtype=torch.int32)
+    leaf = [t.clone().requires_grad_(True) for t in (w, b)]
+    y = M.grouped_linear(x[:0], leaf[0], off, bias=leaf[1], activation="silu")
+    y.sum().backward()
+    assert y.shape == (0, 72) and all(torch.equal(t.grad, torch.zeros_like(t)) for t in leaf)
+
+
+def test_a_cut_few_row_product(cuda_dev):
+    """Rows, columns and depth for which the contraction is cut: the parts' order is fixed."""
+    for m, k, n in ((37, 4160, 256), (64, 8192, 1000), (130, 4096, 520), (16, 4160, 8)):
+        x, w, b, r, dy = make(cuda_dev, m, k, n, BF, m)
+        run_case(x, w, b, r, dy, "silu", BF)
+
+
 def test_partial_gradients(cuda_dev):
     """Each subset of the inputs that require a gradient gives the same gradients."""
     x, w, b, r, dy = make(cuda_dev, 140, 72, 96, BF, 4)

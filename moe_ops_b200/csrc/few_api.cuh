@@ -122,10 +122,11 @@ static int few_ring(fewtc::Params& p, int phases, int nb, int table_bytes) {
   return MOE_OK;
 }
 
-// Workspace: logits [T, E] fp32, h [T*K, H] (fp32 for the CUDA cores, else 16 bits), then for
-// the tensor-core kernel its counters and fp32 results.
+// Workspace: logits [T, E] fp32; h [T*K, H] (fp32 for the CUDA cores, else 16 bits); the CUDA
+// cores' slot weights and positions; the tensor-core kernel's counters; the experts' outputs, fp32
+// [parts, T*K, d] (one part for the CUDA cores).
 struct FewWorkspace {
-  size_t logits, h, counters, part, total;
+  size_t logits, h, slots, counters, part, total;
   int num_counters, max_units;
   FewSplit split0, split1;
 };
@@ -134,19 +135,21 @@ static FewWorkspace few_workspace(int64_t T, int64_t d, int64_t H, int64_t E, in
   const size_t S = (size_t)(T * K);
   w.logits = 0;
   w.h = align256((size_t)T * E * 4);
-  w.counters = w.h + align256(S * H * 4);
-  if (dtype == MOE_F32 || d == 0 || H == 0) {
-    w.total = w.counters;
-    return w;
+  w.slots = w.h + align256(S * H * 4);
+  w.counters = w.slots + align256(S * 8);
+  w.part = w.counters;
+  int parts = 1;
+  if (dtype != MOE_F32 && d > 0 && H > 0) {
+    // experts that the tokens are expected to touch when each picks K of E
+    const double touched = K >= E ? (double)E : E * (1.0 - pow(1.0 - (double)K / E, (double)T));
+    w.split0 = few_split0(touched, H, d);
+    w.split1 = few_split1(touched, d, H);
+    parts = w.split1.parts;
+    w.max_units = few::plan_max_units((int)S, (int)E, few_nb(T));
+    w.num_counters = 2 + w.max_units;
+    w.part = w.counters + align256((size_t)w.num_counters * 4);
   }
-  // experts that the tokens are expected to touch when each picks K of E
-  const double touched = K >= E ? (double)E : E * (1.0 - pow(1.0 - (double)K / E, (double)T));
-  w.split0 = few_split0(touched, H, d);
-  w.split1 = few_split1(touched, d, H);
-  w.max_units = few::plan_max_units((int)S, (int)E, few_nb(T));
-  w.num_counters = 2 + w.max_units;
-  w.part = w.counters + align256((size_t)w.num_counters * 4);
-  w.total = w.part + align256((size_t)w.split1.parts * S * d * 4);
+  w.total = w.part + align256((size_t)parts * S * d * 4);
   return w;
 }
 
@@ -190,31 +193,23 @@ static int few_router_launch(const FewArgs& a, float* logits, int* zero, int num
   return MOE_OK;
 }
 
-template <typename T>
-static int few_simt_launch(const FewArgs& a, const few::Routing& r, float* h) {
-  const int S = r.num_tokens * r.K;
-  const int plan = few::plan_bytes(S, r.E, few::kSimtRows);
-  const bool vec = (a.d * sizeof(T)) % 16 == 0 && (a.hidden * sizeof(T)) % 16 == 0 &&
-                   aligned16(a.x) && aligned16(a.w_gate) && aligned16(a.w_up) && aligned16(a.w_down);
-  const int sms = num_sms(current_device());
-  const int64_t gu = (int64_t)few::plan_max_units(S, r.E, few::kSimtRows) * a.hidden;
-  const dim3 grid_gu((unsigned)std::max<int64_t>(1, std::min<int64_t>((gu + 7) / 8, 4 * sms)));
-  const dim3 grid_dn((unsigned)std::min<int64_t>((a.d + 7) / 8, 4 * sms));
-  const size_t smem_dn = plan + (size_t)8 * r.num_tokens * 4;
+template <typename T, bool VEC>
+static int few_simt_launch(const FewArgs& a, const few::Routing& r, const FewWorkspace& w) {
+  uint8_t* ws = (uint8_t*)a.workspace;
+  float *h = (float*)(ws + w.h), *o = (float*)(ws + w.part), *slot_w = (float*)(ws + w.slots);
+  int* slot_pos = (int*)(slot_w + r.num_tokens * r.K);
+  const int S = r.num_tokens * r.K, plan = few::plan_bytes(S, r.E, few::kSimtRows);
+  const int64_t units = few::plan_max_units(S, r.E, few::kSimtRows), most = 4 * num_sms(current_device());
+  const auto grid = [&](int64_t warps) { return dim3((unsigned)std::max<int64_t>(1, std::min((warps + 7) / 8, most))); };
   const T *x = (const T*)a.x, *wg = (const T*)a.w_gate, *wu = (const T*)a.w_up, *wd = (const T*)a.w_down;
-  T* y = (T*)a.out;
   const int d = (int)a.d, H = (int)a.hidden;
-  if (vec) {
-    MOE_CUDA_CHECK(launch_pdl(few::gate_up_simt_kernel<T, true>, grid_gu, dim3(256), plan, a.stream,
-                              x, wg, wu, h, r, d, H));
-    MOE_CUDA_CHECK(launch_pdl(few::down_simt_kernel<T, true>, grid_dn, dim3(256), smem_dn, a.stream,
-                              (const float*)h, wd, y, r, d, H));
-  } else {
-    MOE_CUDA_CHECK(launch_pdl(few::gate_up_simt_kernel<T, false>, grid_gu, dim3(256), plan, a.stream,
-                              x, wg, wu, h, r, d, H));
-    MOE_CUDA_CHECK(launch_pdl(few::down_simt_kernel<T, false>, grid_dn, dim3(256), smem_dn, a.stream,
-                              (const float*)h, wd, y, r, d, H));
-  }
+  MOE_CUDA_CHECK(launch_pdl(few::gate_up_simt_kernel<T, VEC>, grid(units * H), dim3(256), plan, a.stream, x,
+                            wg, wu, h, slot_pos, slot_w, r, d, H));
+  MOE_CUDA_CHECK(launch_pdl(few::down_simt_kernel<T, VEC>, grid(units * d), dim3(256), plan, a.stream,
+                            (const float*)h, wd, o, r, d, H));
+  MOE_CUDA_CHECK(launch_pdl(few::combine_simt_kernel<T>, grid((int64_t)r.num_tokens * d / 32 + 1), dim3(256), 0,
+                            a.stream, (const float*)o, (const int*)slot_pos, (const float*)slot_w, (T*)a.out,
+                            r.num_tokens, r.K, d));
   return MOE_OK;
 }
 
@@ -323,7 +318,11 @@ static int few_tokens_run(const FewArgs& a) {
     }
   }
   if (tc) return few_tc_launch(a, r, w);
-  return MOE_DISPATCH_DTYPE(a.dtype, T, [&] { return few_simt_launch<T>(a, r, (float*)(ws + w.h)); });
+  return MOE_DISPATCH_DTYPE(a.dtype, T, [&] {
+    const bool vec = (a.d * sizeof(T)) % 16 == 0 && (a.hidden * sizeof(T)) % 16 == 0 && aligned16(a.x) &&
+                     aligned16(a.w_gate) && aligned16(a.w_up) && aligned16(a.w_down);
+    return vec ? few_simt_launch<T, true>(a, r, w) : few_simt_launch<T, false>(a, r, w);
+  });
 }
 
 }  // namespace moe

@@ -282,8 +282,9 @@ __device__ __forceinline__ void build_plan(const Plan& p, const Routing& r, int 
 }
 
 // ------------------------------------------------------------------------- CUDA cores
-// One warp per weight row (and per unit of up to 8 rows of activations), exact fp32 FMAs; h is
-// kept in fp32.  Bound by the weight stream at one or two rows per expert.
+// One warp per weight row (and per unit of up to 8 rows of activations), exact fp32 FMAs; h and the
+// experts' outputs are kept in fp32.  Three launches: gate and up, down, combine.  Bound by the
+// weight stream at one or two rows per expert, by loads in flight at more.
 constexpr int kSimtRows = 8;
 
 template <typename T, bool VEC>
@@ -297,10 +298,78 @@ __device__ __forceinline__ void load_vec(const T* p, float* v) {
   }
 }
 
+// acc[q] += <w, x[q]> over k for this lane (V elements at a time); rows past a unit repeat its first,
+// so that no load waits for a branch.
+template <typename T, bool VEC, int NW>
+__device__ __forceinline__ void lane_dots(const T* const (&w)[NW], const T* const (&x)[kSimtRows], int K,
+                                          int lane, float (&acc)[NW][kSimtRows]) {
+  constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
+#pragma unroll 2
+  for (int k = lane * V; k < K; k += 32 * V) {
+    float wv[NW][V];
+#pragma unroll
+    for (int i = 0; i < NW; ++i) load_vec<T, VEC>(w[i] + k, wv[i]);
+#pragma unroll
+    for (int q = 0; q < kSimtRows; ++q) {
+      float xv[V];
+      load_vec<T, VEC>(x[q] + k, xv);
+#pragma unroll
+      for (int i = 0; i < NW; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[i][q] = fmaf(wv[i][j], xv[j], acc[i][q]);
+    }
+  }
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// h[pos, j]; block 0 also leaves each slot's position (-1: dropped) and weight for the combine.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
 gate_up_simt_kernel(const T* __restrict__ x, const T* __restrict__ wg, const T* __restrict__ wu,
-                    float* __restrict__ h, Routing r, int d, int H) {
+                    float* h, int* slot_pos, float* slot_w, Routing r, int d, int H) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int S = r.num_tokens * r.K;
+  const Plan p = plan_view(smem, S, r.E, kSimtRows);
+  pdl_launch_dependents();
+  pdl_wait();
+  build_plan(p, r, kSimtRows);
+  if (blockIdx.x == 0)
+    for (int s = threadIdx.x; s < S; s += blockDim.x) {
+      slot_pos[s] = p.pos[s];
+      slot_w[s] = p.w[s];
+    }
+  const int lane = threadIdx.x & 31;
+  const int warps = gridDim.x * (blockDim.x >> 5);
+  const int64_t total = (int64_t)*p.num_units * H;
+  for (int64_t i = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < total; i += warps) {
+    const int u = (int)(i / H), j = (int)(i - (int64_t)u * H);
+    const int n = p.unit_n[u], pos0 = p.unit_pos[u];
+    const int64_t row = ((int64_t)p.unit_e[u] * H + j) * d;
+    const T* const w[2] = {wg + row, wu + row};
+    const T* xr[kSimtRows];
+#pragma unroll
+    for (int q = 0; q < kSimtRows; ++q) xr[q] = x + (int64_t)(p.slot[pos0 + (q < n ? q : 0)] / r.K) * d;
+    float acc[2][kSimtRows] = {};
+    lane_dots<T, VEC, 2>(w, xr, d, lane, acc);
+    float g = 0.f, v = 0.f;
+#pragma unroll
+    for (int q = 0; q < kSimtRows; ++q) {
+      const float a = warp_sum(acc[0][q]), b = warp_sum(acc[1][q]);
+      if (lane == q) { g = a; v = b; }
+    }
+    if (lane < n) h[(int64_t)(pos0 + lane) * H + j] = g * sigmoid_f32(g) * v;
+  }
+}
+
+// o[pos, n] = h[pos] . Wd[e][n].  h is fp32, so the weights are widened as they are loaded.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+down_simt_kernel(const float* h, const T* __restrict__ wd, float* o, Routing r, int d, int H) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int S = r.num_tokens * r.K;
   const Plan p = plan_view(smem, S, r.E, kSimtRows);
@@ -310,93 +379,59 @@ gate_up_simt_kernel(const T* __restrict__ x, const T* __restrict__ wg, const T* 
   constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
   const int lane = threadIdx.x & 31;
   const int warps = gridDim.x * (blockDim.x >> 5);
-  const int64_t total = (int64_t)*p.num_units * H;
+  const int64_t total = (int64_t)*p.num_units * d;
   for (int64_t i = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < total; i += warps) {
-    const int u = (int)(i / H), j = (int)(i % H);
+    const int u = (int)(i / d), col = (int)(i - (int64_t)u * d);
     const int n = p.unit_n[u], pos0 = p.unit_pos[u];
-    const int64_t row = ((int64_t)p.unit_e[u] * H + j) * d;
-    const T* xr[kSimtRows];
+    const T* w = wd + ((int64_t)p.unit_e[u] * d + col) * H;
+    const float* hr[kSimtRows];
 #pragma unroll
-    for (int q = 0; q < kSimtRows; ++q) xr[q] = x + (int64_t)(p.slot[pos0 + (q < n ? q : 0)] / r.K) * d;
-    float ag[kSimtRows] = {}, au[kSimtRows] = {};
-    for (int k = lane * V; k < d; k += 32 * V) {
-      float g[V], v[V];
-      load_vec<T, VEC>(wg + row + k, g);
-      load_vec<T, VEC>(wu + row + k, v);
+    for (int q = 0; q < kSimtRows; ++q) hr[q] = h + (int64_t)(pos0 + (q < n ? q : 0)) * H;
+    float acc[kSimtRows] = {};
+#pragma unroll 2
+    for (int k = lane * V; k < H; k += 32 * V) {
+      float wv[V];
+      load_vec<T, VEC>(w + k, wv);
 #pragma unroll
       for (int q = 0; q < kSimtRows; ++q) {
-        if (q >= n) break;
-        float xv[V];
-        load_vec<T, VEC>(xr[q] + k, xv);
+        float hv[V];
+        if constexpr (VEC) {
 #pragma unroll
-        for (int c = 0; c < V; ++c) {
-          ag[q] = fmaf(g[c], xv[c], ag[q]);
-          au[q] = fmaf(v[c], xv[c], au[q]);
+          for (int j = 0; j < V; j += 4)
+            *reinterpret_cast<float4*>(hv + j) = *reinterpret_cast<const float4*>(hr[q] + k + j);
+        } else {
+          hv[0] = hr[q][k];
         }
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[q] = fmaf(wv[j], hv[j], acc[q]);
       }
     }
+    float mine = 0.f;
 #pragma unroll
     for (int q = 0; q < kSimtRows; ++q) {
-      if (q >= n) break;
-      float a = ag[q], b = au[q];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        b += __shfl_xor_sync(0xffffffffu, b, o);
-      }
-      if (lane == 0) h[(int64_t)(pos0 + q) * H + j] = a * sigmoid_f32(a) * b;
+      const float a = warp_sum(acc[q]);
+      if (lane == q) mine = a;
     }
+    if (lane < n) o[(int64_t)(pos0 + lane) * d + col] = mine;
   }
 }
 
-// y[t, n] = sum over the experts in ascending order of p * (h . Wd[e][n]); one warp per n.
-template <typename T, bool VEC>
+// y[t] = sum over t's slots, in order, of their weight times their row of o.
+template <typename T>
 __global__ void __launch_bounds__(256)
-down_simt_kernel(const float* __restrict__ h, const T* __restrict__ wd, T* __restrict__ y, Routing r,
-                 int d, int H) {
-  extern __shared__ __align__(16) uint8_t smem[];
-  const int S = r.num_tokens * r.K;
-  const Plan p = plan_view(smem, S, r.E, kSimtRows);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float* acc = reinterpret_cast<float*>(smem + plan_bytes(S, r.E, kSimtRows)) + warp * r.num_tokens;
+combine_simt_kernel(const float* o, const int* slot_pos, const float* slot_w, T* __restrict__ y,
+                    int num_tokens, int K, int d) {
   pdl_wait();
-  build_plan(p, r, kSimtRows);
-  constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
-  const int warps = gridDim.x * (blockDim.x >> 5);
-  const int units = *p.num_units;
-  for (int n0 = blockIdx.x * (blockDim.x >> 5) + warp; n0 < d; n0 += warps) {
-    for (int t = lane; t < r.num_tokens; t += 32) acc[t] = 0.f;
-    __syncwarp();
-    for (int u = 0; u < units; ++u) {
-      const int n = p.unit_n[u], pos0 = p.unit_pos[u];
-      const T* row = wd + ((int64_t)p.unit_e[u] * d + n0) * H;
-      float a[kSimtRows] = {};
-      for (int k = lane * V; k < H; k += 32 * V) {
-        float wv[V];
-        load_vec<T, VEC>(row + k, wv);
-#pragma unroll
-        for (int q = 0; q < kSimtRows; ++q) {
-          if (q >= n) break;
-          const float* hr = h + (int64_t)(pos0 + q) * H + k;
-#pragma unroll
-          for (int c = 0; c < V; ++c) a[q] = fmaf(wv[c], __ldcg(hr + c), a[q]);
-        }
-      }
-#pragma unroll
-      for (int q = 0; q < kSimtRows; ++q) {
-        if (q >= n) break;
-        float v = a[q];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == 0) {
-          const int s = p.slot[pos0 + q];
-          acc[s / r.K] += p.w[s] * v;
-        }
-      }
+  const int64_t total = (int64_t)num_tokens * d;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int t = (int)(i / d), col = (int)(i - (int64_t)t * d);
+    float acc = 0.f;
+    for (int k = 0; k < K; ++k) {
+      const int pos = slot_pos[t * K + k];
+      if (pos >= 0) acc = fmaf(slot_w[t * K + k], o[(int64_t)pos * d + col], acc);
     }
-    __syncwarp();
-    for (int t = lane; t < r.num_tokens; t += 32) y[(int64_t)t * d + n0] = from_f32<T>(acc[t]);
-    __syncwarp();
+    y[i] = from_f32<T>(acc);
   }
 }
 

@@ -68,7 +68,8 @@ __device__ __forceinline__ float act_bwd(float z) {
   }
   if constexpr (ACT == MOE_ACT_SILU) {
     const float s = FAST ? __fdividef(1.f, 1.f + __expf(-z)) : sigmoid_f32(z);
-    return s == 0.f ? 0.f : s * (1.f + z * (1.f - s));
+    // s is 0 far below -100; the bound keeps 0 * inf out at z = -inf
+    return s * (1.f + fmaxf(z, -100.f) * (1.f - s));
   }
   return 1.f;
 }

@@ -76,7 +76,7 @@ static FewSplit few_split1(double units, int64_t d, int64_t H) {
 // the rate an SM reads L2 (50), and its MMAs (75 each, and up to 250 a stage); a chunk costs
 // about 1000 more, and adding parts up at the end 6000 and a pass over them.  Heights that fill
 // 1 to 4 waves of the SMs are compared, and whole ones.  (37 rows, K = 7168, N = 4096: picks 148
-// chunks of 111 rows and a quarter of K, 26.7 us; 128 rows 30 us, 128 rows and a fifth 37 us.)
+// chunks of 111 rows and a quarter of K, 26.7 us; 128 rows and a third 33 us, and a fifth 37 us.)
 static FewSplit few_split_linear(double units, int64_t rows, int64_t KB, double n) {
   const double sms = num_sms(current_device());
   double best = 1e30;

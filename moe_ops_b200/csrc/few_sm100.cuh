@@ -4,7 +4,7 @@
 // With n rows (1 to 64) per weight matrix the product does 2 n flops per 2-byte weight, far
 // below the ridge: the kernel is a stream over the weights and everything else hides behind it.
 // The weights are the MMA's A operand (M = 128 weight rows) and the activations its B operand
-// (N = n rounded up to 16).  A tcgen05.mma takes about 80 cycles here however small it is (the
+// (N = n rounded up to 16).  A tcgen05.mma takes its thread about 80 cycles however small it is (the
 // same measured for M = 64 and 128, N = 16 to 112), 51 bytes of weights per cycle when its 128
 // rows are all in use, against the 26 that an SM's share of HBM delivers: M tiles should be full.
 // (With the roles swapped, 256 weight rows as N, an instruction covers twice the weights but
@@ -22,9 +22,7 @@
 //
 // Work split.  The host picks each phase's tile height and the number of chunks that a tile's
 // contraction is cut into (`parts`) from the sizes alone, so that the chunks fill whole waves of
-// the SMs (results depend on neither routing nor timing).  Each chunk starts its contraction at
-// another block, so that SMs that start together do not all read the same columns of rows that
-// lie a power of two apart (1 token, d = 4096: 120 -> 112 us).  Phase 0 is never cut: adding up
+// the SMs (results depend on neither routing nor timing).  Phase 0 is never cut: adding up
 // parts of h before phase 1 costs a fence, an atomic and a second pass per cut, and while the
 // weights saturate HBM each of these takes microseconds (6 and 5 us measured for a block's first
 // ones).  Parts of the outputs are fp32 and cost little: all are added at the end, in order.
@@ -43,8 +41,8 @@
 //   warp 1      TMEM owner and MMA issuer.
 //   warps 2-3   activations: 16-byte cp.async into the same swizzle (rows are gathered: any
 //               token, any h row), which arrive on the stage's barrier when they land: these
-//               warps run ahead by the whole ring, as the weights do (handing stages over 3
-//               behind held the stream to 3.6 TB/s).
+//               warps run ahead by the whole ring, as the weights do (handing each stage over 3
+//               later: 32 tokens, d = 7168, E = 256, H = 2048 2019 us, so 1950 us).
 //   warps 4-7   epilogue, one accumulator lane (weight row) per thread.
 //
 // Every wait is bounded; one that gives up sets the abort flag and device error 1.
@@ -158,7 +156,7 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   // Accumulator sets: 2 M tiles x 2 accumulators of NB columns, or 4 of one M tile, which the
   // epilogue adds.  An MMA that adds to the one before it starts later (linear, 1 row, one M tile:
-  // 26.6 us with one accumulator, 24.0 us with four).
+  // 26.6 us with one accumulator, 24.6 us with four).
   constexpr int kBufs = NB == 64 ? 2 : 4;
   constexpr uint32_t kTmemCols = kBufs * 4 * NB;
   const int ST = p.stages;
@@ -264,7 +262,7 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
   // Chunk t: unit u (expert e, first row row0, n rows), weight rows from w0, blocks
   // [kb0, kb0 + len) of the contraction.
   struct Chunk {
-    int phase, u, w0, part, kb0, len, e, row0, n, turn;
+    int phase, u, w0, part, kb0, len, e, row0, n;
   };
   auto decode = [&](int t) {
     Chunk c;
@@ -277,7 +275,6 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
     c.u = tile / sh.tiles;
     c.w0 = (tile - c.u * sh.tiles) * sh.rows;
     part_range(c.phase ? KB1 : KB0, parts, c.part, c.kb0, c.len);
-    c.turn = (int)((unsigned)t * 37u % (unsigned)c.len);
     if constexpr (MODE == kMoe) {
       c.e = plan.unit_e[c.u]; c.row0 = plan.unit_pos[c.u]; c.n = plan.unit_n[c.u];
     } else {
@@ -332,17 +329,16 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
         const bool gate_up = MODE == kMoe && !c.phase;
         const CUtensorMap* m0 = MODE == kMoe && c.phase ? &map2 : &map0;
         const auto& sh = p.shape[c.phase];
-        for (int kb = c.kb0 + c.turn, left = c.len; left > 0; left -= sh.blocks) {
+        for (int kb = c.kb0, left = c.len; left > 0; left -= sh.blocks) {
           if (!ptx::wait_bounded(ptx::smem_u32(&s.empty[stage]), parity, abort_flag, kWaitNs)) { ok = false; break; }
           const uint32_t bar = ptx::smem_u32(&s.full[stage]);
           uint32_t dst = ptx::smem_u32(smem) + stage * stage_bytes;
           const int nb = min(left, sh.blocks);
           ptx::mbar_arrive_expect_tx(bar, nb * (gate_up ? 2 : 1) * sh.rows * 128);
-          for (int j = 0; j < nb; ++j) {
+          for (int j = 0; j < nb; ++j, ++kb) {
             ptx::tma_load_3d(dst, m0, bar, kb * BK, c.w0, c.e);
             if (gate_up) ptx::tma_load_3d(dst + sh.second, &map1, bar, kb * BK, c.w0, c.e);
             dst += sh.block_bytes;
-            if (++kb == c.kb0 + c.len) kb = c.kb0;
           }
           if (++stage == ST) { stage = 0; parity ^= 1; }
         }
@@ -454,11 +450,11 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
       }
       const auto& sh = p.shape[c.phase];
       const uint32_t w_bytes = sh.blocks * sh.block_bytes;
-      for (int kb = c.kb0 + c.turn, left = c.len; left > 0; left -= sh.blocks) {
+      for (int kb = c.kb0, left = c.len; left > 0; left -= sh.blocks) {
         if (!warp_wait(s.empty[stage], parity)) { ok = false; break; }
         uint32_t dst = ptx::smem_u32(smem) + stage * stage_bytes + w_bytes;
         const int nb = min(left, sh.blocks);
-        for (int j = 0; j < nb; ++j, dst += NB * 128) {
+        for (int j = 0; j < nb; ++j, ++kb, dst += NB * 128) {
           const bool in = kb * BK + c16 * 8 < cols;  // cols is a multiple of 8
 #pragma unroll
           for (int i = 0; i < NB / 8; ++i) {
@@ -467,7 +463,6 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
               ptx::cp_async16(dst + r * 128 + ((c16 ^ (r & 7)) << 4),
                               rows[i] + (in ? kb * BK : -(c16 * 8)), in ? 16u : 0u);
           }
-          if (++kb == c.kb0 + c.len) kb = c.kb0;
         }
         ptx::cp_async_arrive(ptx::smem_u32(&s.full[stage]));
         if (++stage == ST) { stage = 0; parity ^= 1; }

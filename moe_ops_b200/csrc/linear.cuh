@@ -118,22 +118,21 @@ linear_rows_kernel(const T* __restrict__ A, const T* __restrict__ B, const Linea
 // column sums of dz taken from its fp32 values before they are rounded.  A block owns
 // kDzRows consecutive rows of one group and kDzCols columns; its column sums go to
 // partial[chunk, n] and dbias_kernel adds the chunks of a group in order, so the result does
-// not depend on the order blocks run in.  HBM-bound: 2 reads + 1 write of m * n elements.
-constexpr int kDzRows = 128;
+// not depend on the order blocks run in.  HBM-bound: 2 reads + 1 write of m * n elements (bf16,
+// 4099 x 7168: 27 us at the copy rate, 41 us for relu, 43 to 52 us for the others, and 8 to 10 us
+// with the bias gradient's second launch).  The activation is a template parameter and registers
+// are capped at 64: four rows' loads in flight per thread, four blocks per SM (one kernel for all
+// activations: silu 78 us).
+constexpr int kDzRows = 64;
 constexpr int kDzThreads = 256;
-
-template <typename T, int V>
-struct Pack {
-  T v[V];
-};
 
 // V = elements of a thread's column group (8 for 16-bit and 4 for fp32 when rows are 16-byte
 // multiples, else 1); blockDim = (columns / V = 32, 8 rows).
-template <typename T, int V>
-__global__ void __launch_bounds__(kDzThreads)
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kDzThreads, 4)
 dz_kernel(const T* __restrict__ dout, const T* __restrict__ z, T* __restrict__ dz,
           float* __restrict__ partial, const int32_t* __restrict__ offsets, int plus_one, int E,
-          int64_t m, int64_t N, int act) {
+          int64_t m, int64_t N) {
   extern __shared__ int prefix[];
   __shared__ float red[8][32 * V + 1];
   row_chunks(prefix, offsets, plus_one, E, m, kDzRows);
@@ -147,24 +146,27 @@ dz_kernel(const T* __restrict__ dout, const T* __restrict__ z, T* __restrict__ d
     const int64_t r1 = min(r0 + kDzRows, gr.start + gr.rows);
     float sum[V] = {};
     if (n < N) {
-      MOE_SWITCH_ACT(act, ACT, {
-        _Pragma("unroll 4") for (int64_t r = r0 + ty; r < r1; r += 8) {
-          const int64_t at = r * N + n;
-          using P = Pack<T, V>;
-          union { P p; typename std::conditional<V * sizeof(T) == 16, uint4, T>::type u; } d, zz, o;
-          d.u = __ldg(reinterpret_cast<const decltype(d.u)*>(dout + at));
-          if constexpr (ACT != MOE_ACT_NONE) zz.u = __ldg(reinterpret_cast<const decltype(d.u)*>(z + at));
-          _Pragma("unroll") for (int j = 0; j < V; ++j) {
-            float v = to_f32(d.p.v[j]);
-            if constexpr (ACT != MOE_ACT_NONE) {
-              v *= act_bwd<ACT, sizeof(T) == 2>(to_f32(zz.p.v[j]));
-              o.p.v[j] = from_f32<T>(v);
-            }
-            sum[j] += v;
+      union Vec {
+        typename std::conditional<V * sizeof(T) == 16, uint4, T>::type u;
+        T v[V];
+      };
+#pragma unroll 4
+      for (int64_t r = r0 + ty; r < r1; r += 8) {
+        const int64_t at = r * N + n;
+        Vec d, zz, o;
+        d.u = __ldg(reinterpret_cast<const decltype(d.u)*>(dout + at));
+        if constexpr (ACT != MOE_ACT_NONE) zz.u = __ldg(reinterpret_cast<const decltype(d.u)*>(z + at));
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          float v = to_f32(d.v[j]);
+          if constexpr (ACT != MOE_ACT_NONE) {
+            v *= act_bwd<ACT, sizeof(T) == 2>(to_f32(zz.v[j]));
+            o.v[j] = from_f32<T>(v);
           }
-          if constexpr (ACT != MOE_ACT_NONE) *reinterpret_cast<decltype(d.u)*>(dz + at) = o.u;
+          sum[j] += v;
         }
-      })
+        if constexpr (ACT != MOE_ACT_NONE) *reinterpret_cast<decltype(d.u)*>(dz + at) = o.u;
+      }
     }
     if (partial) {
       __syncthreads();

@@ -237,12 +237,14 @@ static int act_bwd(const void* grad_out, const void* preact, void* dz, void* gra
     constexpr int V = 16 / (int)sizeof(T);
     const int cols = 32 * (vec ? V : 1);
     const dim3 grid((unsigned)((n + cols - 1) / cols), (unsigned)std::min<int64_t>(chunks, 32768));
-    if (vec)
-      dz_kernel<T, V><<<grid, kDzThreads, smem, s>>>((const T*)grad_out, (const T*)preact, (T*)dz, partial,
-                                                     offsets, plus_one, E, m, n, activation);
-    else
-      dz_kernel<T, 1><<<grid, kDzThreads, smem, s>>>((const T*)grad_out, (const T*)preact, (T*)dz, partial,
-                                                     offsets, plus_one, E, m, n, activation);
+    MOE_SWITCH_ACT(activation, ACT, {
+      if (vec)
+        dz_kernel<T, V, ACT><<<grid, kDzThreads, smem, s>>>(
+            (const T*)grad_out, (const T*)preact, (T*)dz, partial, offsets, plus_one, E, m, n);
+      else
+        dz_kernel<T, 1, ACT><<<grid, kDzThreads, smem, s>>>(
+            (const T*)grad_out, (const T*)preact, (T*)dz, partial, offsets, plus_one, E, m, n);
+    })
     MOE_LAUNCH_CHECK();
     return (int)MOE_OK;
   });

@@ -37,15 +37,21 @@ struct LinearArgs {
   cudaStream_t stream;
 };
 
-// Rows per group up to which a warp per weight row is taken over 64 x 64 tiles (which need at least
-// a slice of 32 in K per step, and 64 rows to be full).
-constexpr int kLinearWarpRows = 16;
+// A warp per weight row is taken over 64 x 64 tiles, which run K / 32 slices one after the other at
+// about 2 us each while few blocks share an SM, up to 64 rows a group or 24 tiles and 2^26
+// multiplications.  fp32, tiles / warps in us: 32 x 1024 x 1024 70 / 14, 64 x 1024 x 1024 70 / 24,
+// 64 x 256 x 300 24 / 8, 333 x 257 x 130 25 / 12, 700 x 300 x 300 27 / 35, 1000 x 64 x 1000 14 / 91,
+// 834 rows of 20 groups x 725 x 663 110 / 291.
+static bool linear_warps_win(int64_t m, int64_t n, int64_t k, int E) {
+  return (double)m * (double)n * (double)k <= (double)(1 << 26) &&
+         (m <= 64ll * E || (m + simt::TM - 1) / simt::TM * ((n + simt::TN - 1) / simt::TN) <= 24);
+}
 
 template <typename T>
 static int linear_simt(const LinearArgs& a) {
   const LinearEpilogue<T> epi{(T*)a.out, (T*)a.preact, (const T*)a.bias, (const T*)a.residual, a.act};
-  if (!a.b_mn && a.E <= gmm::kMaxGroups && a.m <= (int64_t)kLinearWarpRows * a.E && a.n < (1 << 30) &&
-      a.k < (1 << 30)) {
+  if (!a.b_mn && a.E <= gmm::kMaxGroups && a.n < (1 << 30) && a.k < (1 << 30) &&
+      linear_warps_win(a.m, a.n, a.k, a.E)) {
     const int64_t warps = ((a.m + kWarpRows - 1) / kWarpRows + (a.offsets ? a.E : 0)) * a.n;
     const unsigned grid = (unsigned)std::min<int64_t>((warps + 7) / 8, 8 * num_sms(current_device()));
     const size_t smem = (size_t)(a.E + 1) * 4;

@@ -32,7 +32,7 @@
 // without waiting for anyone, and at the very end for all chunks: the kernel makes progress
 // whatever share of its blocks is resident.  The weight producer never waits for h, so the ring
 // fills with Wd while the last h tiles are finished; phase 1 goes unit by unit in phase 0's
-// order.  A finished h tile is published (fence and atomic) only when the next chunk's
+// order.  A finished h tile is published (barrier and releasing atomic) only when the next chunk's
 // accumulator is ready or there is nothing else to do, and output chunks are counted once per
 // block.
 //
@@ -478,10 +478,11 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
     Chunk c;
     int held_unit = -1;  // kMoe: the unit of an h tile that is stored but not published
     int outputs = 0;     // chunks of the outputs that this block has stored
+    // The barrier orders every thread's stores before the lead's release, which is cumulative over
+    // them; a fence of each thread before the barrier would not be part of that release.
     auto publish = [&]() {
-      ptx::fence_acq_rel_gpu();
       ptx::named_barrier(1, 128);
-      if (lead) ptx::red_add_gpu(c_done + held_unit, 1);
+      if (lead) ptx::red_add_release_gpu(c_done + held_unit, 1);
       held_unit = -1;
     };
     // The four warps meet at barriers, so each wait's outcome is agreed on by all of them.
@@ -551,9 +552,8 @@ few_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUt
     // Abandoned work is not published (the wait that gave up has set the abort flag).
     if (MODE == kMoe && held_unit >= 0 && ptx::named_barrier_all(1, 128, *abort_flag == 0)) publish();
     if (tickets) {
-      ptx::fence_acq_rel_gpu();
       ptx::named_barrier(1, 128);
-      if (lead && outputs > 0) ptx::red_add_gpu(c_out, outputs);
+      if (lead && outputs > 0) ptx::red_add_release_gpu(c_out, outputs);
     }
   }
 

@@ -10,6 +10,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_NAME = "libmoe_b200.so"
 LIB_PATH = os.environ.get("MOE_B200_LIB") or os.path.join(
@@ -173,6 +174,36 @@ def on_device(t: torch.Tensor):
 def raw_stream(t: torch.Tensor) -> int:
     """stream_of without building a Stream object."""
     return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
+def direct(*tensors: torch.Tensor | None) -> bool:
+    """Whether a call on these tensors may go to the library at once.
+
+    False while something records or transforms calls (jit.trace, make_fx and other dispatch
+    modes, torch.compile, functorch, forward-mode differentiation) or a tensor is of another
+    class (fake, distributed, ...): such a call goes through the registered op, which those
+    see.  Under a microsecond, a tenth of a registered op's own cost.
+    """
+    if (torch.compiler.is_compiling() or torch._C._get_tracing_state() is not None
+            or torch._C._len_torch_dispatch_stack() > 0
+            or torch._C._functorch.peek_interpreter_stack() is not None
+            or forward_ad._current_level >= 0):
+        return False
+    for t in tensors:
+        if t is not None and type(t) not in _PLAIN:
+            return False
+    return True
+
+
+def refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
+    """Raises where an input carries a forward-mode tangent, which the kernels would drop."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 def check(status: int, what: str) -> None:

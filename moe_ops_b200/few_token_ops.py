@@ -12,9 +12,10 @@ Two ways it differs from the assembled layer, both towards fewer roundings: the 
 logits stay in fp32 (the assembled layer rounds them to x's dtype, so close logits may rank
 differently), and gate, up and the experts' outputs are never rounded to 16 bits.
 
-Forward only: the calls refuse inputs that require a gradient while grad mode is on.  They are
-plain functions over the C ABI (no ``torch.library`` op), because at one token the host's
-part of a call is of the order of the kernel's time.
+Forward only: the calls refuse inputs that require a gradient while grad mode is on, and inputs
+with a forward-mode tangent.  Eager calls go to the C ABI at once, because at one token the host's
+part of a call is of the order of the kernel's time; under torch's tracers and torch.compile they go
+through the registered ops ``moeb200::few_tokens`` and ``moeb200::few_experts``.
 """
 from __future__ import annotations
 
@@ -78,6 +79,34 @@ def _run(x, route, w_gate, w_up, w_down, dims, K: int, given: bool) -> torch.Ten
     return y
 
 
+@torch.library.custom_op("moeb200::few_tokens", mutates_args=())
+def few_tokens(x: torch.Tensor, w_router: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
+               w_down: torch.Tensor, top_k: int, router_bias: Optional[torch.Tensor]) -> torch.Tensor:
+    """moe_few_tokens for checked arguments; router_bias in fp32."""
+    route = (w_router.contiguous(), None if router_bias is None else router_bias.contiguous())
+    E, H, d = w_gate.shape
+    return _run(x, route, w_gate, w_up, w_down, (x.shape[0], d, E, H), top_k, False)
+
+
+@torch.library.custom_op("moeb200::few_experts", mutates_args=())
+def few_experts(x: torch.Tensor, weights: torch.Tensor, indices: torch.Tensor, w_gate: torch.Tensor,
+                w_up: torch.Tensor, w_down: torch.Tensor) -> torch.Tensor:
+    """moe_few_experts for checked arguments; weights in fp32, indices in int32."""
+    E, H, d = w_gate.shape
+    return _run(x, (weights.contiguous(), indices.contiguous()), w_gate, w_up, w_down,
+                (x.shape[0], d, E, H), weights.shape[1], True)
+
+
+@few_tokens.register_fake
+def _(x, w_router, w_gate, w_up, w_down, top_k, router_bias):
+    return x.new_empty(x.shape)
+
+
+@few_experts.register_fake
+def _(x, weights, indices, w_gate, w_up, w_down):
+    return x.new_empty(x.shape)
+
+
 def moe_few_tokens(x: torch.Tensor, w_router: torch.Tensor, w_gate: torch.Tensor,
                    w_up: torch.Tensor, w_down: torch.Tensor, top_k: int,
                    router_bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -95,6 +124,7 @@ def moe_few_tokens(x: torch.Tensor, w_router: torch.Tensor, w_gate: torch.Tensor
     """
     T, d, E, H = dims = _check_experts(x, w_gate, w_up, w_down)
     _lib.require_cuda(w_router, router_bias)
+    given_bias = router_bias
     if w_router.shape != (E, d) or w_router.dtype != x.dtype or w_router.device != x.device:
         raise ValueError(f"w_router must be [{E}, {d}] of x's dtype and device")
     if not 0 < top_k <= min(E, MAX_TOPK):
@@ -106,6 +136,9 @@ def moe_few_tokens(x: torch.Tensor, w_router: torch.Tensor, w_gate: torch.Tensor
     _no_grad_only(x, w_router, w_gate, w_up, w_down)
     if T == 0:
         return torch.empty_like(x)
+    if not _lib.direct(x, w_router, w_gate, w_up, w_down, router_bias):
+        _lib.refuse_tangents("moe_few_tokens", x, w_router, w_gate, w_up, w_down, given_bias)
+        return torch.ops.moeb200.few_tokens(x, w_router, w_gate, w_up, w_down, top_k, router_bias)
     return _run(x, (w_router.contiguous(), router_bias), w_gate, w_up, w_down, dims, top_k, False)
 
 
@@ -134,6 +167,9 @@ def moe_few_experts(x: torch.Tensor, weights: torch.Tensor, indices: torch.Tenso
     if indices.dtype == torch.int64:
         # out-of-range values stay out of range in 32 bits
         indices = indices.clamp(-1, E).to(torch.int32)
+    if not _lib.direct(x, weights, indices, w_gate, w_up, w_down):
+        _lib.refuse_tangents("moe_few_experts", x, weights, w_gate, w_up, w_down)
+        return torch.ops.moeb200.few_experts(x, weights.float(), indices, w_gate, w_up, w_down)
     route = (weights.float().contiguous(), indices.contiguous())
     return _run(x, route, w_gate, w_up, w_down, dims, K, True)
 

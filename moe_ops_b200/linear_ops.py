@@ -18,8 +18,10 @@ wgrad GEMMs.  The residual's gradient is dy itself.
 
 Activations: "none", "relu", "gelu" (erf), "gelu_tanh", "silu".
 
-Plain functions and autograd Functions over the C ABI (no ``torch.library`` ops): for one row
-the host's part of a call is of the order of the kernel's time.
+Eager calls go to the C ABI at once: for one row the host's part of a call is of the order of the
+kernel's time.  Under torch's tracers, torch.compile and functorch they go through the
+registered ops ``moeb200::linear_fwd`` and ``moeb200::linear_bwd``.  There is no forward-mode
+derivative; a dual input raises.
 """
 from __future__ import annotations
 
@@ -59,6 +61,8 @@ def _workspace_bytes(m: int, n: int, k: int, E: int, trans_b: int, code: int) ->
 def _forward(x, w, bias, residual, offsets, act: int, trans_b: bool, E: int, n: int, want_z: bool):
     """x [m, k], w [E, n, k] or [E, k, n] (2-D when dense), contiguous; returns (y, z or None)."""
     m, k = x.shape
+    if _copied(x, n):
+        x, w, bias, residual = _aligned(x), _aligned(w), _aligned(bias), _aligned(residual)
     y = torch.empty((m, n), device=x.device, dtype=x.dtype)
     z = torch.empty_like(y) if want_z else None
     lib = _lib.load()
@@ -83,6 +87,8 @@ def _bwd_workspace_bytes(m: int, n: int, E: int, act: int, code: int) -> int:
 def _backward(dy, x, w, z, offsets, act: int, trans_b: bool, E: int, n: int, bias_shape, wanted):
     """(dx, dw, dbias), None where not wanted."""
     m, k = x.shape
+    if _copied(x, n):
+        x, w = _aligned(x), _aligned(w)
     dx = torch.empty_like(x) if wanted[0] else None
     dw = torch.empty_like(w) if wanted[1] else None
     db = torch.empty(bias_shape, device=x.device, dtype=x.dtype) if wanted[2] else None
@@ -100,11 +106,59 @@ def _backward(dy, x, w, z, offsets, act: int, trans_b: bool, E: int, n: int, bia
     return dx, dw, db
 
 
+def _sizes(w, trans_b: bool) -> tuple[int, int]:
+    """(E, n) of a weight [n, k] (E = 1), [E, n, k] or [E, k, n]."""
+    return (1, w.shape[0]) if w.dim() == 2 else (w.shape[0], w.shape[1 if trans_b else 2])
+
+
+@torch.library.custom_op("moeb200::linear_fwd", mutates_args=())
+def linear_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor],
+               residual: Optional[torch.Tensor], offsets: Optional[torch.Tensor], act: int,
+               trans_b: bool, want_z: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """(y, z): y = act(z) + residual, z = x . w^T + bias per row range; z is empty unless wanted."""
+    E, n = _sizes(w, trans_b)
+    x, w, bias, residual, offsets = (t if t is None else t.contiguous()
+                                     for t in (x, w, bias, residual, offsets))
+    y, z = _forward(x, w, bias, residual, offsets, act, trans_b, E, n, want_z)
+    return y, x.new_empty(0) if z is None else z
+
+
+@linear_fwd.register_fake
+def _(x, w, bias, residual, offsets, act, trans_b, want_z):
+    shape = (x.shape[0], _sizes(w, trans_b)[1])
+    return x.new_empty(shape), x.new_empty(shape if want_z else (0,))
+
+
+@torch.library.custom_op("moeb200::linear_bwd", mutates_args=())
+def linear_bwd(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, z: Optional[torch.Tensor],
+               offsets: Optional[torch.Tensor], act: int, trans_b: bool, want_x: bool, want_w: bool,
+               want_bias: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dw, dbias) of linear_fwd from its z (not read without an activation); empty where not
+    wanted."""
+    E, n = _sizes(w, trans_b)
+    dy, x, w, z, offsets = (t if t is None else t.contiguous() for t in (dy, x, w, z, offsets))
+    got = _backward(dy, x, w, z, offsets, act, trans_b, E, n, (n,) if w.dim() == 2 else (E, n),
+                    (want_x, want_w, want_bias))
+    return tuple(x.new_empty(0) if t is None else t for t in got)
+
+
+@linear_bwd.register_fake
+def _(dy, x, w, z, offsets, act, trans_b, want_x, want_w, want_bias):
+    E, n = _sizes(w, trans_b)
+    bias = (n,) if w.dim() == 2 else (E, n)
+    return (x.new_empty(x.shape if want_x else (0,)), w.new_empty(w.shape if want_w else (0,)),
+            x.new_empty(bias if want_bias else (0,)))
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, residual, offsets, act, trans_b, E, n):
-        y, z = _forward(x, w, bias, residual, offsets, act, trans_b, E, n,
-                        want_z=act != 0 and any(ctx.needs_input_grad[:3]))
+        want_z = act != 0 and any(ctx.needs_input_grad[:3])
+        if _lib.direct(x, w, bias, residual, offsets):
+            y, z = _forward(x, w, bias, residual, offsets, act, trans_b, E, n, want_z)
+        else:
+            y, z = torch.ops.moeb200.linear_fwd(x, w, bias, residual, offsets, act, trans_b, want_z)
+            z = z if want_z else None
         ctx.save_for_backward(x, w, z, offsets)
         ctx.cfg = (act, trans_b, E, n, None if bias is None else bias.shape)
         return y
@@ -116,8 +170,11 @@ class _Linear(torch.autograd.Function):
         act, trans_b, E, n, bias_shape = ctx.cfg
         wanted = ctx.needs_input_grad[:3]
         dx = dw = db = None
-        if any(wanted):
+        if any(wanted) and _lib.direct(dy, x, w, z, offsets):
             dx, dw, db = _backward(dy.contiguous(), x, w, z, offsets, act, trans_b, E, n, bias_shape, wanted)
+        elif any(wanted):
+            got = torch.ops.moeb200.linear_bwd(dy, x, w, z, offsets, act, trans_b, *wanted)
+            dx, dw, db = (t if on else None for t, on in zip(got, wanted))
         return dx, dw, db, dy if ctx.needs_input_grad[3] else None, None, None, None, None, None
 
 
@@ -126,6 +183,10 @@ class _Linear(torch.autograd.Function):
 # cores; below, the CUDA cores take them as they are.  (bf16 2000 x 1001 x 1500, forward: 58 us
 # with the copies; the CUDA cores' 21 TFLOP/s would make it 290 us.)
 _PAD_FROM = 1 << 24
+
+
+def _copied(x, n) -> bool:
+    return x.dtype != torch.float32 and x.shape[0] * n * x.shape[1] >= _PAD_FROM
 
 
 def _aligned(t):
@@ -142,12 +203,13 @@ def _padded(x, w, bias, residual, offsets, act, trans_b, E, n):
 
 
 def _apply(x, w, bias, residual, offsets, act, trans_b, E, n):
-    m, k = x.shape
-    if x.dtype != torch.float32 and m * n * k >= _PAD_FROM:
-        if n % 8 or k % 8:
-            return _padded(x, w, bias, residual, offsets, act, trans_b, E, n)
-        x, w, bias, residual = _aligned(x), _aligned(w), _aligned(bias), _aligned(residual)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias, residual)):
+    if (n % 8 or x.shape[1] % 8) and _copied(x, n):
+        return _padded(x, w, bias, residual, offsets, act, trans_b, E, n)
+    given = (x, w, bias, residual)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in given):
+        return _Linear.apply(x, w, bias, residual, offsets, act, trans_b, E, n)
+    if not _lib.direct(*given, offsets):
+        # the autograd Function refuses what it cannot differentiate (forward mode, functorch)
         return _Linear.apply(x, w, bias, residual, offsets, act, trans_b, E, n)
     return _forward(x, w, bias, residual, offsets, act, trans_b, E, n, False)[0]
 

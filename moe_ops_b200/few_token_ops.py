@@ -124,7 +124,6 @@ def moe_few_tokens(x: torch.Tensor, w_router: torch.Tensor, w_gate: torch.Tensor
     """
     T, d, E, H = dims = _check_experts(x, w_gate, w_up, w_down)
     _lib.require_cuda(w_router, router_bias)
-    given_bias = router_bias
     if w_router.shape != (E, d) or w_router.dtype != x.dtype or w_router.device != x.device:
         raise ValueError(f"w_router must be [{E}, {d}] of x's dtype and device")
     if not 0 < top_k <= min(E, MAX_TOPK):
@@ -132,12 +131,15 @@ def moe_few_tokens(x: torch.Tensor, w_router: torch.Tensor, w_gate: torch.Tensor
     if router_bias is not None:
         if router_bias.shape != (E,) or router_bias.device != x.device:
             raise ValueError(f"router_bias must be [{E}] on x's device")
-        router_bias = router_bias.detach().float().contiguous()
-    _no_grad_only(x, w_router, w_gate, w_up, w_down)
+    _no_grad_only(x, w_router, w_gate, w_up, w_down, router_bias)
     if T == 0:
         return torch.empty_like(x)
-    if not _lib.direct(x, w_router, w_gate, w_up, w_down, router_bias):
-        _lib.refuse_tangents("moe_few_tokens", x, w_router, w_gate, w_up, w_down, given_bias)
+    direct = _lib.direct(x, w_router, w_gate, w_up, w_down, router_bias)
+    if not direct:
+        _lib.refuse_tangents("moe_few_tokens", x, w_router, w_gate, w_up, w_down, router_bias)
+    if router_bias is not None:
+        router_bias = router_bias.detach().float().contiguous()
+    if not direct:
         return torch.ops.moeb200.few_tokens(x, w_router, w_gate, w_up, w_down, top_k, router_bias)
     return _run(x, (w_router.contiguous(), router_bias), w_gate, w_up, w_down, dims, top_k, False)
 

@@ -102,8 +102,8 @@ class MoELayer(torch.nn.Module):
             return False
         if self.top_k > MAX_TOPK:
             return False
-        return not torch.is_grad_enabled() or not (
-            x.requires_grad or any(p.requires_grad for p in self.parameters()))
+        learned = (x, self.router_bias, *self.parameters())
+        return not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in learned)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         out = self._routed(x)

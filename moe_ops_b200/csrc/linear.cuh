@@ -119,10 +119,11 @@ linear_rows_kernel(const T* __restrict__ A, const T* __restrict__ B, const Linea
 // kDzRows consecutive rows of one group and kDzCols columns; its column sums go to
 // partial[chunk, n] and dbias_kernel adds the chunks of a group in order, so the result does
 // not depend on the order blocks run in.  HBM-bound: 2 reads + 1 write of m * n elements (bf16,
-// 4099 x 7168: 27 us at the copy rate, 41 us for relu, 43 to 52 us for the others, and 8 to 10 us
-// with the bias gradient's second launch).  The activation is a template parameter and registers
-// are capped at 64: four rows' loads in flight per thread, four blocks per SM (one kernel for all
-// activations: silu 78 us).
+// 4099 x 7168, cold L2: 27 us at the copy rate, 49 to 51 us for relu, gelu and gelu_tanh, 59 us for
+// silu, and 10 us with the bias gradient's second launch).  The activation is a template parameter and
+// registers are capped at 64: three rows' loads in flight per thread, four blocks per SM (one kernel
+// for all activations: silu 78 us; four rows: gelu 55, silu 64 us, where silu and relu spill 40 to 52
+// bytes; two rows: gelu 66 us).  relu and silu still spill 16 to 24 bytes.
 constexpr int kDzRows = 64;
 constexpr int kDzThreads = 256;
 
@@ -150,7 +151,7 @@ dz_kernel(const T* __restrict__ dout, const T* __restrict__ z, T* __restrict__ d
         typename std::conditional<V * sizeof(T) == 16, uint4, T>::type u;
         T v[V];
       };
-#pragma unroll 4
+#pragma unroll 3
       for (int64_t r = r0 + ty; r < r1; r += 8) {
         const int64_t at = r * N + n;
         Vec d, zz, o;

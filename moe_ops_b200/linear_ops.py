@@ -152,9 +152,9 @@ def _(dy, x, w, z, offsets, act, trans_b, want_x, want_w, want_bias):
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, bias, residual, offsets, act, trans_b, E, n):
+    def forward(ctx, x, w, bias, residual, offsets, act, trans_b, E, n, direct):
         want_z = act != 0 and any(ctx.needs_input_grad[:3])
-        if _lib.direct(x, w, bias, residual, offsets):
+        if direct:
             y, z = _forward(x, w, bias, residual, offsets, act, trans_b, E, n, want_z)
         else:
             y, z = torch.ops.moeb200.linear_fwd(x, w, bias, residual, offsets, act, trans_b, want_z)
@@ -175,7 +175,7 @@ class _Linear(torch.autograd.Function):
         elif any(wanted):
             got = torch.ops.moeb200.linear_bwd(dy, x, w, z, offsets, act, trans_b, *wanted)
             dx, dw, db = (t if on else None for t, on in zip(got, wanted))
-        return dx, dw, db, dy if ctx.needs_input_grad[3] else None, None, None, None, None, None
+        return dx, dw, db, dy if ctx.needs_input_grad[3] else None, *([None] * 6)
 
 
 # 16-bit operands whose rows are not 16-byte multiples, or that start off a 16-byte boundary: from
@@ -205,12 +205,11 @@ def _padded(x, w, bias, residual, offsets, act, trans_b, E, n):
 def _apply(x, w, bias, residual, offsets, act, trans_b, E, n):
     if (n % 8 or x.shape[1] % 8) and _copied(x, n):
         return _padded(x, w, bias, residual, offsets, act, trans_b, E, n)
-    given = (x, w, bias, residual)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in given):
-        return _Linear.apply(x, w, bias, residual, offsets, act, trans_b, E, n)
-    if not _lib.direct(*given, offsets):
-        # the autograd Function refuses what it cannot differentiate (forward mode, functorch)
-        return _Linear.apply(x, w, bias, residual, offsets, act, trans_b, E, n)
+    direct = _lib.direct(x, w, bias, residual, offsets)
+    # The autograd Function refuses what it cannot differentiate (forward mode, functorch).
+    if not direct or (torch.is_grad_enabled()
+                      and any(t is not None and t.requires_grad for t in (x, w, bias, residual))):
+        return _Linear.apply(x, w, bias, residual, offsets, act, trans_b, E, n, direct)
     return _forward(x, w, bias, residual, offsets, act, trans_b, E, n, False)[0]
 
 

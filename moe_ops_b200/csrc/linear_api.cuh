@@ -37,25 +37,46 @@ struct LinearArgs {
   cudaStream_t stream;
 };
 
-// A warp per weight row is taken over 64 x 64 tiles, which run K / 32 slices one after the other at
-// about 2 us each while few blocks share an SM, up to 64 rows a group or 24 tiles and 2^26
-// multiplications.  fp32, tiles / warps in us: 32 x 1024 x 1024 70 / 14, 64 x 1024 x 1024 70 / 24,
-// 64 x 256 x 300 24 / 8, 333 x 257 x 130 25 / 12, 700 x 300 x 300 27 / 35, 1000 x 64 x 1000 14 / 91,
-// 834 rows of 20 groups x 725 x 663 110 / 291.
-static bool linear_warps_win(int64_t m, int64_t n, int64_t k, int E) {
-  return (double)m * (double)n * (double)k <= (double)(1 << 26) &&
-         (m <= 64ll * E || (m + simt::TM - 1) / simt::TM * ((n + simt::TN - 1) / simt::TN) <= 24);
+// A warp per weight row (linear_rows_kernel), or 64 x 64 tiles: the smaller of two estimates in us.
+//   warps  6 + chunks of at most 8 rows x n x (k + the joining of a row's sums) x the time of a
+//          weight, which grows with the rows of a chunk; no less than the loop's latency.
+//   tiles  8 + K / 32 slices one after the other, each as long as the blocks that an SM holds ask.
+// m rows are taken to pick their group at random.  Measured, tiles / warps in us, fp32 unless said:
+//   1 x 7168 -> 11008 655 / 169    16: 661 / 476    32: 665 / 935     (rows x k -> n)
+//   16 x 4096 -> 4096 254 / 94     32: 255 / 183    64: 256 / 351
+//   8 x 4097 -> 4097  257 / 121    24: 257 / 267    48: 259 / 638
+//   64 x 1024 -> 1024 71 / 38      128: 70 / 60     256: 70 / 108
+//   8 x 300 -> 7168   29 / 19      32: 29 / 41      333 x 257 -> 130  25 / 12
+//   256 x 7168 -> 300 442 / 256    bf16 4 x 4097 -> 4097  454 / 72    16: 460 / 178
+//   grouped, 8 x 1999 -> 2001  64: 198 / 196    128: 269 / 388;  bf16  32: 277 / 132   128: 323 / 376
+//   grouped, 64 x 999 -> 1001  16: 140 / 52     256: 326 / 232   1024: 370 / 683
+static bool linear_warps_win(int64_t m, int64_t n, int64_t k, int E, int elem_size, bool vec) {
+  const auto ceil_div = [](double a, double b) { return ceil(a / b); };
+  const double live = E <= 1 ? 1.0 : E * (1.0 - pow(1.0 - 1.0 / E, (double)m));
+  // pieces of up to `rows` rows that the groups' rows fall into
+  const auto pieces = [&](double rows) {
+    return E <= 1 ? ceil_div(m, rows) : std::max(live, m / rows + live / 2);
+  };
+  const double chunks = pieces(kWarpRows), q = std::min<double>(kWarpRows, m / chunks);
+  const double weight = vec ? 2.0 + 0.1 * q : 2.4 + 0.3 * q;  // us per 10^6
+  const double turns = k * elem_size / (32.0 * (vec ? 16 : elem_size));
+  const double warps = 6 + std::max(chunks * n * (k + (vec ? 250.0 : 100.0)) * weight * 1e-6,
+                                    turns * (0.3 + 0.08 * q));
+  const double blocks = ceil_div(pieces(simt::TM) * ceil_div(n, simt::TN), num_sms(current_device()));
+  const double slice = elem_size == 4 ? 0.7 + 1.3 * blocks : 1.5 + 1.8 * blocks;
+  return warps < 8 + ceil_div(k, simt::TK) * slice;
 }
 
 template <typename T>
 static int linear_simt(const LinearArgs& a) {
   const LinearEpilogue<T> epi{(T*)a.out, (T*)a.preact, (const T*)a.bias, (const T*)a.residual, a.act};
+  const bool vec = (a.k * sizeof(T)) % 16 == 0 && aligned16(a.A) && aligned16(a.B);
   if (!a.b_mn && a.E <= gmm::kMaxGroups && a.n < (1 << 30) && a.k < (1 << 30) &&
-      linear_warps_win(a.m, a.n, a.k, a.E)) {
+      linear_warps_win(a.m, a.n, a.k, a.E, sizeof(T), vec)) {
     const int64_t warps = ((a.m + kWarpRows - 1) / kWarpRows + (a.offsets ? a.E : 0)) * a.n;
     const unsigned grid = (unsigned)std::min<int64_t>((warps + 7) / 8, 8 * num_sms(current_device()));
     const size_t smem = (size_t)(a.E + 1) * 4;
-    if ((a.k * sizeof(T)) % 16 == 0 && aligned16(a.A) && aligned16(a.B))
+    if (vec)
       linear_rows_kernel<T, true><<<grid, 256, smem, a.stream>>>(
           (const T*)a.A, (const T*)a.B, epi, a.offsets, a.plus_one, a.E, a.m, (int)a.n, (int)a.k);
     else

@@ -61,8 +61,10 @@ def _workspace_bytes(m: int, n: int, k: int, E: int, trans_b: int, code: int) ->
 def _forward(x, w, bias, residual, offsets, act: int, trans_b: bool, E: int, n: int, want_z: bool):
     """x [m, k], w [E, n, k] or [E, k, n] (2-D when dense), contiguous; returns (y, z or None)."""
     m, k = x.shape
-    if _copied(x, n):
-        x, w, bias, residual = _aligned(x), _aligned(w), _aligned(bias), _aligned(residual)
+    px, pw, pb, pr = x.data_ptr(), w.data_ptr(), _lib.ptr(bias), _lib.ptr(residual)
+    if (px | pw | (pb or 0) | (pr or 0)) & 15:
+        x, w, bias, residual = _on_boundary(m, n, k, E, trans_b, x, w, bias, residual)
+        px, pw, pb, pr = x.data_ptr(), w.data_ptr(), _lib.ptr(bias), _lib.ptr(residual)
     y = torch.empty((m, n), device=x.device, dtype=x.dtype)
     z = torch.empty_like(y) if want_z else None
     lib = _lib.load()
@@ -71,8 +73,7 @@ def _forward(x, w, bias, residual, offsets, act: int, trans_b: bool, E: int, n: 
         ws_bytes = _workspace_bytes(m, n, k, E, int(trans_b), code)
         ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8) if ws_bytes else None
         st = lib.moe_linear_fwd(
-            x.data_ptr(), w.data_ptr(), _lib.ptr(bias), _lib.ptr(residual), y.data_ptr(), _lib.ptr(z),
-            _lib.ptr(offsets), 0 if offsets is None else offsets.numel(), m, n, k, E, int(trans_b),
+            px, pw, pb, pr, y.data_ptr(), _lib.ptr(z), _lib.ptr(offsets), 0 if offsets is None else offsets.numel(), m, n, k, E, int(trans_b),
             act, code, _lib.ptr(ws), ws_bytes, _lib.raw_stream(x))
     _lib.check(st, "moe_linear_fwd")
     _lib.count_launches(1)
@@ -87,8 +88,8 @@ def _bwd_workspace_bytes(m: int, n: int, E: int, act: int, code: int) -> int:
 def _backward(dy, x, w, z, offsets, act: int, trans_b: bool, E: int, n: int, bias_shape, wanted):
     """(dx, dw, dbias), None where not wanted."""
     m, k = x.shape
-    if _copied(x, n):
-        x, w = _aligned(x), _aligned(w)
+    if (x.data_ptr() | w.data_ptr()) & 15:
+        x, w = _on_boundary(m, n, k, E, False, x, w)
     dx = torch.empty_like(x) if wanted[0] else None
     dw = torch.empty_like(w) if wanted[1] else None
     db = torch.empty(bias_shape, device=x.device, dtype=x.dtype) if wanted[2] else None
@@ -179,18 +180,36 @@ class _Linear(torch.autograd.Function):
 
 
 # 16-bit operands whose rows are not 16-byte multiples, or that start off a 16-byte boundary: from
-# this many multiplications on they are copied into rows that are (zeros behind) for the tensor
-# cores; below, the CUDA cores take them as they are.  (bf16 2000 x 1001 x 1500, forward: 58 us
-# with the copies; the CUDA cores' 21 TFLOP/s would make it 290 us.)
+# this many multiplications on, and if _copy_pays, they are copied into rows that are (zeros behind)
+# for the tensor cores; otherwise the CUDA cores take them as they are.
 _PAD_FROM = 1 << 24
 
 
-def _copied(x, n) -> bool:
-    return x.dtype != torch.float32 and x.shape[0] * n * x.shape[1] >= _PAD_FROM
+def _copy_pays(m: int, n: int, E: int, trans_b: bool) -> bool:
+    """Whether m rows over E groups amortise a copy of every group's weights.
+
+    Measured, bf16, CUDA cores / copy and tensor cores in us (rows, K -> N):
+        4 x 4097 -> 4097        72 / 85     8: 114 / 85     64: 475 / 95
+        2 x 7167 -> 11007       211 / 269   4: 275 / 269    16: 712 / 273
+        8 groups 1999 -> 2001   32: 132 / 140   64: 214 / 138
+        64 groups 999 -> 1001   16: 52 / 224    256: 247 / 245   512: 390 / 247
+    Without trans_b the CUDA cores have only 64 x 64 tiles, whose time follows K and how many there
+    are, while a copy's follows E * N * K:
+        1 x 4097 -> 4097        468 / 98
+        8 groups 1999 -> 2001   1: 231 / 133    64: 276 / 139
+        32 groups 999 -> 1001   1: 121 / 125    16: 159 / 133
+        64 groups 999 -> 1001   32: 165 / 229   64: 310 / 240
+    """
+    return m > 4 * E if trans_b else (E * n <= 40000 or m >= E)
 
 
-def _aligned(t):
-    return t if t is None or t.data_ptr() % 16 == 0 else t.clone()
+def _on_boundary(m, n, k, E, trans_b, x, w, *others):
+    """The operands, those off a 16-byte boundary copied where that lets the tensor cores take them."""
+    off = [t is not None and t.data_ptr() & 15 != 0 for t in (x, w, *others)]
+    if (x.dtype == torch.float32 or n % 8 or k % 8 or m * n * k < _PAD_FROM
+            or (off[1] and not _copy_pays(m, n, E, trans_b))):
+        return x, w, *others
+    return tuple(t.clone() if o else t for t, o in zip((x, w, *others), off))
 
 
 def _padded(x, w, bias, residual, offsets, act, trans_b, E, n):
@@ -203,12 +222,15 @@ def _padded(x, w, bias, residual, offsets, act, trans_b, E, n):
 
 
 def _apply(x, w, bias, residual, offsets, act, trans_b, E, n):
-    if (n % 8 or x.shape[1] % 8) and _copied(x, n):
+    m, k = x.shape
+    grads = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias, residual))
+    # (the backward's dgrad reads the weights as a product without trans_b does)
+    if ((n % 8 or k % 8) and x.dtype != torch.float32 and m * n * k >= _PAD_FROM
+            and _copy_pays(m, n, E, trans_b and not grads)):
         return _padded(x, w, bias, residual, offsets, act, trans_b, E, n)
     direct = _lib.direct(x, w, bias, residual, offsets)
     # The autograd Function refuses what it cannot differentiate (forward mode, functorch).
-    if not direct or (torch.is_grad_enabled()
-                      and any(t is not None and t.requires_grad for t in (x, w, bias, residual))):
+    if grads or not direct:
         return _Linear.apply(x, w, bias, residual, offsets, act, trans_b, E, n, direct)
     return _forward(x, w, bias, residual, offsets, act, trans_b, E, n, False)[0]
 

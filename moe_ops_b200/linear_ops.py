@@ -88,8 +88,8 @@ def _bwd_workspace_bytes(m: int, n: int, E: int, act: int, code: int) -> int:
 def _backward(dy, x, w, z, offsets, act: int, trans_b: bool, E: int, n: int, bias_shape, wanted):
     """(dx, dw, dbias), None where not wanted."""
     m, k = x.shape
-    if (x.data_ptr() | w.data_ptr()) & 15:
-        x, w = _on_boundary(m, n, k, E, False, x, w)
+    if (x.data_ptr() | w.data_ptr() | dy.data_ptr()) & 15:
+        x, w, dy = _on_boundary(m, n, k, E, False, x, w, dy)
     dx = torch.empty_like(x) if wanted[0] else None
     dw = torch.empty_like(w) if wanted[1] else None
     db = torch.empty(bias_shape, device=x.device, dtype=x.dtype) if wanted[2] else None

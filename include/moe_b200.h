@@ -360,8 +360,8 @@ int moe_few_experts_fwd(const void* x, const float* weights, const int32_t* indi
  * A [m_total, k], B [E, N, K] if trans_b else [E, K, N], bias [E, n] or NULL, residual
  * [m_total, n] or NULL, out [m_total, n]; preact [m_total, n] receives z rounded to dtype (for
  * the backward), or NULL.  Offsets as in moe_gmm_fwd (replaces an moe_gmm_fwd followed by
- * elementwise passes); a dense product is offsets NULL, num_offsets 0, num_experts 1.  Rows
- * behind the last offset get residual (or zero).  residual may not overlap out.  The sum, the
+ * elementwise passes); a dense product is offsets NULL, num_offsets 0, num_experts 1.  At most 1024
+ * experts.  Rows behind the last offset get residual (or zero).  residual may not overlap out.  The sum, the
  * bias, the activation and the residual are in fp32; out is rounded once.  Workspace:
  * moe_linear_workspace_bytes(...) bytes (0 for many rows: then it may be NULL), 16-byte aligned,
  * not shared with a call that may run at the same time. */

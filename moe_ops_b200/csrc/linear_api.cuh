@@ -71,7 +71,7 @@ template <typename T>
 static int linear_simt(const LinearArgs& a) {
   const LinearEpilogue<T> epi{(T*)a.out, (T*)a.preact, (const T*)a.bias, (const T*)a.residual, a.act};
   const bool vec = (a.k * sizeof(T)) % 16 == 0 && aligned16(a.A) && aligned16(a.B);
-  if (!a.b_mn && a.E <= gmm::kMaxGroups && a.n < (1 << 30) && a.k < (1 << 30) &&
+  if (!a.b_mn && a.n < (1 << 30) && a.k < (1 << 30) &&
       linear_warps_win(a.m, a.n, a.k, a.E, sizeof(T), vec)) {
     const int64_t warps = ((a.m + kWarpRows - 1) / kWarpRows + (a.offsets ? a.E : 0)) * a.n;
     const unsigned grid = (unsigned)std::min<int64_t>((warps + 7) / 8, 8 * num_sms(current_device()));
@@ -87,7 +87,7 @@ static int linear_simt(const LinearArgs& a) {
   }
   const dim3 grid((unsigned)((a.m + simt::TM - 1) / simt::TM), (unsigned)((a.n + simt::TN - 1) / simt::TN),
                   (unsigned)a.E);
-  MOE_REQUIRE(grid.y <= 65535 && grid.z <= 65535, "linear: too large for the CUDA-core path");
+  MOE_REQUIRE(grid.y <= 65535, "linear: too large for the CUDA-core path");
   simt::gmm_rows_simt_kernel<T><<<grid, 256, 0, a.stream>>>(
       (const T*)a.A, (const T*)a.B, epi, a.offsets, a.plus_one, a.m, a.n, a.k, a.b_mn);
   MOE_LAUNCH_CHECK();
@@ -95,7 +95,7 @@ static int linear_simt(const LinearArgs& a) {
 }
 
 static bool linear_tc_ok(const LinearArgs& a) {
-  return a.dtype != MOE_F32 && a.k > 0 && a.k % 8 == 0 && a.n % 8 == 0 && a.E <= gmm::kMaxGroups &&
+  return a.dtype != MOE_F32 && a.k > 0 && a.k % 8 == 0 && a.n % 8 == 0 &&
          aligned16(a.A) && aligned16(a.B) && aligned16(a.out) && aligned16(a.preact) &&
          aligned16(a.bias) && aligned16(a.residual) && a.m < (1ll << 31) && a.n < (1ll << 31) &&
          a.k < (1ll << 31);
@@ -230,6 +230,7 @@ static int check_linear(const void* a, const void* b, const void* out, const int
                         int num_offsets, int64_t m, int64_t n, int64_t k, int E, int act, int dtype) {
   MOE_REQUIRE(act >= MOE_ACT_NONE && act <= MOE_ACT_SILU, "linear: bad activation %d", act);
   MOE_REQUIRE(E >= 1 || offsets != nullptr || m == 0, "linear: no groups");
+  MOE_REQUIRE(E <= gmm::kMaxGroups, "linear: more than %d experts", gmm::kMaxGroups);
   // An operand with no elements may be NULL.
   if (m > 0 && n > 0)
     MOE_REQUIRE(out && ((a && b) || k == 0 || E == 0), "linear: NULL operand");
@@ -252,7 +253,6 @@ static BwdWorkspace bwd_workspace(int64_t m, int64_t n, int E, int act, int dtyp
 static int act_bwd(const void* grad_out, const void* preact, void* dz, void* grad_bias,
                    const int32_t* offsets, int num_offsets, int64_t m, int64_t n, int E, int activation,
                    int dtype, float* partial, cudaStream_t s) {
-  MOE_REQUIRE(E <= gmm::kMaxGroups, "linear_bwd: more than %d experts", gmm::kMaxGroups);
   const bool act = activation != MOE_ACT_NONE;
   const int plus_one = num_offsets == E + 1;
   if (!grad_bias) partial = nullptr;

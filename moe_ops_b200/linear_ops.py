@@ -33,6 +33,7 @@ import torch.nn.functional as F
 
 from . import _lib
 
+MAX_GROUPS = 1024
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 
@@ -73,8 +74,9 @@ def _forward(x, w, bias, residual, offsets, act: int, trans_b: bool, E: int, n: 
         ws_bytes = _workspace_bytes(m, n, k, E, int(trans_b), code)
         ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8) if ws_bytes else None
         st = lib.moe_linear_fwd(
-            px, pw, pb, pr, y.data_ptr(), _lib.ptr(z), _lib.ptr(offsets), 0 if offsets is None else offsets.numel(), m, n, k, E, int(trans_b),
-            act, code, _lib.ptr(ws), ws_bytes, _lib.raw_stream(x))
+            px, pw, pb, pr, y.data_ptr(), _lib.ptr(z), _lib.ptr(offsets),
+            0 if offsets is None else offsets.numel(), m, n, k, E, int(trans_b), act, code,
+            _lib.ptr(ws), ws_bytes, _lib.raw_stream(x))
     _lib.check(st, "moe_linear_fwd")
     _lib.count_launches(1)
     return y, z
@@ -287,6 +289,8 @@ def grouped_linear(A: torch.Tensor, B: torch.Tensor, offsets: torch.Tensor,
     if A.dim() != 2 or B.dim() != 3 or B.shape[2 if trans_b else 1] != A.shape[1]:
         raise ValueError(f"A [M, K] and B do not match: {list(A.shape)}, {list(B.shape)}, trans_b={trans_b}")
     E, n = B.shape[0], B.shape[1 if trans_b else 2]
+    if E > MAX_GROUPS:
+        raise ValueError(f"at most {MAX_GROUPS} experts (got {E})")
     act = _check(A, B, bias, residual, (A.shape[0], n), (E, n), activation)
     _lib.require_cuda(offsets)
     if offsets.numel() not in (E, E + 1) or offsets.numel() == 0 or offsets.device != A.device:

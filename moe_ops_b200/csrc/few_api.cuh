@@ -122,8 +122,9 @@ static int few_ring(fewtc::Params& p, int phases, int nb, int table_bytes) {
   return MOE_OK;
 }
 
-// Workspace: logits [T, E] fp32; h [T*K, H] (fp32 for the CUDA cores, else 16 bits); the CUDA
-// cores' slot weights and positions; the tensor-core kernel's counters; the experts' outputs, fp32
+// Workspace: logits [T, E] fp32; h [T*K, H] (fp32 for the CUDA cores, which also take 16-bit operands
+// off a boundary, so 4 bytes an element; the tensor cores use half); the CUDA cores' slot weights and
+// positions; the tensor-core kernel's counters; the experts' outputs, fp32
 // [parts, T*K, d] (one part for the CUDA cores).
 struct FewWorkspace {
   size_t logits, h, slots, counters, part, total;

@@ -164,7 +164,6 @@ struct Plan {
   int16_t* pos;       // [S]; holds the slot's expert while the plan is built
   int16_t* rank;      // [S] scratch
   uint16_t* slot;     // [S]
-  uint16_t* unit_of;  // [S] unit of a position
   int16_t* unit_e;    // [U]
   uint16_t* unit_pos; // [U] first position
   uint16_t* unit_n;   // [U] rows
@@ -176,7 +175,7 @@ __host__ __device__ inline int plan_max_units(int S, int E, int rows_per_unit) {
 }
 __host__ __device__ inline int plan_bytes(int S, int E, int rows_per_unit) {
   const int U = plan_max_units(S, E, rows_per_unit);
-  return ((4 * S + 4 * E + 4 * (E + 1) + 2 * S * 4 + 2 * U * 3 + 4 + 4) + 15) / 16 * 16;
+  return ((4 * S + 4 * E + 4 * (E + 1) + 2 * S * 3 + 2 * U * 3 + 4 + 4) + 15) / 16 * 16;
 }
 __device__ inline Plan plan_view(uint8_t* mem, int S, int E, int rows_per_unit) {
   const int U = plan_max_units(S, E, rows_per_unit);
@@ -188,8 +187,7 @@ __device__ inline Plan plan_view(uint8_t* mem, int S, int E, int rows_per_unit) 
   p.pos = reinterpret_cast<int16_t*>(p.num_units + 1);
   p.rank = p.pos + S;
   p.slot = reinterpret_cast<uint16_t*>(p.rank + S);
-  p.unit_of = p.slot + S;
-  p.unit_e = reinterpret_cast<int16_t*>(p.unit_of + S);
+  p.unit_e = reinterpret_cast<int16_t*>(p.slot + S);
   p.unit_pos = reinterpret_cast<uint16_t*>(p.unit_e + U);
   p.unit_n = p.unit_pos + U;
   return p;
@@ -276,8 +274,6 @@ __device__ __forceinline__ void build_plan(const Plan& p, const Routing& r, int 
       p.slot[at] = (uint16_t)s;
     }
   }
-  for (int u = threadIdx.x; u < *p.num_units; u += blockDim.x)
-    for (int i = 0; i < p.unit_n[u]; ++i) p.unit_of[p.unit_pos[u] + i] = (uint16_t)u;
   __syncthreads();
 }
 

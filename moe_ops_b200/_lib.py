@@ -105,8 +105,9 @@ SIGNATURES = {
 _lib = None
 _lock = threading.Lock()
 
-# Instrumentation used by bench.py: number of library kernels launched so far, and an
-# optional list that collects (name, start_event, end_event, flops) around every grouped
+# Instrumentation used by bench.py: number of library kernels launched so far (the main kernels
+# of each call: zeroed counters, rows behind the last group, the bias gradient's second pass
+# and the CUDA cores' extra launches of the few-token layer are not counted), and an optional list that collects (name, start_event, end_event, flops) around every grouped
 # GEMM call (CUDA events on the launching stream).
 launch_count = 0
 gemm_timing: list | None = None

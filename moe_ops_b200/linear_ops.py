@@ -8,8 +8,9 @@
 
 ``grouped_linear`` stands beside ``grouped_gemm`` (same A, B, offsets and trans_b) for experts
 with biases or an activation of their own; ``linear`` is the dense product next to the routed
-experts (a shared expert, a projection).  One launch: the sum, the bias, the activation and the
-residual are in fp32 and y is rounded once.
+experts (a shared expert, a projection).  The sum, the bias, the activation and the residual are in
+fp32 inside the product's kernel and y is rounded once.  (A cut few-row product launches one more
+kernel, which zeroes its counters, and a grouped call one more for the rows behind the last group.)
 
 Both are differentiable in every tensor argument.  With an activation the forward also writes z
 (rounded to the dtype) when a gradient will be needed; the backward is one elementwise pass
@@ -239,7 +240,7 @@ def _apply(x, w, bias, residual, offsets, act, trans_b, E, n):
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
            activation: str = "none", residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """act(x . weight^T + bias) + residual, in one launch.
+    """act(x . weight^T + bias) + residual, in the product's kernel.
 
     Args:
         x: [..., K].

@@ -88,7 +88,12 @@ class MoELayer(torch.nn.Module):
         self.fused_permute = False
         # > 0: calls of up to that many tokens (at most 128) without gradients and without
         # token dropping run moe_few_tokens; its router logits are not rounded to x's dtype, so
-        # experts whose logits are close may rank differently than in the assembled layer
+        # experts whose logits are close may rank differently than in the assembled layer.
+        # Faster up to 48 tokens on every layer measured, up to 128 where the weights are
+        # tens of MB (bf16, assembled / few, us: d = 4096, 64 experts, H = 11008, top-2:
+        # 1 token 342 / 126, 64 2363 / 2246, 128 2778 / 2742; d = 7168, 256 experts,
+        # H = 2048, top-8: 1 342 / 181, 48 2802 / 2561, 64 3235 / 3524; d = 1024,
+        # 8 experts, H = 2816, top-2: 1 222 / 46, 128 214 / 91)
         self.few_tokens = 0
 
     @torch.no_grad()

@@ -52,3 +52,26 @@ def test_layer():
         m.few_tokens = 16
         ops = recorded(lambda a: m(a), fake(5, 64))
         assert ops == ["moeb200.few_tokens.default"] + ["moeb200.linear_fwd.default"] * 2
+
+
+def test_registered_ops_give_the_real_shapes():
+    """Shapes and dtypes of the four ops' fake forms."""
+    ops, f32 = torch.ops.moeb200, torch.float32
+    with FakeTensorMode():
+        x, w, B, off, dy = fake(7, 64), fake(24, 64), fake(3, 64, 24), fake(4, dtype=torch.int32), fake(7, 24)
+        wr, wg, wd = fake(8, 64), fake(8, 48, 64), fake(8, 64, 48)
+        got = {
+            "linear_fwd": ops.linear_fwd(x, w, None, None, None, 4, True, True),
+            "linear_fwd, no z": ops.linear_fwd(x, B, None, None, off, 0, False, False),
+            "linear_bwd": ops.linear_bwd(dy, x, w, dy, None, 4, True, True, True, True),
+            "linear_bwd, grouped": ops.linear_bwd(dy, x, B, None, off, 0, False, False, True, True),
+            "few_tokens": (ops.few_tokens(x, wr, wg, wg, wd, 2, None),),
+            "few_experts": (ops.few_experts(x, fake(7, 2, dtype=f32), fake(7, 2, dtype=torch.int32), wg, wg, wd),),
+        }
+    want = {
+        "linear_fwd": [(7, 24), (7, 24)], "linear_fwd, no z": [(7, 24), (0,)],
+        "linear_bwd": [(7, 64), (24, 64), (24,)], "linear_bwd, grouped": [(0,), (3, 64, 24), (3, 24)],
+        "few_tokens": [(7, 64)], "few_experts": [(7, 64)],
+    }
+    for name, out in got.items():
+        assert [tuple(t.shape) for t in out] == want[name] and all(t.dtype == BF for t in out), name

@@ -183,7 +183,8 @@ int moe_unpermute_bwd(const void* grad_out, const void* input_fwd, int dtype,
  * A [M_total, K]; B [E, N, K] if trans_b else [E, K, N]; C [M_total, N].
  * C[rows of e] = A[rows of e] @ (B[e]^T if trans_b else B[e]), fp32 accumulation.
  * bf16/fp16 run on the tcgen05 tensor-core kernel; fp32 (and shapes whose rows are not
- * 16-byte multiples) on a CUDA-core kernel with fp32 FMA. */
+ * 16-byte multiples) on a CUDA-core kernel with fp32 FMA.  Here, in moe_gmm_dgrad and in
+ * moe_gmm_wgrad a dense product is offsets NULL, num_offsets 0, num_experts 1. */
 int moe_gmm_fwd(const void* A, const void* B, void* C, const int32_t* offsets,
                 int32_t num_offsets, int64_t m_total, int64_t n, int64_t k, int32_t num_experts,
                 int trans_b, int dtype, void* stream);

@@ -234,7 +234,7 @@ static int check_linear(const void* a, const void* b, const void* out, const int
   // An operand with no elements may be NULL.
   if (m > 0 && n > 0)
     MOE_REQUIRE(out && ((a && b) || k == 0 || E == 0), "linear: NULL operand");
-  return check_gmm_args(out, out, out, offsets, num_offsets, out ? m : 0, n, k, E, dtype);
+  return check_gmm_args(out, out, out, offsets, num_offsets, out ? m : 0, n, k, E, dtype, true);
 }
 
 // Workspace of the backward: dz [m, n] (unless there is no activation), then the bias gradient's

@@ -458,11 +458,12 @@ static int gmm_wgrad(const void* X, const void* Y, void* Out, const int32_t* off
 }
 
 static int check_gmm_args(const void* a, const void* b, const void* c, const int32_t* offsets,
-                          int num_offsets, int64_t m_total, int64_t n, int64_t k, int E, int dtype) {
+                          int num_offsets, int64_t m_total, int64_t n, int64_t k, int E, int dtype,
+                          bool dense_ok = false) {
   MOE_REQUIRE(dtype_ok(dtype), "gmm: bad dtype %d", dtype);
   MOE_REQUIRE(E >= 0 && m_total >= 0 && n >= 0 && k >= 0, "gmm: negative size");
-  // No offsets: one group of all m_total rows (a dense product).
-  const bool dense = offsets == nullptr && num_offsets == 0 && E == 1;
+  // No offsets, where the entry takes that: one group of all m_total rows (a dense product).
+  const bool dense = dense_ok && offsets == nullptr && num_offsets == 0 && E == 1;
   MOE_REQUIRE(dense || num_offsets == E || num_offsets == E + 1,
               "gmm: num_offsets must be E or E+1 (got %d, E=%d)", num_offsets, E);
   MOE_REQUIRE(dense || E == 0 || offsets != nullptr, "gmm: offsets is NULL");
@@ -828,7 +829,7 @@ int moe_unpermute_bwd(const void* grad_out, const void* input_fwd, int dtype,
 int moe_gmm_fwd(const void* A, const void* B, void* C, const int32_t* offsets, int32_t num_offsets,
                 int64_t m_total, int64_t n, int64_t k, int32_t E, int trans_b, int dtype,
                 void* stream) {
-  int rc = check_gmm_args(A, B, C, offsets, num_offsets, m_total, n, k, E, dtype);
+  int rc = check_gmm_args(A, B, C, offsets, num_offsets, m_total, n, k, E, dtype, true);
   if (rc) return rc;
   if (E == 0) return MOE_OK;
   // trans_b: B[e] is [N, K] (K-major operand); else [K, N] (MN-major operand).
@@ -868,7 +869,7 @@ int moe_gmm_wgrad_gather(const void* A_src, const int32_t* a_rows, int64_t a_src
 int moe_gmm_dgrad(const void* grad_C, const void* B, void* grad_A, const int32_t* offsets,
                   int32_t num_offsets, int64_t m_total, int64_t n, int64_t k, int32_t E,
                   int trans_b, int dtype, void* stream) {
-  int rc = check_gmm_args(grad_C, B, grad_A, offsets, num_offsets, m_total, n, k, E, dtype);
+  int rc = check_gmm_args(grad_C, B, grad_A, offsets, num_offsets, m_total, n, k, E, dtype, true);
   if (rc) return rc;
   if (E == 0) return MOE_OK;
   // grad_A [M, K] = grad_C [M, N] . B'[e], contraction over N.  With trans_b, B[e] is
@@ -901,7 +902,7 @@ int moe_gmm_dgrad_dual(const void* grad_C1, const void* B1, const void* grad_C2,
 int moe_gmm_wgrad(const void* A, const void* grad_C, void* grad_B, const int32_t* offsets,
                   int32_t num_offsets, int64_t m_total, int64_t n, int64_t k, int32_t E,
                   int trans_b, int dtype, void* stream) {
-  int rc = check_gmm_args(A, grad_C, grad_B, offsets, num_offsets, m_total, n, k, E, dtype);
+  int rc = check_gmm_args(A, grad_C, grad_B, offsets, num_offsets, m_total, n, k, E, dtype, true);
   if (rc) return rc;
   if (E == 0) return MOE_OK;
   const int plus_one = num_offsets == E + 1;

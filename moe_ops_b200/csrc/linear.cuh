@@ -119,11 +119,11 @@ linear_rows_kernel(const T* __restrict__ A, const T* __restrict__ B, const Linea
 // kDzRows consecutive rows of one group and kDzCols columns; its column sums go to
 // partial[chunk, n] and dbias_kernel adds the chunks of a group in order, so the result does
 // not depend on the order blocks run in.  HBM-bound: 2 reads + 1 write of m * n elements (bf16,
-// 4099 x 7168, cold L2: 27 us at the copy rate, 49 to 51 us for relu, gelu and gelu_tanh, 59 us for
-// silu, and 10 us with the bias gradient's second launch).  The activation is a template parameter and
+// 4099 x 7168, cold L2: 27 us at the copy rate, 49 us for relu, gelu and gelu_tanh, 59 us for silu,
+// and 10 us with the bias gradient's second launch).  The activation is a template parameter and
 // registers are capped at 64: three rows' loads in flight per thread, four blocks per SM (one kernel
-// for all activations: silu 78 us; four rows: gelu 55, silu 64 us, where silu and relu spill 40 to 52
-// bytes; two rows: gelu 66 us).  relu and silu still spill 16 to 24 bytes.
+// for all activations: silu 78 us; four rows: silu 66 us, relu and silu spill 40 to 52 bytes; two
+// rows: gelu 64 us).  relu and silu still spill 16 to 20 bytes.
 constexpr int kDzRows = 64;
 constexpr int kDzThreads = 256;
 

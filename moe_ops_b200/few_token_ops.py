@@ -66,11 +66,11 @@ def _run(x, route, w_gate, w_up, w_down, dims, K: int, given: bool) -> torch.Ten
     x, w_gate, w_up, w_down = (x.contiguous(), w_gate.contiguous(), w_up.contiguous(),
                                w_down.contiguous())
     lib = _lib.load()
-    y = torch.empty((T, d), device=x.device, dtype=x.dtype)
+    y = x.new_empty((T, d))
     fn = lib.moe_few_experts_fwd if given else lib.moe_few_tokens_fwd
     with _lib.on_device(x):
         ws_bytes = _workspace_bytes(T, d, H, E, K, code)
-        ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8)
+        ws = x.new_empty(ws_bytes, dtype=torch.uint8)
         st = fn(x.data_ptr(), _lib.ptr(route[0]), _lib.ptr(route[1]), w_gate.data_ptr(),
                 w_up.data_ptr(), w_down.data_ptr(), code, T, d, H, E, K, y.data_ptr(),
                 ws.data_ptr(), ws_bytes, _lib.raw_stream(x))

@@ -67,13 +67,13 @@ def _forward(x, w, bias, residual, offsets, act: int, trans_b: bool, E: int, n: 
     if (px | pw | (pb or 0) | (pr or 0)) & 15:
         x, w, bias, residual = _on_boundary(m, n, k, E, trans_b, x, w, bias, residual)
         px, pw, pb, pr = x.data_ptr(), w.data_ptr(), _lib.ptr(bias), _lib.ptr(residual)
-    y = torch.empty((m, n), device=x.device, dtype=x.dtype)
+    y = x.new_empty((m, n))
     z = torch.empty_like(y) if want_z else None
     lib = _lib.load()
     code = _lib.dtype_code(x.dtype)
     with _lib.on_device(x):
         ws_bytes = _workspace_bytes(m, n, k, E, int(trans_b), code)
-        ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8) if ws_bytes else None
+        ws = x.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
         st = lib.moe_linear_fwd(
             px, pw, pb, pr, y.data_ptr(), _lib.ptr(z), _lib.ptr(offsets),
             0 if offsets is None else offsets.numel(), m, n, k, E, int(trans_b), act, code,
@@ -95,12 +95,12 @@ def _backward(dy, x, w, z, offsets, act: int, trans_b: bool, E: int, n: int, bia
         x, w, dy = _on_boundary(m, n, k, E, False, x, w, dy)
     dx = torch.empty_like(x) if wanted[0] else None
     dw = torch.empty_like(w) if wanted[1] else None
-    db = torch.empty(bias_shape, device=x.device, dtype=x.dtype) if wanted[2] else None
+    db = x.new_empty(bias_shape) if wanted[2] else None
     code = _lib.dtype_code(x.dtype)
     lib = _lib.load()
     with _lib.on_device(x):
         ws_bytes = _bwd_workspace_bytes(m, n, E, act, code) if act or wanted[2] else 0
-        ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8) if ws_bytes else None
+        ws = x.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
         st = lib.moe_linear_bwd(
             dy.data_ptr(), x.data_ptr(), w.data_ptr(), _lib.ptr(z), _lib.ptr(dx), _lib.ptr(dw),
             _lib.ptr(db), _lib.ptr(offsets), 0 if offsets is None else offsets.numel(), m, n, k, E,
@@ -164,21 +164,23 @@ class _Linear(torch.autograd.Function):
             y, z = torch.ops.moeb200.linear_fwd(x, w, bias, residual, offsets, act, trans_b, want_z)
             z = z if want_z else None
         ctx.save_for_backward(x, w, z, offsets)
-        ctx.cfg = (act, trans_b, E, n, None if bias is None else bias.shape)
+        ctx.cfg = (act, trans_b, E, n, None if bias is None else bias.shape, direct)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, w, z, offsets = ctx.saved_tensors
-        act, trans_b, E, n, bias_shape = ctx.cfg
+        act, trans_b, E, n, bias_shape, direct = ctx.cfg
         wanted = ctx.needs_input_grad[:3]
         dx = dw = db = None
-        if any(wanted) and _lib.direct(dy, x, w, z, offsets):
-            dx, dw, db = _backward(dy.contiguous(), x, w, z, offsets, act, trans_b, E, n, bias_shape, wanted)
-        elif any(wanted):
-            got = torch.ops.moeb200.linear_bwd(dy, x, w, z, offsets, act, trans_b, *wanted)
-            dx, dw, db = (t if on else None for t, on in zip(got, wanted))
+        if True in wanted:
+            if direct and _lib.direct(dy):
+                dx, dw, db = _backward(dy.contiguous(), x, w, z, offsets, act, trans_b, E, n, bias_shape, wanted)
+            else:
+                _lib.refuse_tangents("the backward of linear", dy)
+                got = torch.ops.moeb200.linear_bwd(dy, x, w, z, offsets, act, trans_b, *wanted)
+                dx, dw, db = (t if on else None for t, on in zip(got, wanted))
         return dx, dw, db, dy if ctx.needs_input_grad[3] else None, *([None] * 6)
 
 
@@ -226,7 +228,9 @@ def _padded(x, w, bias, residual, offsets, act, trans_b, E, n):
 
 def _apply(x, w, bias, residual, offsets, act, trans_b, E, n):
     m, k = x.shape
-    grads = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias, residual))
+    grads = torch.is_grad_enabled() and (
+        x.requires_grad or w.requires_grad or (bias is not None and bias.requires_grad)
+        or (residual is not None and residual.requires_grad))
     # (the backward's dgrad reads the weights as a product without trans_b does)
     if ((n % 8 or k % 8) and x.dtype != torch.float32 and m * n * k >= _PAD_FROM
             and _copy_pays(m, n, E, trans_b and not grads)):

@@ -151,3 +151,17 @@ def test_registered_ops(cuda_dev):
     torch.library.opcheck(ops.few_tokens, (x, wr, wg, wg, wd, 2, None), test_utils=checks)
     p, i = torch.rand(12, 2, device=cuda_dev), torch.zeros(12, 2, device=cuda_dev, dtype=torch.int32)
     torch.library.opcheck(ops.few_experts, (x, p, i, wg, wg, wd), test_utils=checks)
+
+
+def test_a_tangent_of_the_output_gradient_raises(cuda_dev):
+    g = torch.Generator(device=cuda_dev).manual_seed(7)
+    x, w, dy = (torch.randn(*s, device=cuda_dev, generator=g) for s in ((9, 24), (16, 24), (9, 16)))
+    x.requires_grad_(True)
+    y = M.linear(x, w, activation="silu")
+    with fw.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+        torch.autograd.grad(y, x, fw.make_dual(dy, torch.ones_like(dy)))
+    y = M.linear(x, w, activation="silu")
+    with fw.dual_level():
+        got = torch.autograd.grad(y, x, dy)[0]
+    y = M.linear(x, w, activation="silu")
+    assert torch.equal(got, torch.autograd.grad(y, x, dy)[0])

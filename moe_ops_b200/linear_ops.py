@@ -91,6 +91,8 @@ def _bwd_workspace_bytes(m: int, n: int, E: int, act: int, code: int) -> int:
 def _backward(dy, x, w, z, offsets, act: int, trans_b: bool, E: int, n: int, bias_shape, wanted):
     """(dx, dw, dbias), None where not wanted."""
     m, k = x.shape
+    if (n % 8 or k % 8) and x.dtype != torch.float32 and m * n * k >= _PAD_FROM and _copy_pays(m, n, E, False):
+        return _backward_padded(dy, x, w, z, offsets, act, trans_b, E, n, bias_shape, wanted)
     if (x.data_ptr() | w.data_ptr() | dy.data_ptr()) & 15:
         x, w, dy = _on_boundary(m, n, k, E, False, x, w, dy)
     dx = torch.empty_like(x) if wanted[0] else None
@@ -191,7 +193,8 @@ _PAD_FROM = 1 << 24
 
 
 def _copy_pays(m: int, n: int, E: int, trans_b: bool) -> bool:
-    """Whether m rows over E groups amortise a copy of every group's weights.
+    """Whether m rows over E groups amortise a copy of every group's weights.  (The backward asks
+    without trans_b: its dgrad reads the weights as such a product does.)
 
     Measured, bf16, CUDA cores / copy and tensor cores in us (rows, K -> N):
         4 x 4097 -> 4097        72 / 85     8: 114 / 85     64: 475 / 95
@@ -217,24 +220,40 @@ def _on_boundary(m, n, k, E, trans_b, x, w, *others):
     return tuple(t.clone() if o else t for t, o in zip((x, w, *others), off))
 
 
+def _pad_weight(w, trans_b, dn, dk):
+    return F.pad(w, (0, dk, 0, dn) if trans_b else (0, dn, 0, dk))
+
+
 def _padded(x, w, bias, residual, offsets, act, trans_b, E, n):
     k = x.shape[1]
     dn, dk = -n % 8, -k % 8
-    w = F.pad(w, (0, dk, 0, dn) if trans_b else (0, dn, 0, dk))
+    w = _pad_weight(w, trans_b, dn, dk)
     y = _apply(F.pad(x, (0, dk)), w, None if bias is None else F.pad(bias, (0, dn)),
                None if residual is None else F.pad(residual, (0, dn)), offsets, act, trans_b, E, n + dn)
     return y[:, :n].contiguous()
 
 
+def _backward_padded(dy, x, w, z, offsets, act, trans_b, E, n, bias_shape, wanted):
+    """_backward through 16-byte rows, where the forward's rows were too few for a copy."""
+    k = x.shape[1]
+    dn, dk = -n % 8, -k % 8
+    dx, dw, db = _backward(F.pad(dy, (0, dn)), F.pad(x, (0, dk)), _pad_weight(w, trans_b, dn, dk),
+                           None if z is None else F.pad(z, (0, dn)), offsets, act, trans_b, E, n + dn,
+                           None if bias_shape is None else (*bias_shape[:-1], n + dn), wanted)
+    if dx is not None:
+        dx = dx[:, :k].contiguous()
+    if dw is not None:
+        dw = (dw[..., :n, :k] if trans_b else dw[..., :k, :n]).contiguous()
+    return dx, dw, None if db is None else db[..., :n].contiguous()
+
+
 def _apply(x, w, bias, residual, offsets, act, trans_b, E, n):
     m, k = x.shape
+    if (n % 8 or k % 8) and x.dtype != torch.float32 and m * n * k >= _PAD_FROM and _copy_pays(m, n, E, trans_b):
+        return _padded(x, w, bias, residual, offsets, act, trans_b, E, n)
     grads = torch.is_grad_enabled() and (
         x.requires_grad or w.requires_grad or (bias is not None and bias.requires_grad)
         or (residual is not None and residual.requires_grad))
-    # (the backward's dgrad reads the weights as a product without trans_b does)
-    if ((n % 8 or k % 8) and x.dtype != torch.float32 and m * n * k >= _PAD_FROM
-            and _copy_pays(m, n, E, trans_b and not grads)):
-        return _padded(x, w, bias, residual, offsets, act, trans_b, E, n)
     direct = _lib.direct(x, w, bias, residual, offsets)
     # The autograd Function refuses what it cannot differentiate (forward mode, functorch).
     if grads or not direct:

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import moe_ops_b200 as M
+import test_linear_gpu
 
 pytestmark = pytest.mark.gpu
 
@@ -75,3 +76,16 @@ def test_no_copy_of_weights_that_few_rows_read_once(cuda_dev):
     off = torch.tensor([m] * E, device=cuda_dev, dtype=torch.int32)
     assert peak(lambda: M.grouped_linear(x, w, off, bias=b)) < w.numel()
     check(M.grouped_linear(x, w, off, bias=b), x, w[0], b[0], BF)
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float16])
+@pytest.mark.parametrize("m,k,n,E", [(3, 1563, 4951, 0), (4, 2001, 2104, 0), (6, 985, 4908, 2), (47, 3898, 187, 13)])
+def test_gradients_of_odd_rows(cuda_dev, m, k, n, E, dtype):
+    """Rows too few for a copy of the weights in the forward: the same values with and without gradients,
+    and the formula's gradients."""
+    x, w, b, r, dy = test_linear_gpu.make(cuda_dev, m, k, n, dtype, m + k, E=E)
+    g = torch.Generator().manual_seed(m)
+    cuts = torch.sort(torch.randint(0, m + 1, (max(0, E - 1),), generator=g)).values.tolist()
+    off = torch.tensor([0] + cuts + [m], device=cuda_dev, dtype=torch.int32) if E else None
+    for act in ("none", "silu"):
+        test_linear_gpu.run_case(x, w, b, r, dy, act, dtype, offsets=off)
